@@ -5,3 +5,6 @@ from .qgemm import (  # noqa: F401
     QGemmError, block_scaled_gemm, gemm_nvfp4_requant, lib, make_mxfp4, make_mxfp8, make_nvfp4,
     repack_nvfp4, sm1xx_scale_storage_size,
 )
+from .fused import (  # noqa: F401
+    act_backward, gemm_fused, interleave_gate_up, rmsnorm_backward, rmsnorm_mxfp8, transpose_mxfp8,
+)

@@ -22,6 +22,18 @@ namespace qg {
 
 namespace {
 
+bool float_dtype(int d) { return d == QG_DTYPE_F32 || d == QG_DTYPE_BF16; }
+int64_t dtype_bytes(int d) { return d == QG_DTYPE_BF16 ? 2 : 4; }
+bool any_layout(int l) { return l >= QG_LAYOUT_REF_LINEAR && l <= QG_LAYOUT_MMA_KMAJOR; }
+bool mma_layout(int l) { return l == QG_LAYOUT_MMA || l == QG_LAYOUT_MMA_KMAJOR; }
+bool aligned_to(const void* p, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0;
+}
+// A matrix of 16-byte vectors: base and row stride (elements of `dtype`).
+bool vector_rows(const void* p, int64_t ld, int dtype) {
+  return aligned_to(p, 16) && (ld * dtype_bytes(dtype)) % 16 == 0;
+}
+
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -182,10 +194,11 @@ cudaError_t gemm_launch(const PreparedGemm& g, cudaStream_t stream) {
 int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, const void* b_q,
                  const void* b_sf, const float* b_ts, void* c, int c_dtype, int64_t m, int64_t n,
                  int64_t k, int64_t ldc, int sf_layout, uint32_t* status, PreparedGemm* out,
-                 const Gather& gather = Gather(), const Requant& requant = Requant()) {
+                 const Gather& gather = Gather(), const Requant& requant = Requant(),
+                 const EpiParams* epi = nullptr) {
   const bool rq = requant.q != nullptr;
   const bool fp4 = fmt != 0;
-  if (!a_q || !a_sf || !b_q || !b_sf || (!c && !rq)) return QG_ERR_ARG;
+  if (!a_q || !a_sf || !b_q || !b_sf || (!c && !rq && !epi)) return QG_ERR_ARG;
   if (!rq && c_dtype != QG_DTYPE_F32 && c_dtype != QG_DTYPE_BF16) return QG_ERR_DTYPE;
   if (sf_layout != QG_LAYOUT_MMA && sf_layout != QG_LAYOUT_MMA_KMAJOR) return QG_ERR_LAYOUT;
   if (m < 1 || n < 1 || k < 32 || (k % 32) != 0 || ldc < n) return QG_ERR_SHAPE;
@@ -197,7 +210,7 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
   if (int d = check_device()) return d;
   if (!encode_fn()) return QG_ERR_CUDA;
   const int sv = fmt == 1 ? 16 : 32;
-  const int variant = (gather.nranks > 0 || rq || fmt == 2) ? 1 : gemm_variant(fp4, m);
+  const int variant = (gather.nranks > 0 || rq || epi || fmt == 2) ? 1 : gemm_variant(fp4, m);
   const bool pair = variant == 1;
   // Tile of one scheduling unit (a CTA pair: 256 x 256; one CTA: 128 x 256)
   // and the rows each CTA's TMA boxes cover.
@@ -250,6 +263,7 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
     p.rq_row_blocks = static_cast<int>((m + 127) / 128);
     p.rq_sf_blocks = static_cast<int>((n / 16 + 3) / 4);
   }
+  if (epi) p.epi = *epi;
   p.a_ts = fmt == 1 ? a_ts : nullptr;
   p.b_ts = fmt == 1 ? b_ts : nullptr;
   p.status = status;
@@ -266,7 +280,8 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
     if (2 * tiles > (1ll << 31) - 1) return QG_ERR_SHAPE;
     out->grid = 2 * static_cast<int>(tiles);
     // bf16 through TMA stores: the eight-warp epilogue (kind 3).
-    out->out_kind = rq ? 2 : (out->out_bf16 ? (p.n_out > 0 && kPairEpi8 ? 3 : 1) : 0);
+    out->out_kind = epi ? (epi->act == QG_ACT_SWIGLU ? 5 : 4)
+                        : (rq ? 2 : (out->out_bf16 ? (p.n_out > 0 && kPairEpi8 ? 3 : 1) : 0));
   } else {
     out->grid = static_cast<int>(tiles < num_sms() ? tiles : num_sms());
   }
@@ -519,6 +534,219 @@ int qg_gemm_mxfp8(const void* a_q, const void* a_sf, const void* b_q, const void
                   uint32_t* status, qg_stream_t stream) {
   return gemm_common(0, a_q, a_sf, nullptr, b_q, b_sf, nullptr, c, c_dtype, m, n, k, ldc,
                      sf_layout, status, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// ------------------------------------------------------------------ layer operators
+int qg_rmsnorm_mxfp8(const void* x, int x_dtype, int64_t ldx, const void* residual, int64_t ldr,
+                     const void* weight, int w_dtype, float eps, int64_t rows, int64_t k,
+                     int layout, void* q, void* sf, void* h, int64_t ldh, float* rstd,
+                     qg_stream_t stream) {
+  if (!x || !weight || !q || !sf || !(eps >= 0.0f)) return QG_ERR_ARG;
+  if (!float_dtype(x_dtype) || !float_dtype(w_dtype)) return QG_ERR_DTYPE;
+  if (!any_layout(layout)) return QG_ERR_LAYOUT;
+  if (rows < 1 || rows > (1ll << 31) - 256 || k < 32 || k % 32 != 0 || k > kMaxNormK || ldx < k ||
+      (residual && ldr < k) || (h && ldh < k))
+    return QG_ERR_SHAPE;
+  if (!vector_rows(x, ldx, x_dtype) || (residual && !vector_rows(residual, ldr, x_dtype)) ||
+      (h && !vector_rows(h, ldh, x_dtype)) || !aligned16(weight) || !aligned16(q) ||
+      !aligned_to(sf, 4) || !aligned_to(rstd, 4))
+    return QG_ERR_ALIGN;
+  if (int d = check_device()) return d;
+  RmsNormParams p{};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.h = h;
+  p.rstd = rstd;
+  p.q = static_cast<uint8_t*>(q);
+  p.sf = static_cast<uint8_t*>(sf);
+  p.ldx = ldx;
+  p.ldr = ldr;
+  p.ldh = ldh;
+  p.rows = rows;
+  p.k = k;
+  p.row_blocks = (rows + 127) / 128;
+  p.sf_blocks = (k / 32 + 3) / 4;
+  p.layout = layout;
+  p.eps = eps;
+  return launch_rmsnorm_mxfp8(p, x_dtype == QG_DTYPE_BF16, w_dtype == QG_DTYPE_BF16,
+                              reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? QG_OK
+             : QG_ERR_CUDA;
+}
+
+size_t qg_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t k) {
+  if (rows < 1 || k < 1) return 0;
+  return static_cast<size_t>(rmsnorm_backward_parts(rows)) * static_cast<size_t>(k) * 4;
+}
+
+int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, int x_dtype,
+                        const float* rstd, const void* weight, int w_dtype, const void* dres,
+                        int64_t lddres, int64_t rows, int64_t k, void* dx, int64_t lddx,
+                        float* dweight, void* workspace, size_t workspace_bytes,
+                        qg_stream_t stream) {
+  if (!dy || !h || !rstd || !weight || !dx) return QG_ERR_ARG;
+  if (!float_dtype(x_dtype) || !float_dtype(w_dtype)) return QG_ERR_DTYPE;
+  if (rows < 1 || rows > (1ll << 31) - 256 || k < 32 || k % 32 != 0 || k > kMaxNormK ||
+      lddy < k || ldh < k || lddx < k || (dres && lddres < k))
+    return QG_ERR_SHAPE;
+  if (!vector_rows(dy, lddy, x_dtype) || !vector_rows(h, ldh, x_dtype) ||
+      !vector_rows(dx, lddx, x_dtype) || (dres && !vector_rows(dres, lddres, x_dtype)) ||
+      !aligned16(weight) || !aligned_to(rstd, 4) || !aligned_to(dweight, 4))
+    return QG_ERR_ALIGN;
+  if (dweight) {
+    if (!workspace || workspace_bytes < qg_rmsnorm_backward_workspace_bytes(rows, k))
+      return QG_ERR_ARG;
+    if (!aligned16(workspace)) return QG_ERR_ALIGN;
+  }
+  if (int d = check_device()) return d;
+  RmsNormBwdParams p{};
+  p.dy = dy;
+  p.h = h;
+  p.weight = weight;
+  p.dres = dres;
+  p.rstd = rstd;
+  p.dx = dx;
+  p.dw_part = dweight ? static_cast<float*>(workspace) : nullptr;
+  p.lddy = lddy;
+  p.ldh = ldh;
+  p.lddres = lddres;
+  p.lddx = lddx;
+  p.rows = rows;
+  p.k = k;
+  return launch_rmsnorm_backward(p, x_dtype == QG_DTYPE_BF16, w_dtype == QG_DTYPE_BF16, dweight,
+                                 reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? QG_OK
+             : QG_ERR_CUDA;
+}
+
+int qg_gemm_fused(int format, const void* a_q, const void* a_sf, const float* a_ts,
+                  const void* b_q, const void* b_sf, const float* b_ts, int64_t m, int64_t n,
+                  int64_t k, int sf_layout, const qg_epilogue* epilogue, uint32_t* status,
+                  qg_stream_t stream) {
+  if (!epilogue || !epilogue->out) return QG_ERR_ARG;
+  const qg_epilogue& u = *epilogue;
+  if (format < QG_FORMAT_MXFP8 || format > QG_FORMAT_MXFP4) return QG_ERR_DTYPE;
+  if (u.act < QG_ACT_NONE || u.act > QG_ACT_SWIGLU) return QG_ERR_ARG;
+  const bool gated = u.act == QG_ACT_SWIGLU, mx = u.out_dtype == QG_DTYPE_MXFP8;
+  if ((!mx && !float_dtype(u.out_dtype)) || (u.bias && !float_dtype(u.bias_dtype)) ||
+      (u.residual && !float_dtype(u.residual_dtype)))
+    return QG_ERR_DTYPE;
+  if ((mx && !u.out_sf) || (u.ckpt_q && !u.ckpt_sf)) return QG_ERR_ARG;
+  if ((mx && !any_layout(u.out_layout)) || (u.ckpt_q && !any_layout(u.ckpt_layout)))
+    return QG_ERR_LAYOUT;
+  const int64_t n_out = gated ? n / 2 : n;
+  if (m < 1 || n < 1 || m > (1ll << 31) - 256 || n > (1ll << 31) - 256 ||
+      (gated && n % (2 * 128) != 0) || ((mx || u.ckpt_q) && n % 32 != 0) ||
+      (!mx && u.ldc < n_out) || (u.residual && u.ldr < n_out))
+    return QG_ERR_SHAPE;
+  if ((mx && (!aligned16(u.out) || !aligned16(u.out_sf))) ||
+      (!mx && !aligned_to(u.out, dtype_bytes(u.out_dtype))) ||
+      (u.ckpt_q && (!aligned16(u.ckpt_q) || !aligned16(u.ckpt_sf))) ||
+      (u.bias && !aligned_to(u.bias, dtype_bytes(u.bias_dtype))) ||
+      (u.residual && !aligned_to(u.residual, dtype_bytes(u.residual_dtype))))
+    return QG_ERR_ALIGN;
+  EpiParams e{};
+  e.act = u.act;
+  e.bias = u.bias;
+  e.bias_bf16 = u.bias_dtype == QG_DTYPE_BF16;
+  e.res = u.residual;
+  e.ldr = u.ldr;
+  e.res_bf16 = u.residual_dtype == QG_DTYPE_BF16;
+  e.res_vec = u.residual && vector_rows(u.residual, u.ldr, u.residual_dtype);
+  e.out_kind = mx ? kEpiMxfp8 : (u.out_dtype == QG_DTYPE_BF16 ? kEpiBf16 : kEpiF32);
+  e.out_vec = !mx && vector_rows(u.out, u.ldc, u.out_dtype);
+  e.out = u.out;
+  e.ldc = u.ldc;
+  e.out_sf = static_cast<uint8_t*>(u.out_sf);
+  e.out_layout = u.out_layout;
+  e.row_blocks = static_cast<int>((m + 127) / 128);
+  e.out_sf_blocks = static_cast<int>((n_out / 32 + 3) / 4);
+  e.z_sf_blocks = static_cast<int>((n / 32 + 3) / 4);
+  e.z_q = static_cast<uint8_t*>(u.ckpt_q);
+  e.z_sf = static_cast<uint8_t*>(u.ckpt_sf);
+  e.z_layout = u.ckpt_layout;
+  PreparedGemm g;
+  const int rc = gemm_prepare(format, a_q, a_sf, a_ts, b_q, b_sf, b_ts, nullptr, QG_DTYPE_F32, m,
+                              n, k, n, sf_layout, status, &g, Gather(), Requant(), &e);
+  if (rc != QG_OK) return rc;
+  return gemm_launch(g, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? QG_OK
+                                                                               : QG_ERR_CUDA;
+}
+
+size_t qg_act_backward_workspace_bytes(int64_t m, int64_t n) {
+  if (m < 1 || n < 1) return 0;
+  return static_cast<size_t>((m + 127) / 128) * static_cast<size_t>(n) * 4;
+}
+
+int qg_act_backward_mxfp8(const void* dout, int dout_dtype, int64_t ldd, const void* z_q,
+                          const void* z_sf, int z_layout, int act, int64_t m, int64_t n,
+                          void* dz_q, void* dz_sf, void* dzt_q, void* dzt_sf, int out_layout,
+                          float* dbias, void* workspace, size_t workspace_bytes,
+                          qg_stream_t stream) {
+  if (act < QG_ACT_NONE || act > QG_ACT_SWIGLU) return QG_ERR_ARG;
+  const bool z = act != QG_ACT_NONE, gated = act == QG_ACT_SWIGLU;
+  if (!dout || (z && (!z_q || !z_sf)) || !dz_q || !dz_sf || !dzt_q || !dzt_sf) return QG_ERR_ARG;
+  if (!float_dtype(dout_dtype)) return QG_ERR_DTYPE;
+  if ((z && !any_layout(z_layout)) || !mma_layout(out_layout)) return QG_ERR_LAYOUT;
+  if (m < 1 || n < 32 || n % 32 != 0 || (gated && n % 256 != 0) || ldd < (gated ? n / 2 : n) ||
+      m > (1ll << 31) - 256 || n > (1ll << 31) - 256 ||
+      ((m + 127) / 128) * ((n + 127) / 128) > (1ll << 31) - 1)
+    return QG_ERR_SHAPE;
+  if (!vector_rows(dout, ldd, dout_dtype) || (z && !aligned16(z_q)) || !aligned16(dz_q) ||
+      !aligned16(dz_sf) || !aligned16(dzt_q) || !aligned16(dzt_sf) || !aligned_to(dbias, 4))
+    return QG_ERR_ALIGN;
+  if (dbias) {
+    if (!workspace || workspace_bytes < qg_act_backward_workspace_bytes(m, n)) return QG_ERR_ARG;
+    if (!aligned16(workspace)) return QG_ERR_ALIGN;
+  }
+  if (int d = check_device()) return d;
+  ActBackwardParams p{};
+  p.dout = dout;
+  p.ldd = ldd;
+  p.z_q = static_cast<const uint8_t*>(z_q);
+  p.z_sf = static_cast<const uint8_t*>(z_sf);
+  p.z_layout = z_layout;
+  p.m = m;
+  p.n = n;
+  p.dz_q = static_cast<uint8_t*>(dz_q);
+  p.dz_sf = static_cast<uint8_t*>(dz_sf);
+  p.dzt_q = static_cast<uint8_t*>(dzt_q);
+  p.dzt_sf = static_cast<uint8_t*>(dzt_sf);
+  p.mt = (m + 31) / 32 * 32;
+  p.out_layout = out_layout;
+  p.dbias_part = dbias ? static_cast<float*>(workspace) : nullptr;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (launch_act_backward(p, act, dout_dtype == QG_DTYPE_BF16, s) != cudaSuccess)
+    return QG_ERR_CUDA;
+  if (dbias && launch_column_sum(p.dbias_part, static_cast<int>((m + 127) / 128), n, dbias, s) !=
+                   cudaSuccess)
+    return QG_ERR_CUDA;
+  return QG_OK;
+}
+
+int qg_transpose_mxfp8(const void* q, const void* sf, int layout, int64_t rows, int64_t k,
+                       void* tq, void* tsf, int out_layout, qg_stream_t stream) {
+  if (!q || !sf || !tq || !tsf) return QG_ERR_ARG;
+  if (!any_layout(layout) || !mma_layout(out_layout)) return QG_ERR_LAYOUT;
+  if (rows < 1 || k < 32 || k % 32 != 0 || rows > (1ll << 31) - 256 || k > (1ll << 31) - 256 ||
+      ((rows + 127) / 128) * ((k + 127) / 128) > (1ll << 31) - 1)
+    return QG_ERR_SHAPE;
+  if (!aligned16(q) || !aligned16(tq) || !aligned16(tsf)) return QG_ERR_ALIGN;
+  if (int d = check_device()) return d;
+  ActBackwardParams p{};
+  p.z_q = static_cast<const uint8_t*>(q);
+  p.z_sf = static_cast<const uint8_t*>(sf);
+  p.z_layout = layout;
+  p.m = rows;
+  p.n = k;
+  p.dzt_q = static_cast<uint8_t*>(tq);
+  p.dzt_sf = static_cast<uint8_t*>(tsf);
+  p.mt = (rows + 31) / 32 * 32;
+  p.out_layout = out_layout;
+  return launch_transpose_mxfp8(p, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? QG_OK
+             : QG_ERR_CUDA;
 }
 
 // Decode GEMM on CTA pairs for m in (32, 128] at the decode shapes (a build

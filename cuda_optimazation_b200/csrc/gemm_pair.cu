@@ -42,6 +42,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include "gemm_epilogue.cuh"
 #include "qg_codec.cuh"
 #include "qg_gemm.h"
 #include "qg_ptx.cuh"
@@ -218,9 +219,12 @@ __device__ __forceinline__ void tile_coords(int tile, int num_m_tiles, int num_n
 // kOut: 0 fp32 C, 1 bf16 C, 2 NVFP4 output (values + e4m3 block scales,
 // requantised in the epilogue as the reference's tc6 store_tile does,
 // GEMMsm110/include/backends/tc6_nvfp4.cuh:460-503).
-// Threads per CTA: 11 warps; the NVFP4-output epilogue (kOut 2) and the
-// bf16 TMA-store epilogue (kOut 3) add four more epilogue warps (11..14, one
-// per TMEM lane quadrant).
+// 3: bf16 C through TMA stores.  4: the fused epilogue (bias, activation,
+// residual, MXFP8 checkpoint; gemm_epilogue.cuh), 5: the same with the gated
+// activation, whose gate columns are a tile's first 128 and factors its last.
+// Threads per CTA: 11 warps; the NVFP4-output epilogue (kOut 2), the
+// bf16 TMA-store epilogue (kOut 3) and the fused ones add four more epilogue
+// warps (11..14, one per TMEM lane quadrant).
 template <int kOut>
 constexpr int pair_threads() {
   return kOut >= 2 ? 480 : 352;
@@ -770,6 +774,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
               if (col0 + 16 * g < p.n) p.rq_sf[so + g] = static_cast<uint8_t>(sbits[g]);
           }
         }
+      } else if constexpr (kOut >= 4) {
+        // Fused epilogue: 32 columns of a row at a time.  The two warps of a
+        // TMEM lane quadrant take the 64-column blocks {sub, 2 + sub}, which
+        // for the gated form are a gate block and its factors.
+        static_assert(Cfg::kIssuers == 1 || kOut < 4, "one issuer: TMEM column = tile column");
+        const int sub = warp >= 11 ? 1 : 0;
+        auto release = [&]() {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader0);
+        };
+        if constexpr (kOut == 4) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int tcol = (c / 2 * 2 + sub) * 64 + (c & 1) * 32;
+            uint32_t r[32];
+            __syncwarp();
+            tmem_ld_32x32b_x32(t_row + tcol, r);
+            tmem_wait_ld();
+            if (c == 3) release();
+            float z[32];
+            epi_affine(p.epi, r, alpha, n0 + tcol, p.n, lane, z);
+            epi_checkpoint(p.epi, z, row, n0 + tcol, p.m, p.n);
+            epi_act(p.epi.act, z);
+            epi_finish(p.epi, z, row, n0 + tcol, p.m, p.n);
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            const int tcol = sub * 64 + c * 32;
+            uint32_t r[32], f[32];
+            __syncwarp();
+            tmem_ld_32x32b_x32(t_row + tcol, r);
+            tmem_ld_32x32b_x32(t_row + kGateCols + tcol, f);
+            tmem_wait_ld();
+            if (c == 1) release();
+            float z[32], u[32];
+            epi_affine(p.epi, r, alpha, n0 + tcol, p.n, lane, z);
+            epi_checkpoint(p.epi, z, row, n0 + tcol, p.m, p.n);
+            epi_affine(p.epi, f, alpha, n0 + kGateCols + tcol, p.n, lane, u);
+            epi_checkpoint(p.epi, u, row, n0 + kGateCols + tcol, p.m, p.n);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[j] = act_fwd<kActSilu>(z[j]) * u[j];
+            epi_finish(p.epi, z, row, n0 / 2 + tcol, p.m, p.n / 2);
+          }
+        }
       } else if constexpr (kOut == 3) {
         // bf16 through TMA stores with eight epilogue warps (2-5, 11-14; two
         // per TMEM lane quadrant); a warp owns TMEM blocks `sub` and
@@ -997,6 +1047,17 @@ static cudaError_t launch_pair_one(const GemmParams& p, int grid, cudaStream_t s
 
 cudaError_t launch_gemm_pair(const GemmParams& p, int fmt, int out_kind, int grid,
                              cudaStream_t stream) {
+  if (out_kind >= 4) {
+    const bool gated = out_kind == 5;
+    if (fmt == kFmtNvfp4)
+      return gated ? launch_pair_one<kFmtNvfp4, 5>(p, grid, stream)
+                   : launch_pair_one<kFmtNvfp4, 4>(p, grid, stream);
+    if (fmt == kFmtMxfp4)
+      return gated ? launch_pair_one<kFmtMxfp4, 5>(p, grid, stream)
+                   : launch_pair_one<kFmtMxfp4, 4>(p, grid, stream);
+    return gated ? launch_pair_one<kFmtMxfp8, 5>(p, grid, stream)
+                 : launch_pair_one<kFmtMxfp8, 4>(p, grid, stream);
+  }
   if (fmt == kFmtNvfp4) {
     if (out_kind == 3) return launch_pair_one<kFmtNvfp4, 3>(p, grid, stream);
     if (out_kind == 2) return launch_pair_one<kFmtNvfp4, 2>(p, grid, stream);

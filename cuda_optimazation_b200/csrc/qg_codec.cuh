@@ -1,8 +1,10 @@
 // qg_codec.cuh -- NVFP4 element / scale codecs and vector loads shared by the
-// activation quantizers (quantize.cu, gemm_skinny.cu).  Rounding follows
+// activation quantizers (quantize.cu, gemm_skinny.cu), and the MXFP8 rule shared
+// with the layer operators.  Rounding follows
 // make_nvfp4_reference (GEMMsm110/include/requant/nvfp4_reference.cuh:76-112).
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -51,6 +53,47 @@ __device__ __forceinline__ int64_t mma_scale_offset(int64_t row, int64_t sfc, in
   const int64_t br = row >> 7, bs = sfc >> 2, w = row & 127;
   const int64_t chunk = (layout == 1) ? bs * row_blocks + br : br * sf_blocks + bs;
   return chunk * 512 + (w & 31) * 16 + (w >> 5) * 4 + (sfc & 3);
+}
+
+// ------------------------------------------------------------------ MXFP8
+__device__ __forceinline__ int floor_log2_positive(float a) {
+  const uint32_t b = __float_as_uint(a);
+  const int e = static_cast<int>((b >> 23) & 0xffu);
+  if (e != 0) return e - 127;
+  return -149 + (31 - __clz(static_cast<int>(b & 0x7fffffu)));
+}
+
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float d) {
+  return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16);
+}
+
+// ue8m0 code of a block with largest magnitude `amax` (the MXFP8 quantizer's
+// rule: exponent floor(log2 amax) - 8 clamped at -127, 0 for a zero block), and
+// the reciprocal 2^-e of the scale it stands for.  Exponents stay below 121,
+// so the reciprocal is a normal number.
+__device__ __forceinline__ uint32_t mxfp8_scale_code(float amax, float& mul) {
+  const int e = amax > 0.0f ? max(-127, floor_log2_positive(amax) - 8) : -127;
+  mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  return static_cast<uint32_t>(e + 127);
+}
+
+// The scale 2^(code - 127) that a ue8m0 code stands for (code 0: 2^-127, a
+// subnormal; code 255 would be NaN and is never written here).
+__device__ __forceinline__ float e8m0_decode(uint32_t code) {
+  return __uint_as_float(code ? (code == 255u ? 0x7fc00000u : code << 23) : 0x00400000u);
+}
+
+// Two e4m3 bytes -> two floats (exact: every e4m3 value is an f16 value).
+__device__ __forceinline__ float2 e4m3x2_decode(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 
 template <bool kBf16>

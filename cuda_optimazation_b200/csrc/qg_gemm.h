@@ -26,6 +26,28 @@ constexpr int kMaxDevices = 64;
 #endif
 constexpr uint32_t kDiag = QG_DIAG_FLAGS;
 
+// Fused epilogue of the GEMM (gemm_epilogue.cuh): out = act(alpha A B^T + bias)
+// + residual.  The output has n columns, n / 2 for the gated activation.
+enum : int { kEpiF32 = 0, kEpiBf16 = 1, kEpiMxfp8 = 2 };
+struct EpiParams {
+  int act;          // kAct* (qg_act.cuh)
+  int bias_bf16;
+  const void* bias;  // [n], may be null
+  const void* res;   // residual, may be null
+  int64_t ldr;
+  int res_bf16, res_vec;  // *_vec: 16-byte accesses are legal for every full 32-column run
+  int out_kind, out_vec;
+  void* out;        // fp32 / bf16 rows with stride ldc, or e4m3 values, dense
+  int64_t ldc;
+  uint8_t* out_sf;
+  int out_layout;
+  int row_blocks;   // 128-row blocks of the output and the checkpoint
+  int out_sf_blocks, z_sf_blocks;
+  uint8_t* z_q;     // MXFP8 checkpoint of z = alpha A B^T + bias, may be null
+  uint8_t* z_sf;
+  int z_layout;
+};
+
 struct GemmParams {
   CUtensorMap tm_a;    // uint8 [rows][K bytes], box 128 B x kBM, SWIZZLE_128B
   CUtensorMap tm_b;    // uint8 [rows][K bytes], box 128 B x kBN, SWIZZLE_128B
@@ -57,6 +79,7 @@ struct GemmParams {
   int rq_row_blocks, rq_sf_blocks;
   uint32_t* status;
   uint64_t timeout_ns;
+  EpiParams epi;  // out_kind 4 / 5 of launch_gemm_pair
 };
 
 // Decode-shaped NVFP4 GEMM (gemm_skinny.cu): weights W [n][k] on the MMA's M
@@ -115,7 +138,7 @@ cudaError_t launch_gemm_blockscaled(const GemmParams& p, bool fp4, bool out_bf16
                                     cudaStream_t stream);
 // fmt: 0 MXFP8, 1 NVFP4, 2 MXFP4.  out_kind: 0 fp32 C, 1 bf16 C, 2 NVFP4
 // output (rq_* fields; NVFP4 only), 3 bf16 C through TMA stores (n_out > 0)
-// with eight epilogue warps.
+// with eight epilogue warps, 4 the fused epilogue (epi), 5 its gated form.
 cudaError_t launch_gemm_pair(const GemmParams& p, int fmt, int out_kind, int grid,
                              cudaStream_t stream);
 int pair_sf_chunks_per_stage(int fmt);
@@ -147,6 +170,65 @@ cudaError_t launch_repack_mx(bool fp4, const uint8_t* sq, const uint8_t* ssf, in
 cudaError_t launch_e2m1_cvt_selftest(unsigned long long* out, cudaStream_t stream);
 cudaError_t launch_wait_timeout_selftest(uint64_t timeout_ns, uint32_t* status,
                                          cudaStream_t stream);
+
+// RMS norm with residual addition and MXFP8 output, and its gradient
+// (rmsnorm.cu).  Strides in elements; k a multiple of 32, at most kMaxNormK.
+constexpr int64_t kMaxNormK = 32768;
+struct RmsNormParams {
+  const void* x;
+  const void* residual;  // may be null: h = x
+  const void* weight;
+  void* h;               // may be null
+  float* rstd;           // may be null
+  uint8_t* q;            // [rows][k]
+  uint8_t* sf;
+  int64_t ldx, ldr, ldh;
+  int64_t rows, k;
+  int64_t row_blocks, sf_blocks;
+  int layout;
+  float eps;
+};
+struct RmsNormBwdParams {
+  const void* dy;
+  const void* h;
+  const void* weight;
+  const void* dres;  // may be null
+  const float* rstd;
+  void* dx;
+  float* dw_part;    // [rmsnorm_backward_parts(rows)][k]; null: no dw
+  int64_t lddy, ldh, lddres, lddx;
+  int64_t rows, k;
+};
+cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
+                                 cudaStream_t stream);
+int rmsnorm_backward_parts(int64_t rows);
+cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16, float* dw,
+                                    cudaStream_t stream);
+// out[c] = sum over r < parts of part[r][c], in a fixed order.
+cudaError_t launch_column_sum(const float* part, int parts, int64_t k, float* out,
+                              cudaStream_t stream);
+
+// Backward of an activation from its MXFP8 checkpoint, and the transposition of
+// an MXFP8 matrix (act_backward.cu).
+struct ActBackwardParams {
+  const void* dout;      // [m][n], or [m][n / 2] for the gated activation
+  int64_t ldd;
+  const uint8_t* z_q;    // [m][n]; unused for act none: dz = dout
+  const uint8_t* z_sf;
+  int z_layout;
+  int64_t m, n;
+  uint8_t* dz_q;         // [m][n] (unused by the transposition)
+  uint8_t* dz_sf;
+  uint8_t* dzt_q;        // [n][mt]
+  uint8_t* dzt_sf;
+  int64_t mt;            // m rounded up to 32
+  int out_layout;
+  float* dbias_part;     // [ceil(m / 128)][n]; null: no dbias
+};
+cudaError_t launch_act_backward(const ActBackwardParams& p, int act, bool bf16,
+                                cudaStream_t stream);
+// dzt = z turned (dout, dz and dbias unused).
+cudaError_t launch_transpose_mxfp8(const ActBackwardParams& p, cudaStream_t stream);
 
 int num_sms();
 

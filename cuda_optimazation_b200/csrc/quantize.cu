@@ -114,19 +114,6 @@ __global__ void __launch_bounds__(256)
 // ------------------------------------------------------------------ MXFP8
 // One thread per 32-element block: ue8m0 exponent floor(log2(amax)) - 8,
 // elements RN-satfinite e4m3 of x * 2^-e.
-__device__ __forceinline__ int floor_log2_positive(float a) {
-  const uint32_t b = __float_as_uint(a);
-  const int e = static_cast<int>((b >> 23) & 0xffu);
-  if (e != 0) return e - 127;
-  return -149 + (31 - __clz(static_cast<int>(b & 0x7fffffu)));
-}
-
-__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 template <bool kBf16>
 __global__ void __launch_bounds__(256)
     mxfp8_quantize_kernel(const void* x, int64_t rows, int64_t k, int layout, uint8_t* q,

@@ -29,13 +29,16 @@ LIB_PATH = _PKG / "libqgemm_b200.so"
 # qg_status
 OK, ERR_SHAPE, ERR_ALIGN, ERR_LAYOUT, ERR_DTYPE, ERR_CUDA, ERR_TIMEOUT, ERR_ARG, ERR_UNSUPPORTED = range(9)
 # qg_dtype
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_MXFP8 = 0, 1, 2
 # qg_layout
 LAYOUT_REF_LINEAR, LAYOUT_MMA, LAYOUT_MMA_KMAJOR = 0, 1, 2
+# qg_act
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_SWIGLU = range(5)
 # qg_format
 FORMAT_MXFP8, FORMAT_NVFP4, FORMAT_MXFP4 = 0, 1, 2
 
 _VP, _I64, _I32, _U64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint64
+_SZ, _F32 = ctypes.c_size_t, ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/qgemm.h one to one.
 SIGNATURES = {
@@ -71,9 +74,30 @@ SIGNATURES = {
                                    _I64, _I64, _I64, _I32, _VP]),
     "qg_plan_run": (_I32, [_VP, _VP]),
     "qg_plan_destroy": (_I32, [_VP]),
+    "qg_rmsnorm_mxfp8": (_I32, [_VP, _I32, _I64, _VP, _I64, _VP, _I32, _F32, _I64, _I64, _I32,
+                                _VP, _VP, _VP, _I64, _VP, _VP]),
+    "qg_rmsnorm_backward": (_I32, [_VP, _I64, _VP, _I64, _I32, _VP, _VP, _I32, _VP, _I64, _I64,
+                                   _I64, _VP, _I64, _VP, _VP, _SZ, _VP]),
+    "qg_rmsnorm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "qg_gemm_fused": (_I32, [_I32, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I32, _VP, _VP,
+                             _VP]),
+    "qg_act_backward_mxfp8": (_I32, [_VP, _I32, _I64, _VP, _VP, _I32, _I32, _I64, _I64, _VP, _VP,
+                                     _VP, _VP, _I32, _VP, _VP, _SZ, _VP]),
+    "qg_act_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "qg_transpose_mxfp8": (_I32, [_VP, _VP, _I32, _I64, _I64, _VP, _VP, _I32, _VP]),
     "qg_selftest_e2m1_cvt": (_I32, [_VP, _VP]),
     "qg_selftest_wait_timeout": (_I32, [_U64, _VP, _VP]),
 }
+
+
+
+class Epilogue(ctypes.Structure):
+    """qg_epilogue, field by field."""
+    _fields_ = [("act", _I32), ("bias_dtype", _I32), ("bias", _VP), ("residual", _VP),
+                ("ldr", _I64), ("residual_dtype", _I32), ("out_dtype", _I32), ("out", _VP),
+                ("ldc", _I64), ("out_sf", _VP), ("ckpt_q", _VP), ("ckpt_sf", _VP),
+                ("out_layout", _I32), ("ckpt_layout", _I32)]
+
 
 _lib: Optional[ctypes.CDLL] = None
 

@@ -44,7 +44,9 @@ typedef enum {
   QG_ERR_UNSUPPORTED = 8  /* device is not sm_100                           */
 } qg_status;
 
-typedef enum { QG_DTYPE_F32 = 0, QG_DTYPE_BF16 = 1 } qg_dtype;
+/* QG_DTYPE_MXFP8 names the quantised output of qg_gemm_fused; no entry point
+ * takes it for an input. */
+typedef enum { QG_DTYPE_F32 = 0, QG_DTYPE_BF16 = 1, QG_DTYPE_MXFP8 = 2 } qg_dtype;
 
 /* Operand layouts.
  *  QG_LAYOUT_REF_LINEAR : the reference quantizer's byte order
@@ -267,6 +269,113 @@ int qg_gemm_nvfp4_skinny(const void* x, int x_dtype, int64_t m, const void* w_q,
 
 /* Workspace bytes qg_gemm_nvfp4_skinny needs. */
 size_t qg_gemm_nvfp4_skinny_workspace_bytes(int64_t m, int64_t n, int64_t k);
+
+/* ---- Layer operators around the block-scaled GEMM -----------------------
+ * What a transformer layer computes next to its products, writing and reading
+ * the operands that the products use.  Row strides (ld*) are in elements; the
+ * matrices they belong to start 16-byte aligned with rows that are a multiple
+ * of 16 bytes apart, except where an entry point says otherwise.  All sums
+ * are fp32; every output is rounded once.  No reference counterpart. */
+
+/* RMS norm with the residual's addition and MXFP8 output: for every row of
+ * k values, h = x + residual (residual NULL: h = x),
+ *   rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * weight,
+ * with y quantised by qg_quantize_mxfp8's rule into q (rows * k bytes) and sf
+ * (layout as there; scale padding of the MMA layouts is written as zero).
+ * x, residual and h have x_dtype, weight (k values) w_dtype.  h (the sum,
+ * rounded to x_dtype; y is formed from the unrounded sum) and rstd (rows
+ * floats) may be NULL.  h may be x or residual itself.
+ * k % 32 == 0, 32 <= k <= 32768, eps >= 0. */
+int qg_rmsnorm_mxfp8(const void* x, int x_dtype, int64_t ldx, const void* residual, int64_t ldr,
+                     const void* weight, int w_dtype, float eps, int64_t rows, int64_t k,
+                     int layout, void* q, void* sf, void* h, int64_t ldh, float* rstd,
+                     qg_stream_t stream);
+
+/* Gradient of qg_rmsnorm_mxfp8, the quantisation passed straight through: with
+ * dy the gradient of y, xh = h * rstd and g = dy * weight,
+ *   dx = rstd * (g - xh * mean(g * xh)) + dres,   dweight = sum_rows dy * xh.
+ * dy, h, dres (NULL: none) and dx have x_dtype; dx is the gradient of x and of
+ * the residual alike.  dweight (k floats) may be NULL, and workspace with it.
+ * dx may be dy or dres itself.  Deterministic: sums run in a fixed order. */
+int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, int x_dtype,
+                        const float* rstd, const void* weight, int w_dtype, const void* dres,
+                        int64_t lddres, int64_t rows, int64_t k, void* dx, int64_t lddx,
+                        float* dweight, void* workspace, size_t workspace_bytes,
+                        qg_stream_t stream);
+
+/* Workspace bytes qg_rmsnorm_backward needs for dweight. */
+size_t qg_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t k);
+
+/* Activations: gelu is the tanh form, relu's slope at 0 is 0.  QG_ACT_SWIGLU gates: of every 256
+ * columns of z the first 128 are gates g, the next 128 their factors u, and
+ * the output's 128 columns are silu(g) * u (n % 256 == 0). */
+typedef enum {
+  QG_ACT_NONE = 0,
+  QG_ACT_RELU = 1,
+  QG_ACT_SILU = 2,
+  QG_ACT_GELU = 3,
+  QG_ACT_SWIGLU = 4
+} qg_act;
+
+/* Epilogue of qg_gemm_fused.  bias: n values; residual and out: m rows of
+ * n (QG_ACT_SWIGLU: n / 2) columns, any alignment of their type.  out_dtype
+ * QG_DTYPE_MXFP8: out receives dense e4m3 values (columns % 32 == 0) and out_sf
+ * their scales in out_layout (ldc unused).  ckpt_q (NULL: none) and ckpt_sf
+ * receive z in MXFP8 (m x n, ckpt_layout, n % 32 == 0), for
+ * qg_act_backward_mxfp8.  MXFP8 buffers are 16-byte aligned.  residual may be
+ * out itself. */
+typedef struct {
+  int act; /* qg_act */
+  int bias_dtype;
+  const void* bias; /* may be NULL */
+  const void* residual; /* may be NULL */
+  int64_t ldr;
+  int residual_dtype;
+  int out_dtype;
+  void* out;
+  int64_t ldc;
+  void* out_sf;
+  void* ckpt_q;
+  void* ckpt_sf;
+  int out_layout;
+  int ckpt_layout;
+} qg_epilogue;
+
+/* Block-scaled GEMM with bias, activation and residual in its epilogue:
+ *   z = a_ts b_ts A . B^T + bias,   out = act(z) + residual.
+ * format, operands and rules as qg_plan_create_gemm / qg_gemm_*. */
+int qg_gemm_fused(int format, const void* a_q, const void* a_sf, const float* a_ts,
+                  const void* b_q, const void* b_sf, const float* b_ts, int64_t m, int64_t n,
+                  int64_t k, int sf_layout, const qg_epilogue* epilogue, uint32_t* status,
+                  qg_stream_t stream);
+
+/* Backward of an activation from the MXFP8 checkpoint z (m x n, z_layout) of
+ * its input: dz = dout * act'(z) for dout (m rows of n, or n / 2 for
+ * QG_ACT_SWIGLU, dtype dout_dtype), written
+ *   - to dz_q / dz_sf as MXFP8 (m x n, scales along n): the A operand of the
+ *     input gradient dz . W;
+ *   - to dzt_q / dzt_sf turned, as MXFP8 (n x mt, scales along m, mt = m rounded
+ *     up to 32, the columns beyond m zero): the A operand of the weight
+ *     gradient dz^T . x;
+ *   - dbias (n floats, NULL: none): the column sums of dz.
+ * Scales in out_layout, an MMA layout.  With QG_ACT_NONE z_q and z_sf may be
+ * NULL.  n % 32 == 0.  workspace: qg_act_backward_workspace_bytes bytes (0, and
+ * NULL, without dbias).  Deterministic. */
+int qg_act_backward_mxfp8(const void* dout, int dout_dtype, int64_t ldd, const void* z_q,
+                          const void* z_sf, int z_layout, int act, int64_t m, int64_t n,
+                          void* dz_q, void* dz_sf, void* dzt_q, void* dzt_sf, int out_layout,
+                          float* dbias, void* workspace, size_t workspace_bytes,
+                          qg_stream_t stream);
+
+/* Workspace bytes qg_act_backward_mxfp8 needs for dbias. */
+size_t qg_act_backward_workspace_bytes(int64_t m, int64_t n);
+
+/* An MXFP8 matrix (rows x k, k % 32 == 0, any layout) turned: k x rt with rt =
+ * rows rounded up to 32 (zeros beyond), its values requantised with scales
+ * along rows, in out_layout (an MMA layout): the operand of a weight gradient
+ * from an 8-bit activation kept from the forward pass. */
+int qg_transpose_mxfp8(const void* q, const void* sf, int layout, int64_t rows, int64_t k,
+                       void* tq, void* tsf, int out_layout, qg_stream_t stream);
 
 /* ---- Column-parallel GEMM with the output all-gather fused in ----------
  * BASELINE config 5 shards B along N over the GPUs of one box

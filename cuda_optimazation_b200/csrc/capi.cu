@@ -577,7 +577,8 @@ int qg_rmsnorm_mxfp8(const void* x, int x_dtype, int64_t ldx, const void* residu
 
 size_t qg_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t k) {
   if (rows < 1 || k < 1) return 0;
-  return static_cast<size_t>(rmsnorm_backward_parts(rows)) * static_cast<size_t>(k) * 4;
+  // Every CTA's share of dweight, whatever the types and strides of a call.
+  return static_cast<size_t>(rmsnorm_backward_parts(rows, k)) * static_cast<size_t>(k) * 4;
 }
 
 int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, int x_dtype,
@@ -693,7 +694,9 @@ int qg_act_backward_mxfp8(const void* dout, int dout_dtype, int64_t ldd, const v
       m > (1ll << 31) - 256 || n > (1ll << 31) - 256 ||
       ((m + 127) / 128) * ((n + 127) / 128) > (1ll << 31) - 1)
     return QG_ERR_SHAPE;
-  if (!vector_rows(dout, ldd, dout_dtype) || (z && !aligned16(z_q)) || !aligned16(dz_q) ||
+  if (!vector_rows(dout, ldd, dout_dtype) ||
+      (z && (!aligned16(z_q) || (z_layout != QG_LAYOUT_REF_LINEAR && !aligned16(z_sf)))) ||
+      !aligned16(dz_q) ||
       !aligned16(dz_sf) || !aligned16(dzt_q) || !aligned16(dzt_sf) || !aligned_to(dbias, 4))
     return QG_ERR_ALIGN;
   if (dbias) {
@@ -715,12 +718,13 @@ int qg_act_backward_mxfp8(const void* dout, int dout_dtype, int64_t ldd, const v
   p.dzt_sf = static_cast<uint8_t*>(dzt_sf);
   p.mt = (m + 31) / 32 * 32;
   p.out_layout = out_layout;
-  p.dbias_part = dbias ? static_cast<float*>(workspace) : nullptr;
+  const int parts = static_cast<int>((m + 127) / 128);  // one row tile: its sums are dbias
+  p.dbias_part = dbias ? (parts > 1 ? static_cast<float*>(workspace) : dbias) : nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (launch_act_backward(p, act, dout_dtype == QG_DTYPE_BF16, s) != cudaSuccess)
     return QG_ERR_CUDA;
-  if (dbias && launch_column_sum(p.dbias_part, static_cast<int>((m + 127) / 128), n, dbias, s) !=
-                   cudaSuccess)
+  if (dbias && parts > 1 &&
+      launch_column_sum(p.dbias_part, parts, n, dbias, s) != cudaSuccess)
     return QG_ERR_CUDA;
   return QG_OK;
 }
@@ -732,7 +736,9 @@ int qg_transpose_mxfp8(const void* q, const void* sf, int layout, int64_t rows, 
   if (rows < 1 || k < 32 || k % 32 != 0 || rows > (1ll << 31) - 256 || k > (1ll << 31) - 256 ||
       ((rows + 127) / 128) * ((k + 127) / 128) > (1ll << 31) - 1)
     return QG_ERR_SHAPE;
-  if (!aligned16(q) || !aligned16(tq) || !aligned16(tsf)) return QG_ERR_ALIGN;
+  if (!aligned16(q) || (layout != QG_LAYOUT_REF_LINEAR && !aligned16(sf)) || !aligned16(tq) ||
+      !aligned16(tsf))
+    return QG_ERR_ALIGN;
   if (int d = check_device()) return d;
   ActBackwardParams p{};
   p.z_q = static_cast<const uint8_t*>(q);

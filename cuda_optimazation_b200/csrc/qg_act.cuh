@@ -6,10 +6,13 @@
 //              (1 + tanh(v/2)) / 2 = p(v), without its cancellation at z < 0)
 //   gelu'(z) = p (1 + z (1 - p) v'(z))
 //   swiglu(g, u) = silu(g) u
-// exp and the quotient are CUDA's fast forms (2 ulp each); the denominators lie
-// in [1, inf], where an infinite one gives 0 as the limit does.
+// exp2 and the reciprocal are the hardware's approximations (good to about
+// 2^-22 and 1 ulp); the denominators lie in [1, inf], where an infinite one
+// gives 0 as the limit does.
 #pragma once
 #include <cuda_runtime.h>
+
+#include "qg_codec.cuh"
 
 namespace qg {
 
@@ -21,8 +24,11 @@ constexpr int kGateCols = 128;
 constexpr float kGeluC = 1.5957691216057308f;   // 2 sqrt(2 / pi)
 constexpr float kGeluC3 = 0.07135481282636f;    // 0.044715 * kGeluC
 
-__device__ __forceinline__ float over_one_plus_exp(float num, float v) {
-  return __fdividef(num, 1.0f + __expf(-v));
+__device__ __forceinline__ float logistic(float v) {
+  float e, p;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(1.0f + e));
+  return p;
 }
 
 __device__ __forceinline__ float gelu_arg(float z) { return z * fmaf(kGeluC3, z * z, kGeluC); }
@@ -30,8 +36,8 @@ __device__ __forceinline__ float gelu_arg(float z) { return z * fmaf(kGeluC3, z 
 template <int kAct>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (kAct == kActRelu) return z > 0.0f ? z : (z == z ? 0.0f : z);
-  if constexpr (kAct == kActSilu) return over_one_plus_exp(z, z);
-  if constexpr (kAct == kActGelu) return over_one_plus_exp(z, gelu_arg(z));
+  if constexpr (kAct == kActSilu) return z * logistic(z);
+  if constexpr (kAct == kActGelu) return z * logistic(gelu_arg(z));
   return z;
 }
 
@@ -41,14 +47,24 @@ __device__ __forceinline__ float act_slope(float z) {
   z = fabsf(z) > 128.0f ? copysignf(128.0f, z) : z;
   if constexpr (kAct == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
   if constexpr (kAct == kActSilu) {
-    const float p = over_one_plus_exp(1.0f, z);
+    const float p = logistic(z);
     return p * fmaf(z, 1.0f - p, 1.0f);
   }
   if constexpr (kAct == kActGelu) {
-    const float p = over_one_plus_exp(1.0f, gelu_arg(z));
+    const float p = logistic(gelu_arg(z));
     return p * fmaf(z * (1.0f - p), fmaf(3.0f * kGeluC3, z * z, kGeluC), 1.0f);
   }
   return 1.0f;
+}
+
+// Two gates g, factors u and output gradients d at a time:
+// dg = d u silu'(g), du = d silu(g).
+__device__ __forceinline__ void gated_grad2(float2 d, float2 g, float2 u, float2& dg, float2& du) {
+  const float2 p = make_float2(logistic(g.x), logistic(g.y));
+  const float2 gp = mul2(g, p);
+  const float2 slope = fma2(gp, fma2(p, both(-1.0f), both(1.0f)), p);
+  dg = mul2(mul2(d, u), slope);
+  du = mul2(d, gp);
 }
 
 }  // namespace qg

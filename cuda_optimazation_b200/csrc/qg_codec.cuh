@@ -75,12 +75,13 @@ __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float 
 
 // ue8m0 code of a block with largest magnitude `amax` (the MXFP8 quantizer's
 // rule: exponent floor(log2 amax) - 8 clamped at -127, 0 for a zero block), and
-// the reciprocal 2^-e of the scale it stands for.  Exponents stay below 121,
-// so the reciprocal is a normal number.
+// the reciprocal 2^-e of the scale it stands for.  floor(log2) is the exponent
+// field: subnormal amax are below the clamp, and codes end at 247 (an infinite
+// amax), so the reciprocal is a normal number.
 __device__ __forceinline__ uint32_t mxfp8_scale_code(float amax, float& mul) {
-  const int e = amax > 0.0f ? max(-127, floor_log2_positive(amax) - 8) : -127;
-  mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  return static_cast<uint32_t>(e + 127);
+  const uint32_t code = max(__float_as_uint(amax) >> 23, 8u) - 8u;
+  mul = __uint_as_float((254u - code) << 23);
+  return code;
 }
 
 // The scale 2^(code - 127) that a ue8m0 code stands for (code 0: 2^-127, a
@@ -88,6 +89,33 @@ __device__ __forceinline__ uint32_t mxfp8_scale_code(float amax, float& mul) {
 __device__ __forceinline__ float e8m0_decode(uint32_t code) {
   return __uint_as_float(code ? (code == 255u ? 0x7fc00000u : code << 23) : 0x00400000u);
 }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // Two e4m3 bytes -> two floats (exact: every e4m3 value is an f16 value).
 __device__ __forceinline__ float2 e4m3x2_decode(uint32_t two) {

@@ -195,13 +195,13 @@ struct RmsNormBwdParams {
   const void* dres;  // may be null
   const float* rstd;
   void* dx;
-  float* dw_part;    // [rmsnorm_backward_parts(rows)][k]; null: no dw
+  float* dw_part;    // [rmsnorm_backward_parts(rows, k)][k] at most; null: no dw
   int64_t lddy, ldh, lddres, lddx;
   int64_t rows, k;
 };
 cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
                                  cudaStream_t stream);
-int rmsnorm_backward_parts(int64_t rows);
+int rmsnorm_backward_parts(int64_t rows, int64_t k);
 cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16, float* dw,
                                     cudaStream_t stream);
 // out[c] = sum over r < parts of part[r][c], in a fixed order.

@@ -12,8 +12,17 @@
 // g = dy * w:   dx = rstd (g - xh mean(g xh)) + dres,   dw = sum_rows dy xh.
 //
 // Both are bound by HBM: 7 bytes an element forward (bf16 with a residual), 8
-// backward.  A row lives in its CTA's registers between the reduction and the
-// output, so every byte crosses HBM once.
+// backward, every byte crossing once.  A row belongs to a group of threads;
+// thread t of it owns the 8-value vectors t, t + group, ... (kVec at most), so
+// four neighbouring lanes hold one 32-value MX block and sixteen one 4-byte
+// word of scales.
+//
+// Many rows (ring kernels): CTAs stay on their SM and every thread copies its
+// own vectors of the next rows into shared memory ahead of time (cp.async, two
+// or three rows deep), so the bytes in flight do not depend on registers or
+// on where a CTA stands between its two barriers.  A thread reads back only
+// what it copied itself, so the ring needs no barrier.  Few rows, or rows too
+// long for the ring: one CTA per row, values straight to registers.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -21,59 +30,118 @@
 
 #include "qg_codec.cuh"
 #include "qg_gemm.h"
+#include "qg_ptx.cuh"
 
 namespace qg {
 
 namespace {
 
-// Eight consecutive values as fp32 (16 bytes of bf16 or 32 of fp32).  kOnce: a
-// row's own values, read once (streaming, and coherent: an output may be an
-// input's own buffer); otherwise the weight, which every row reads again.
-template <bool kBf16, bool kOnce = true>
-__device__ __forceinline__ void load8(const void* base, int64_t elem, float (&v)[8]) {
-  if constexpr (kBf16) {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + elem);
-    const uint4 a = kOnce ? __ldcs(p) : __ldg(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight consecutive values as four fp32 pairs.
+struct Vec8 {
+  float2 v[4];
+};
+
+// Raw storage of eight consecutive values: 16 bytes of bf16 or 32 of fp32.
+template <bool kBf16>
+struct Raw8 {
+  static constexpr int kChunks = kBf16 ? 1 : 2;
+  uint4 c[kChunks];
+  __device__ __forceinline__ Vec8 decode() const {
+    Vec8 r;
+    const uint32_t* w = &c[0].x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      if constexpr (kBf16)
+        r.v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      else
+        r.v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     }
-  } else {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + elem);
-    const float4 a = kOnce ? __ldcs(p) : __ldg(p), b = kOnce ? __ldcs(p + 1) : __ldg(p + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    return r;
   }
+};
+
+template <bool kBf16>
+constexpr int kElem = kBf16 ? 2 : 4;
+
+// A row's own values, read once (streaming, and coherent: an output may be an
+// input's own buffer).
+template <bool kBf16>
+__device__ __forceinline__ Raw8<kBf16> load_once(const void* base, int64_t elem) {
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) +
+                                                  elem * kElem<kBf16>);
+  Raw8<kBf16> r;
+#pragma unroll
+  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) r.c[i] = __ldcs(p + i);
+  return r;
+}
+
+// The weight, which every row reads again.
+template <bool kBf16>
+__device__ __forceinline__ Raw8<kBf16> load_kept(const void* base, int64_t elem) {
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) +
+                                                  elem * kElem<kBf16>);
+  Raw8<kBf16> r;
+#pragma unroll
+  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) r.c[i] = __ldg(p + i);
+  return r;
 }
 
 template <bool kBf16>
-__device__ __forceinline__ void store8(void* base, int64_t elem, const float (&v)[8]) {
+__device__ __forceinline__ void store8(void* base, int64_t elem, const Vec8& x) {
+  uint4* p = reinterpret_cast<uint4*>(static_cast<uint8_t*>(base) + elem * kElem<kBf16>);
   if constexpr (kBf16) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x.v[i].x, x.v[i].y);
       w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + elem) =
-        make_uint4(w[0], w[1], w[2], w[3]);
+    *p = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
-    float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + elem);
-    p[0] = make_float4(v[0], v[1], v[2], v[3]);
-    p[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      p[i] = make_uint4(__float_as_uint(x.v[2 * i].x), __float_as_uint(x.v[2 * i].y),
+                        __float_as_uint(x.v[2 * i + 1].x), __float_as_uint(x.v[2 * i + 1].y));
   }
 }
 
-// Sum over the CTA in a fixed order; every thread gets it.  `red` holds one
-// float per warp and is free again after the next call's first barrier.
-__device__ __forceinline__ float cta_sum(float v, float* red) {
+// One input's row in a ring slot: 16-byte chunks, the first chunks of all
+// vectors and then (fp32) the second ones, so that a warp's accesses are
+// contiguous.
+template <bool kBf16>
+__device__ __forceinline__ void ring_copy(uint8_t* slot, const void* base, int64_t elem, int v,
+                                          int nvec) {
+  const uint8_t* g = static_cast<const uint8_t*>(base) + (elem + v * 8) * kElem<kBf16>;
+#pragma unroll
+  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     smem_u32(slot + (i * nvec + v) * 16)),
+                 "l"(g + 16 * i)
+                 : "memory");
+}
+template <bool kBf16>
+__device__ __forceinline__ Raw8<kBf16> ring_read(const uint8_t* slot, int v, int nvec) {
+  Raw8<kBf16> r;
+#pragma unroll
+  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) r.c[i] = lds128(slot + (i * nvec + v) * 16);
+  return r;
+}
+__device__ __forceinline__ void ring_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kLeft>
+__device__ __forceinline__ void ring_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+// Sum over the row's threads (blockDim.x of them: one warp, or the whole CTA) in
+// a fixed order; every thread gets it.
+__device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   const int warps = blockDim.x >> 5;
   if (warps == 1) return v;
-  __syncthreads();
+  __syncthreads();  // the previous sum's reads of red
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = (threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.0f;
@@ -82,132 +150,237 @@ __device__ __forceinline__ float cta_sum(float v, float* red) {
   return v;
 }
 
-// One CTA per row; thread t owns the 8-value vectors t, t + blockDim, ...
-// (kVec of them at most), so four neighbouring lanes hold one 32-value MX
-// block and sixteen one 4-byte word of scales.
+__device__ __forceinline__ float sum4(float2 a, float2 b, float2 c, float2 d) {
+  const float2 s = add2(add2(a, b), add2(c, d));
+  return s.x + s.y;
+}
+
+__device__ __forceinline__ float square_sum(const Vec8& h) {
+  return sum4(mul2(h.v[0], h.v[0]), mul2(h.v[1], h.v[1]), mul2(h.v[2], h.v[2]),
+              mul2(h.v[3], h.v[3]));
+}
+
+// y of one vector, quantised and stored.  Every lane of the warp takes part;
+// `in` says whether the vector lies in the row.
+__device__ __forceinline__ void store_y(const RmsNormParams& p, int64_t row, int v, bool in,
+                                        const Vec8& h, const Vec8& w, float rstd, int lane) {
+  Vec8 y;
+  float amax = 0.0f;
+  if (in) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y.v[i] = mul2(mul2(h.v[i], both(rstd)), w.v[i]);
+      amax = fmaxf(fmaxf(amax, fabsf(y.v[i].x)), fabsf(y.v[i].y));
+    }
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  float mul;
+  const uint32_t code = mxfp8_scale_code(amax, mul);  // 0 beyond the row: padding
+  if (in) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y.v[i] = mul2(y.v[i], both(mul));
+    *reinterpret_cast<uint2*>(p.q + row * p.k + v * 8) =
+        make_uint2(cvt_e4m3x4(y.v[0].x, y.v[0].y, y.v[1].x, y.v[1].y),
+                   cvt_e4m3x4(y.v[2].x, y.v[2].y, y.v[3].x, y.v[3].y));
+  }
+  if (p.layout == 0) {
+    if (in && (lane & 3) == 0) p.sf[row * (p.k / 32) + v / 4] = static_cast<uint8_t>(code);
+  } else {
+    // Codes of the word's four blocks, joined over lanes 0, 4, 8, 12 of 16.
+    uint32_t word = code | __shfl_down_sync(0xffffffffu, code, 4) << 8;
+    word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
+    if (in && (lane & 15) == 0)
+      *reinterpret_cast<uint32_t*>(
+          p.sf + mma_scale_offset(row, v / 4, p.row_blocks, p.sf_blocks, p.layout)) = word;
+  }
+}
+
+// The scale words of the rows that fill the last 128-row chunks read as zero:
+// threads `first`, first + step, ... write them, neighbours neighbouring words.
+__device__ __forceinline__ void pad_scales(const RmsNormParams& p, int first, int step) {
+  if (p.layout == 0) return;
+  const int used = static_cast<int>(p.rows - (p.row_blocks - 1) * 128);
+  if (used == 128) return;
+  const int words = static_cast<int>(p.sf_blocks) * 128;
+  for (int i = first; i < words; i += step) {
+    const int bs = i >> 7, w = i & 127;
+    if ((w >> 2) + (w & 3) * 32 < used) continue;
+    const int64_t chunk = p.layout == 1 ? bs * p.row_blocks + p.row_blocks - 1
+                                        : (p.row_blocks - 1) * p.sf_blocks + bs;
+    reinterpret_cast<uint32_t*>(p.sf + chunk * 512)[w] = 0u;
+  }
+}
+
+// ------------------------------------------------------------------ forward
+// One CTA per row; CTAs past the rows write the padding.
 template <bool kBf16, bool kWBf16, int kVec>
-__global__ void __launch_bounds__(512) rmsnorm_mxfp8_kernel(const RmsNormParams p) {
+__global__ void __launch_bounds__(1024) rmsnorm_direct_kernel(const RmsNormParams p) {
   __shared__ float red[32];
   const int64_t row = blockIdx.x;
+  if (row >= p.rows) {
+    const int pads = static_cast<int>(gridDim.x - p.rows);
+    pad_scales(p, static_cast<int>(row - p.rows) * blockDim.x + threadIdx.x, pads * blockDim.x);
+    return;
+  }
   const int nvec = static_cast<int>(p.k / 8);
-  float h[kVec][8];
+  Vec8 h[kVec];
+  Raw8<kWBf16> w[kVec];
   float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v < nvec) {
-      load8<kBf16>(p.x, row * p.ldx + v * 8, h[i]);
+      h[i] = load_once<kBf16>(p.x, row * p.ldx + v * 8).decode();
+      w[i] = load_kept<kWBf16>(p.weight, v * 8);
       if (p.residual) {
-        float r[8];
-        load8<kBf16>(p.residual, row * p.ldr + v * 8, r);
+        const Vec8 r = load_once<kBf16>(p.residual, row * p.ldr + v * 8).decode();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] += r[j];
+        for (int j = 0; j < 4; ++j) h[i].v[j] = add2(h[i].v[j], r.v[j]);
       }
       if (p.h) store8<kBf16>(p.h, row * p.ldh + v * 8, h[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
+      ss += square_sum(h[i]);
     }
   }
-  ss = cta_sum(ss, red);
-  const float rstd = rsqrtf(ss / static_cast<float>(p.k) + p.eps);
+  const float rstd = rsqrtf(row_sum(ss, red) / static_cast<float>(p.k) + p.eps);
   if (threadIdx.x == 0 && p.rstd) p.rstd[row] = rstd;
-  const int lane = threadIdx.x & 31;
-  const int64_t sfk = p.k / 32;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    const bool in = v < nvec;
-    float y[8];
-    float amax = 0.0f;
-    if (in) {
-      float w[8];
-      load8<kWBf16, false>(p.weight, v * 8, w);
+    store_y(p, row, v, v < nvec, h[i], w[i].decode(), rstd, threadIdx.x & 31);
+  }
+}
+
+// blockDim (group, rows at a time).
+template <bool kBf16, bool kWBf16, int kVec, int kStages>
+__global__ void __launch_bounds__(512) rmsnorm_ring_kernel(const RmsNormParams p) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float red[32];
+  const int nvec = static_cast<int>(p.k / 8);
+  const int row_bytes = static_cast<int>(p.k) * kElem<kBf16>;
+  const int slot_bytes = p.residual ? 2 * row_bytes : row_bytes;
+  uint8_t* mine = ring + threadIdx.y * kStages * slot_bytes;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < p.rows) {
+      uint8_t* slot = mine + stage * slot_bytes;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[j] = h[i][j] * rstd * w[j];
-        amax = fmaxf(amax, fabsf(y[j]));
+      for (int i = 0; i < kVec; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < nvec) {
+          ring_copy<kBf16>(slot, p.x, row * p.ldx, v, nvec);
+          if (p.residual) ring_copy<kBf16>(slot + row_bytes, p.residual, row * p.ldr, v, nvec);
+        }
       }
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    float mul;
-    const uint32_t code = mxfp8_scale_code(amax, mul);  // 0 beyond the row: padding
-    if (in)
-      *reinterpret_cast<uint2*>(p.q + row * p.k + v * 8) =
-          make_uint2(cvt_e4m3x4(y[0] * mul, y[1] * mul, y[2] * mul, y[3] * mul),
-                     cvt_e4m3x4(y[4] * mul, y[5] * mul, y[6] * mul, y[7] * mul));
-    if (p.layout == 0) {
-      if (in && (lane & 3) == 0) p.sf[row * sfk + v / 4] = static_cast<uint8_t>(code);
-    } else {
-      uint32_t word = 0;
+    ring_commit();
+  };
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        word |= __shfl_sync(0xffffffffu, code, (lane & 16) + 4 * j) << (8 * j);
-      if ((lane & 15) == 0 && in)
-        *reinterpret_cast<uint32_t*>(
-            p.sf + mma_scale_offset(row, v / 4, p.row_blocks, p.sf_blocks, p.layout)) = word;
+  for (int s = 0; s < kStages; ++s) fetch(first + s * step, s);
+  int stage = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    ring_wait<kStages - 1>();
+    const uint8_t* slot = mine + stage * slot_bytes;
+    Vec8 h[kVec];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < nvec) {
+        h[i] = ring_read<kBf16>(slot, v, nvec).decode();
+        if (p.residual) {
+          const Vec8 r = ring_read<kBf16>(slot + row_bytes, v, nvec).decode();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) h[i].v[j] = add2(h[i].v[j], r.v[j]);
+        }
+        ss += square_sum(h[i]);
+      }
+    }
+    fetch(row + kStages * step, stage);
+    if (++stage == kStages) stage = 0;
+    const float rstd = rsqrtf(row_sum(ss, red) / static_cast<float>(p.k) + p.eps);
+    if (threadIdx.x == 0 && p.rstd) p.rstd[row] = rstd;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      const bool in = v < nvec;
+      Vec8 w;
+      if (in) {
+        if (p.h) store8<kBf16>(p.h, row * p.ldh + v * 8, h[i]);
+        w = load_kept<kWBf16>(p.weight, v * 8).decode();
+      }
+      store_y(p, row, v, in, h[i], w, rstd, threadIdx.x & 31);
     }
   }
-  // The scale words of the rows that fill the last 128-row chunk read as 0;
-  // the CTAs share them out.
-  if (p.layout != 0) {
-    const int64_t pad = (p.row_blocks * 128 - p.rows) * p.sf_blocks;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < pad;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-      const int64_t r = p.rows + i / p.sf_blocks, c = i % p.sf_blocks;
-      *reinterpret_cast<uint32_t*>(
-          p.sf + mma_scale_offset(r, 4 * c, p.row_blocks, p.sf_blocks, p.layout)) = 0u;
-    }
+  ring_wait<0>();
+  const int t = threadIdx.y * blockDim.x + threadIdx.x, n = blockDim.x * blockDim.y;
+  pad_scales(p, static_cast<int>(blockIdx.x) * n + t, static_cast<int>(gridDim.x) * n);
+}
+
+// ------------------------------------------------------------------ backward
+// dot += g xh and dw += dy xh of one vector.
+template <bool kWBf16>
+__device__ __forceinline__ float bwd_dot(const Vec8& dy, const Vec8& h, const Vec8& w, float rstd,
+                                         Vec8& dw) {
+  float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 t = mul2(dy.v[j], mul2(h.v[j], both(rstd)));
+    dw.v[j] = add2(dw.v[j], t);
+    s = fma2(t, w.v[j], s);
   }
+  return s.x + s.y;
+}
+
+// dx of one vector: rstd (dy w - xh c) + dres.
+__device__ __forceinline__ Vec8 bwd_dx(const Vec8& dy, const Vec8& h, const Vec8& w, float rstd,
+                                       float c) {
+  Vec8 d;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    d.v[j] = mul2(both(rstd), fma2(mul2(h.v[j], both(rstd)), both(-c), mul2(dy.v[j], w.v[j])));
+  return d;
 }
 
 // CTA b takes rows b, b + grid, ...; each thread owns the same columns of all
 // of them, so its share of dw stays in registers and is written once, to row b
 // of the partial sums.
 template <bool kBf16, bool kWBf16, int kVec>
-__global__ void __launch_bounds__(512) rmsnorm_backward_kernel(const RmsNormBwdParams p) {
+__global__ void __launch_bounds__(512) rmsnorm_backward_direct_kernel(const RmsNormBwdParams p) {
   __shared__ float red[32];
   const int nvec = static_cast<int>(p.k / 8);
   const float inv_k = 1.0f / static_cast<float>(p.k);
-  float dw[kVec][8];
+  Vec8 dw[kVec];
 #pragma unroll
   for (int i = 0; i < kVec; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[i][j] = 0.0f;
+    for (int j = 0; j < 4; ++j) dw[i].v[j] = make_float2(0.0f, 0.0f);
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float rstd = __ldg(p.rstd + row);
-    float g[kVec][8], xh[kVec][8];
+    Raw8<kBf16> dy[kVec], h[kVec];
+    Raw8<kWBf16> w[kVec];
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
       if (v < nvec) {
-        float w[8];
-        load8<kBf16>(p.dy, row * p.lddy + v * 8, g[i]);
-        load8<kBf16>(p.h, row * p.ldh + v * 8, xh[i]);
-        load8<kWBf16, false>(p.weight, v * 8, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          xh[i][j] *= rstd;
-          dw[i][j] = fmaf(g[i][j], xh[i][j], dw[i][j]);
-          g[i][j] *= w[j];
-          dot = fmaf(g[i][j], xh[i][j], dot);
-        }
+        dy[i] = load_once<kBf16>(p.dy, row * p.lddy + v * 8);
+        h[i] = load_once<kBf16>(p.h, row * p.ldh + v * 8);
+        w[i] = load_kept<kWBf16>(p.weight, v * 8);
+        dot += bwd_dot<kWBf16>(dy[i].decode(), h[i].decode(), w[i].decode(), rstd, dw[i]);
       }
     }
-    const float c = cta_sum(dot, red) * inv_k;
+    const float c = row_sum(dot, red) * inv_k;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
       if (v < nvec) {
-        float d[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = rstd * fmaf(-xh[i][j], c, g[i][j]);
+        Vec8 d = bwd_dx(dy[i].decode(), h[i].decode(), w[i].decode(), rstd, c);
         if (p.dres) {
-          float r[8];
-          load8<kBf16>(p.dres, row * p.lddres + v * 8, r);
+          const Vec8 r = load_once<kBf16>(p.dres, row * p.lddres + v * 8).decode();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] += r[j];
+          for (int j = 0; j < 4; ++j) d.v[j] = add2(d.v[j], r.v[j]);
         }
         store8<kBf16>(p.dx, row * p.lddx + v * 8, d);
       }
@@ -222,89 +395,264 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_kernel(const RmsNormBwdP
   }
 }
 
-// out[c] = sum over `parts` rows of part[.][c], in a fixed order: eight threads
-// of a column sum every eighth row and are joined in shared memory.
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* part, int parts, int64_t k,
-                                                         float* out) {
-  __shared__ float sum[8][32];
-  const int64_t c = blockIdx.x * 32ll + threadIdx.x;
-  float s = 0.0f;
-  if (c < k)
-    for (int r = threadIdx.y; r < parts; r += 8) s += part[r * k + c];
-  sum[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < k) {
+// blockDim (group, rows at a time).  dy and h are read from the ring twice
+// instead of being held over the reduction.
+template <bool kBf16, bool kWBf16, int kVec, int kStages>
+__global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNormBwdParams p) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float red[32];
+  const int nvec = static_cast<int>(p.k / 8);
+  const float inv_k = 1.0f / static_cast<float>(p.k);
+  const int row_bytes = static_cast<int>(p.k) * kElem<kBf16>;
+  const int slot_bytes = p.dres ? 3 * row_bytes : 2 * row_bytes;
+  uint8_t* mine = ring + threadIdx.y * kStages * slot_bytes;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < p.rows) {
+      uint8_t* slot = mine + stage * slot_bytes;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += sum[i][threadIdx.x];
-    out[c] = s;
+      for (int i = 0; i < kVec; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < nvec) {
+          ring_copy<kBf16>(slot, p.dy, row * p.lddy, v, nvec);
+          ring_copy<kBf16>(slot + row_bytes, p.h, row * p.ldh, v, nvec);
+          if (p.dres) ring_copy<kBf16>(slot + 2 * row_bytes, p.dres, row * p.lddres, v, nvec);
+        }
+      }
+    }
+    ring_commit();
+  };
+  Vec8 dw[kVec];
+  Raw8<kWBf16> w[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dw[i].v[j] = make_float2(0.0f, 0.0f);
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) w[i] = load_kept<kWBf16>(p.weight, v * 8);
+  }
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(first + s * step, s);
+  int stage = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    const float rstd = __ldg(p.rstd + row);
+    ring_wait<kStages - 1>();
+    const uint8_t* slot = mine + stage * slot_bytes;
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < nvec)
+        dot += bwd_dot<kWBf16>(ring_read<kBf16>(slot, v, nvec).decode(),
+                               ring_read<kBf16>(slot + row_bytes, v, nvec).decode(),
+                               w[i].decode(), rstd, dw[i]);
+    }
+    const float c = row_sum(dot, red) * inv_k;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < nvec) {
+        Vec8 d = bwd_dx(ring_read<kBf16>(slot, v, nvec).decode(),
+                        ring_read<kBf16>(slot + row_bytes, v, nvec).decode(), w[i].decode(), rstd,
+                        c);
+        if (p.dres) {
+          const Vec8 r = ring_read<kBf16>(slot + 2 * row_bytes, v, nvec).decode();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d.v[j] = add2(d.v[j], r.v[j]);
+        }
+        store8<kBf16>(p.dx, row * p.lddx + v * 8, d);
+      }
+    }
+    fetch(row + kStages * step, stage);
+    if (++stage == kStages) stage = 0;
+  }
+  ring_wait<0>();
+  if (!p.dw_part) return;
+  if (blockDim.y == 1) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < nvec) store8<false>(p.dw_part, blockIdx.x * p.k + v * 8, dw[i]);
+    }
+    return;
+  }
+  // The CTA's row groups, joined in order through the ring's memory.
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) store8<false>(sums, threadIdx.y * p.k + v * 8, dw[i]);
+  }
+  __syncthreads();
+  for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < p.k; c += blockDim.x * blockDim.y) {
+    float s = sums[c];
+    for (int y = 1; y < static_cast<int>(blockDim.y); ++y) s += sums[y * p.k + c];
+    p.dw_part[blockIdx.x * p.k + c] = s;
   }
 }
 
-// Threads per CTA and vectors per thread of a row of k values: whole warps,
-// at most 512 threads until a thread would hold more than eight vectors.
+// out[c] = sum over `parts` rows of part[.][c], in a fixed order: 32 threads of
+// a column sum every 32nd row and are joined in shared memory.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* part, int parts, int64_t k,
+                                                          float* out) {
+  __shared__ float sum[32][33];
+  const int64_t c = blockIdx.x * 32ll + threadIdx.x;
+  float s = 0.0f;
+  if (c < k)
+    for (int r = threadIdx.y; r < parts; r += 32) s += part[r * k + c];
+  sum[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = sum[threadIdx.x][threadIdx.y];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int64_t oc = blockIdx.x * 32ll + threadIdx.y;
+  if (threadIdx.x == 0 && oc < k) out[oc] = s;
+}
+
+// ------------------------------------------------------------------ shapes
+constexpr int kRingSmem = 220 * 1024;  // shared memory of an SM that rings may take
+constexpr int kRingVec = 4;            // vectors of a row per thread
+
+// Ring kernels: rows of at most kRingVec x 512 vectors, one warp per row and
+// eight rows per CTA up to 1024 values.  Three slots a row group where two
+// such CTAs fit an SM, else two; none (stages 0) where a CTA does not fit or
+// the rows do not go round: with fewer than two rows per resident CTA nothing
+// would be prefetched.
+struct RingShape {
+  int group = 0, rows = 0, stages = 0, smem = 0, grid = 0;
+};
+RingShape ring_shape(int64_t rows, int64_t k, int64_t slot_bytes) {
+  RingShape s;
+  const int64_t nvec = k / 8;
+  if (nvec > 512 * kRingVec) return s;
+  s.group = static_cast<int>((nvec + kRingVec - 1) / kRingVec + 31) / 32 * 32;
+  s.rows = s.group == 32 ? 8 : 1;
+  const int64_t slots = slot_bytes * s.rows;
+  const int stages = 2 * (3 * slots + 1024) <= kRingSmem ? 3 : 2;
+  if (stages * slots > kRingSmem) return s;
+  int64_t ctas = kRingSmem / (stages * slots + 1024);
+  if (ctas < 1) ctas = 1;
+  if (ctas > 512 / (s.group * s.rows)) ctas = 512 / (s.group * s.rows);  // 128 registers
+  s.grid = static_cast<int>(ctas * num_sms());
+  if (rows < 2ll * s.grid * s.rows) return s;
+  s.stages = stages;
+  s.smem = static_cast<int>(stages * slots);
+  return s;
+}
+
+// Direct kernels: whole warps, as many threads as the row has vectors, up to
+// `most`.
 struct RowShape {
   int threads, vec;
 };
-RowShape row_shape(int64_t k) {
+RowShape row_shape(int64_t k, int most) {
   const int64_t nvec = k / 8;
   RowShape s{};
-  for (s.vec = 1; s.vec < 8 && nvec > 512 * s.vec; s.vec *= 2) {
+  for (s.vec = 1; s.vec < 8 && nvec > static_cast<int64_t>(most) * s.vec; s.vec *= 2) {
   }
   s.threads = static_cast<int>((nvec + s.vec - 1) / s.vec + 31) / 32 * 32;
   return s;
 }
 
-template <bool kBf16, bool kWBf16>
-void launch_norm(const RmsNormParams& p, RowShape s, cudaStream_t stream) {
-  const int grid = static_cast<int>(p.rows);
-  if (s.vec == 1) rmsnorm_mxfp8_kernel<kBf16, kWBf16, 1><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 2) rmsnorm_mxfp8_kernel<kBf16, kWBf16, 2><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 4) rmsnorm_mxfp8_kernel<kBf16, kWBf16, 4><<<grid, s.threads, 0, stream>>>(p);
-  else rmsnorm_mxfp8_kernel<kBf16, kWBf16, 8><<<grid, s.threads, 0, stream>>>(p);
+template <typename K, typename P>
+void launch_ring(K kernel, const P& p, const RingShape& s, cudaStream_t stream) {
+  static bool done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return;
+  if (!done[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem) !=
+        cudaSuccess)
+      return;
+    done[dev] = true;
+  }
+  kernel<<<s.grid, dim3(s.group, s.rows), s.smem, stream>>>(p);
 }
 
 template <bool kBf16, bool kWBf16>
-void launch_norm_bwd(const RmsNormBwdParams& p, RowShape s, int grid, cudaStream_t stream) {
-  if (s.vec == 1) rmsnorm_backward_kernel<kBf16, kWBf16, 1><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 2) rmsnorm_backward_kernel<kBf16, kWBf16, 2><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 4) rmsnorm_backward_kernel<kBf16, kWBf16, 4><<<grid, s.threads, 0, stream>>>(p);
-  else rmsnorm_backward_kernel<kBf16, kWBf16, 8><<<grid, s.threads, 0, stream>>>(p);
+void launch_norm(const RmsNormParams& p, cudaStream_t stream) {
+  const RingShape r =
+      ring_shape(p.rows, p.k, p.k * kElem<kBf16> * (p.residual ? 2 : 1));
+  if (r.stages == 3)
+    return launch_ring(rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 3>, p, r, stream);
+  if (r.stages == 2)
+    return launch_ring(rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 2>, p, r, stream);
+  const RowShape s = row_shape(p.k, 1024);
+  // Padding words of the last chunks, four per thread.
+  int pads = 0;
+  if (p.layout != 0 && p.rows % 128 != 0)
+    pads = static_cast<int>((p.sf_blocks * 128 + 4 * s.threads - 1) / (4 * s.threads));
+  const int grid = static_cast<int>(p.rows) + pads;
+  if (s.vec == 1) rmsnorm_direct_kernel<kBf16, kWBf16, 1><<<grid, s.threads, 0, stream>>>(p);
+  else if (s.vec == 2) rmsnorm_direct_kernel<kBf16, kWBf16, 2><<<grid, s.threads, 0, stream>>>(p);
+  else rmsnorm_direct_kernel<kBf16, kWBf16, 4><<<grid, s.threads, 0, stream>>>(p);
+}
+
+int backward_direct_grid(int64_t rows) {
+  const int64_t most = 2ll * num_sms();
+  return static_cast<int>(rows < most ? rows : most);
+}
+
+template <bool kBf16, bool kWBf16>
+int launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
+  const RingShape r = ring_shape(p.rows, p.k, p.k * kElem<kBf16> * (p.dres ? 3 : 2));
+  if (r.stages) {
+    if (r.stages == 3)
+      launch_ring(rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 3>, p, r, stream);
+    else
+      launch_ring(rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 2>, p, r, stream);
+    return r.grid;
+  }
+  const RowShape s = row_shape(p.k, 512);
+  const int grid = backward_direct_grid(p.rows);
+  if (s.vec == 1)
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 1><<<grid, s.threads, 0, stream>>>(p);
+  else if (s.vec == 2)
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 2><<<grid, s.threads, 0, stream>>>(p);
+  else if (s.vec == 4)
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4><<<grid, s.threads, 0, stream>>>(p);
+  else
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8><<<grid, s.threads, 0, stream>>>(p);
+  return grid;
 }
 
 }  // namespace
 
 cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
                                  cudaStream_t stream) {
-  const RowShape s = row_shape(p.k);
-  if (bf16) w_bf16 ? launch_norm<true, true>(p, s, stream) : launch_norm<true, false>(p, s, stream);
-  else w_bf16 ? launch_norm<false, true>(p, s, stream) : launch_norm<false, false>(p, s, stream);
+  if (bf16) w_bf16 ? launch_norm<true, true>(p, stream) : launch_norm<true, false>(p, stream);
+  else w_bf16 ? launch_norm<false, true>(p, stream) : launch_norm<false, false>(p, stream);
   return cudaGetLastError();
 }
 
-int rmsnorm_backward_parts(int64_t rows) {
-  const int64_t most = 2ll * num_sms();
-  return static_cast<int>(rows < most ? rows : most);
+int rmsnorm_backward_parts(int64_t rows, int64_t k) {
+  int most = backward_direct_grid(rows);
+  for (int64_t inputs = 2; inputs <= 3; ++inputs)
+    for (int64_t elem = 2; elem <= 4; elem += 2) {
+      const RingShape r = ring_shape(rows, k, k * elem * inputs);
+      if (r.stages && r.grid > most) most = r.grid;
+    }
+  return most;
 }
 
 cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16, float* dw,
                                     cudaStream_t stream) {
-  const RowShape s = row_shape(p.k);
-  const int grid = rmsnorm_backward_parts(p.rows);
+  int parts;
   if (bf16)
-    w_bf16 ? launch_norm_bwd<true, true>(p, s, grid, stream)
-           : launch_norm_bwd<true, false>(p, s, grid, stream);
+    parts = w_bf16 ? launch_norm_bwd<true, true>(p, stream) : launch_norm_bwd<true, false>(p, stream);
   else
-    w_bf16 ? launch_norm_bwd<false, true>(p, s, grid, stream)
-           : launch_norm_bwd<false, false>(p, s, grid, stream);
+    parts = w_bf16 ? launch_norm_bwd<false, true>(p, stream)
+                   : launch_norm_bwd<false, false>(p, stream);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !dw) return e;
-  return launch_column_sum(p.dw_part, grid, p.k, dw, stream);
+  return launch_column_sum(p.dw_part, parts, p.k, dw, stream);
 }
 
 cudaError_t launch_column_sum(const float* part, int parts, int64_t k, float* out,
                               cudaStream_t stream) {
-  column_sum_kernel<<<static_cast<int>((k + 31) / 32), dim3(32, 8), 0, stream>>>(part, parts, k,
-                                                                                out);
+  column_sum_kernel<<<static_cast<int>((k + 31) / 32), dim3(32, 32), 0, stream>>>(part, parts, k,
+                                                                                 out);
   return cudaGetLastError();
 }
 

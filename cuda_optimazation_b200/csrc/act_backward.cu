@@ -32,6 +32,7 @@
 #include "qg_act.cuh"
 #include "qg_codec.cuh"
 #include "qg_gemm.h"
+#include "qg_ptx.cuh"
 
 namespace qg {
 
@@ -39,35 +40,53 @@ namespace {
 
 constexpr int kTile = 128;  // rows, and columns of a set, of a CTA
 
+// Staging: a thread copies its own pieces of the tile into shared memory
+// (cp.async) before it works on any, and reads back only what it copied.
+template <int kBytes>
+__device__ __forceinline__ void stage_copy(uint8_t* to, const void* from) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void stage_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+// All but the last `left` of the four row groups have arrived.
+__device__ __forceinline__ void stage_wait(int left) {
+  if (left >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (left == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Eight gradients: 16 bytes of bf16, or two 16-byte pieces `second` apart.
 template <bool kBf16>
-__device__ __forceinline__ void load_grad8(const void* base, int64_t elem, float (&v)[8]) {
+__device__ __forceinline__ void read_grad8(const uint8_t* at, int second, float2 (&v)[4]) {
+  const uint4 a = lds128(at);
   if constexpr (kBf16) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(
-        static_cast<const __nv_bfloat16*>(base) + elem));
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i)
+      v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   } else {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + elem);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    const uint4 b = lds128(at + second);
+    v[0] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
+    v[1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+    v[2] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
+    v[3] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
   }
 }
 
-// Eight consecutive values of an MXFP8 row with scale s.
-__device__ __forceinline__ void load_mx8(const uint8_t* q, float s, float2 (&v)[4]) {
-  const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
+// Eight values of an MXFP8 row with scale s.
+__device__ __forceinline__ void read_mx8(const uint8_t* at, float s, float2 (&v)[4]) {
+  const uint2 w = *reinterpret_cast<const uint2*>(at);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     v[i] = mul2(e4m3x2_decode((i < 2 ? w.x : w.y) >> (16 * (i & 1))), both(s));
 }
-
-// Larger of two pairs of 16-bit unsigned values.
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
 
 // Upper halves of two non-negative floats' patterns: b's in the high half.
 __device__ __forceinline__ uint32_t upper2(float a, float b) {
@@ -86,13 +105,24 @@ __device__ __forceinline__ float upper_half(uint32_t r) {
   return __uint_as_float(r & 0xffff0000u);
 }
 
+// Bytes that one thread stages of a 32-row group: its 4 rows of the gradient
+// and of each set of z.
+template <int kAct, bool kBf16>
+constexpr int staged_bytes() {
+  return 4 * ((kAct >= 0 ? (kBf16 ? 16 : 32) : 0) +
+              8 * (kAct == kActNone ? 0 : kAct == kActSwiglu ? 2 : 1));
+}
+
 // kAct < 0: z itself (the transposition).  kGroups: 32-row groups of the tile
 // that are worked on at once, by four warps each.
 template <int kAct, bool kBf16, int kGroups>
 __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBackwardParams p) {
   constexpr int kSets = kAct == kActSwiglu ? 2 : 1;
   constexpr bool kGrad = kAct >= 0, kZ = kAct != kActNone;
-  __shared__ uint4 row_sf[kSets][32], col_sf[kSets][32], z_sf[kSets][32];  // 512-byte chunks
+  constexpr int kGradBytes = kGrad ? (kBf16 ? 16 : 32) : 0;
+  extern __shared__ __align__(16) uint8_t staged[];
+  __shared__ uint4 row_sf[kSets][32], col_sf[kSets][32];  // 512-byte chunks
+  __shared__ float4 z_scale[kSets][4][4][8];               // [row group][warp][row / 4]
   __shared__ float part[kGroups > 1 ? kGroups : 1][kSets * kTile];
   const int warp = (threadIdx.x >> 5) & 3, group = threadIdx.x >> 7, lane = threadIdx.x & 31;
   const int rg = lane >> 2, cg = lane & 3;
@@ -104,29 +134,65 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
   // This lane's first column of z (of the gate set) and of dout.
   const int64_t zc = static_cast<int64_t>(tc) * kSets * kTile + warp * 32 + cg * 8;
   const int64_t dc = static_cast<int64_t>(tc) * kTile + warp * 32 + cg * 8;
+  const bool active = zc < p.n;  // p.n is a multiple of 32: a warp is in or out as a whole
   const int64_t row_blocks = (p.m + 127) / 128, n_blocks = (p.n + 127) / 128;
   const int64_t sf_blocks = (p.n / 32 + 3) / 4, t_blocks = (p.mt / 32 + 3) / 4;
+  // Staged pieces: [row group][row][gradient pieces, sets] of each thread.
+  uint8_t* stage_d = staged + (threadIdx.x & 127) * 16;
+  uint8_t* stage_z = staged + 16 * kGradBytes * 128 + (threadIdx.x & 127) * 8;
+  if (active) {
+    const uint8_t* d = static_cast<const uint8_t*>(p.dout) +
+                       ((m0 + group * 32 + rg * 4) * p.ldd + dc) * (kBf16 ? 2 : 4);
+    const uint8_t* z = p.z_q + (m0 + group * 32 + rg * 4) * p.n + zc;
+#pragma unroll
+    for (int rb = group; rb < 4; rb += kGroups) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (rb * 32 + rg * 4 + i < rows) {
+          const int at = rb * 4 + i;
+          if constexpr (kGrad) {
+            stage_copy<16>(stage_d + at * kGradBytes * 128, d);
+            if constexpr (!kBf16) stage_copy<16>(stage_d + (at * 2 + 1) * 2048, d + 16);
+          }
+          if constexpr (kZ) {
+#pragma unroll
+            for (int s = 0; s < kSets; ++s)
+              stage_copy<8>(stage_z + (at * kSets + s) * 1024, z + s * kTile);
+          }
+        }
+        d += p.ldd * (kBf16 ? 2 : 4);
+        z += p.n;
+      }
+      d += 28 * p.ldd * (kBf16 ? 2 : 4);
+      z += 28 * p.n;
+      stage_commit();
+    }
+  }
   if (threadIdx.x < kSets * 32) {
     const int s = threadIdx.x / 32, i = threadIdx.x % 32;
     row_sf[s][i] = make_uint4(0, 0, 0, 0);
     col_sf[s][i] = make_uint4(0, 0, 0, 0);
     if constexpr (kZ) {
+      // Row i's 16 bytes of the chunk: scales of rows i, i + 32, i + 64, i + 96.
+      const int64_t bs = static_cast<int64_t>(tc) * kSets + s;
+      uint32_t w[4] = {0, 0, 0, 0};
       if (p.z_layout != 0) {
-        const int64_t bs = static_cast<int64_t>(tc) * kSets + s;
         const int64_t chunk = p.z_layout == 1 ? bs * row_blocks + tm : tm * sf_blocks + bs;
-        z_sf[s][i] = __ldg(reinterpret_cast<const uint4*>(p.z_sf + chunk * 512) + i);
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(p.z_sf + chunk * 512) + i);
+        w[0] = c.x; w[1] = c.y; w[2] = c.z; w[3] = c.w;
+      } else {
+        for (int r = 0; r < 4; ++r)
+          for (int c = 0; c < 4; ++c)
+            if (r * 32 + i < rows && bs * 4 + c < p.n / 32)
+              w[r] |= static_cast<uint32_t>(
+                          __ldg(p.z_sf + (m0 + r * 32 + i) * (p.n / 32) + bs * 4 + c))
+                      << (8 * c);
       }
-    }
-  }
-  if constexpr (kZ) {
-    if (p.z_layout == 0) {
-      for (int i = threadIdx.x; i < kSets * kTile * 4; i += 128 * kGroups) {
-        const int s = i / (kTile * 4), r = i / 4 % kTile, c = i % 4;
-        const int64_t sc = (static_cast<int64_t>(tc) * kSets + s) * 4 + c;
-        if (r < rows && sc < p.n / 32)
-          reinterpret_cast<uint8_t*>(z_sf[s])[(r & 31) * 16 + (r >> 5) * 4 + c] =
-              __ldg(p.z_sf + (m0 + r) * (p.n / 32) + sc);
-      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          reinterpret_cast<float*>(z_scale[s][r][c])[i] = e8m0_decode(w[r] >> (8 * c) & 0xffu);
     }
   }
   __syncthreads();
@@ -135,29 +201,33 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
   for (int s = 0; s < kSets; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[s][j] = make_float2(0.0f, 0.0f);
-  if (zc < p.n) {  // p.n is a multiple of 32: a warp is in or out as a whole
+  if (active) {
+    uint8_t* row_out = p.dz_q + (m0 + group * 32 + rg * 4) * p.n + zc;
+    uint8_t* col_out = p.dzt_q + zc * p.mt + m0 + group * 32 + rg * 4;
+#pragma unroll 1
     for (int rb = group; rb * 32 < rows; rb += kGroups) {
       const int r0 = rb * 32 + rg * 4;  // this lane's first row of the tile
-      const uint8_t* zq = kZ ? p.z_q + (m0 + r0) * p.n + zc : nullptr;
-      const int64_t de = (m0 + r0) * p.ldd + dc;
+      stage_wait(kGroups > 1 ? 0 : 3 - rb);
       float2 v[kSets][4][4];
+      float zs[kSets][4];
+      if constexpr (kZ) {
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          const float4 f = z_scale[s][rb][warp][rg];
+          zs[s][0] = f.x; zs[s][1] = f.y; zs[s][2] = f.z; zs[s][3] = f.w;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (r0 + i < rows) {
+          const int at = rb * 4 + i;
           float2 d[4];
-          if constexpr (kGrad) {
-            float f[8];
-            load_grad8<kBf16>(p.dout, de + i * p.ldd, f);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = make_float2(f[2 * j], f[2 * j + 1]);
-          }
+          if constexpr (kGrad)
+            read_grad8<kBf16>(stage_d + at * kGradBytes * 128, 2048, d);
           if constexpr (kZ) {
 #pragma unroll
             for (int s = 0; s < kSets; ++s)
-              load_mx8(zq + i * p.n + s * kTile,
-                       e8m0_decode(reinterpret_cast<const uint8_t*>(
-                           z_sf[s])[(rg * 4 + i) * 16 + rb * 4 + warp]),
-                       v[s][i]);
+              read_mx8(stage_z + (at * kSets + s) * 1024, zs[s][i], v[s][i]);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -184,10 +254,10 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
           float peak[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            peak[i] = fmaxf(fabsf(x[i][0].x), fabsf(x[i][0].y));
-#pragma unroll
-            for (int j = 1; j < 4; ++j)
-              peak[i] = fmaxf(fmaxf(peak[i], fabsf(x[i][j].x)), fabsf(x[i][j].y));
+            peak[i] = max3_abs(x[i][0].x, x[i][0].y, x[i][1].x);
+            peak[i] = max3_abs(peak[i], x[i][1].y, x[i][2].x);
+            peak[i] = max3_abs(peak[i], x[i][2].y, x[i][3].x);
+            peak[i] = max3_abs(peak[i], x[i][3].y, 0.0f);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -206,7 +276,7 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
                 w[e] = cvt_e4m3x4(a.x, a.y, b.x, b.y);
               }
               if (r0 + i < rows)
-                *reinterpret_cast<uint2*>(p.dz_q + (m0 + r0 + i) * p.n + zc + s * kTile) =
+                *reinterpret_cast<uint2*>(row_out + i * p.n + s * kTile) =
                     make_uint2(w[0], w[1]);
             }
             if (cg == 0) {
@@ -224,11 +294,9 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
         uint32_t t[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float a = fmaxf(fmaxf(fabsf(x[0][j].x), fabsf(x[1][j].x)),
-                                fmaxf(fabsf(x[2][j].x), fabsf(x[3][j].x)));
-          const float b = fmaxf(fmaxf(fabsf(x[0][j].y), fabsf(x[1][j].y)),
-                                fmaxf(fabsf(x[2][j].y), fabsf(x[3][j].y)));
-          t[j] = upper2(a, b);
+          const float a = max3_abs(x[0][j].x, x[1][j].x, x[2][j].x);
+          const float b = max3_abs(x[0][j].y, x[1][j].y, x[2][j].y);
+          t[j] = upper2(max3_abs(a, x[3][j].x, 0.0f), max3_abs(b, x[3][j].y, 0.0f));
         }
         const bool b4 = lane & 16, b3 = lane & 8;
 #pragma unroll
@@ -247,7 +315,7 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
           to[0] = static_cast<uint8_t>(c >> 7);
           to[16] = static_cast<uint8_t>(c >> 23);
         }
-        uint8_t* tq = p.dzt_q + (zc + s * kTile) * p.mt + m0 + r0;
+        uint8_t* tq = col_out + s * kTile * p.mt;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t rj = __shfl_sync(0xffffffffu, r, cg + 8 * j);
@@ -262,6 +330,8 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
             sum[s][j] = add2(sum[s][j], add2(add2(x[0][j], x[1][j]), add2(x[2][j], x[3][j])));
         }
       }
+      row_out += 32 * p.n;
+      col_out += 32;
     }
     if constexpr (kGrad) {
       if (p.dbias_part) {
@@ -314,15 +384,28 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
 constexpr int kGroupsSmall = 4;
 bool small_grid(int grid) { return grid < 4 * num_sms(); }
 
-template <int kAct>
-void launch_act(const ActBackwardParams& p, bool bf16, int grid, cudaStream_t stream) {
-  if (small_grid(grid)) {
-    if (bf16) act_backward_kernel<kAct, true, kGroupsSmall><<<grid, 512, 0, stream>>>(p);
-    else act_backward_kernel<kAct, false, kGroupsSmall><<<grid, 512, 0, stream>>>(p);
-  } else {
-    if (bf16) act_backward_kernel<kAct, true, 1><<<grid, 128, 0, stream>>>(p);
-    else act_backward_kernel<kAct, false, 1><<<grid, 128, 0, stream>>>(p);
+template <int kAct, bool kBf16, int kGroups>
+cudaError_t launch_one(const ActBackwardParams& p, int grid, cudaStream_t stream) {
+  constexpr int kSmem = staged_bytes<kAct, kBf16>() * 4 * 128;
+  auto kernel = act_backward_kernel<kAct, kBf16, kGroups>;
+  static bool done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
+    return cudaErrorInvalidDevice;
+  if (!done[dev]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    done[dev] = true;
   }
+  kernel<<<grid, 128 * kGroups, kSmem, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <int kAct, bool kBf16>
+cudaError_t launch_act(const ActBackwardParams& p, int grid, cudaStream_t stream) {
+  return small_grid(grid) ? launch_one<kAct, kBf16, kGroupsSmall>(p, grid, stream)
+                          : launch_one<kAct, kBf16, 1>(p, grid, stream);
 }
 
 int act_grid(const ActBackwardParams& p, int sets) {
@@ -335,24 +418,22 @@ int act_grid(const ActBackwardParams& p, int sets) {
 cudaError_t launch_act_backward(const ActBackwardParams& p, int act, bool bf16,
                                 cudaStream_t stream) {
   const int grid = act_grid(p, act == kActSwiglu ? 2 : 1);
+#define QG_ACT_CASE(a) \
+  case a:              \
+    return bf16 ? launch_act<a, true>(p, grid, stream) : launch_act<a, false>(p, grid, stream);
   switch (act) {
-    case kActNone: launch_act<kActNone>(p, bf16, grid, stream); break;
-    case kActRelu: launch_act<kActRelu>(p, bf16, grid, stream); break;
-    case kActSilu: launch_act<kActSilu>(p, bf16, grid, stream); break;
-    case kActGelu: launch_act<kActGelu>(p, bf16, grid, stream); break;
-    case kActSwiglu: launch_act<kActSwiglu>(p, bf16, grid, stream); break;
+    QG_ACT_CASE(kActNone)
+    QG_ACT_CASE(kActRelu)
+    QG_ACT_CASE(kActSilu)
+    QG_ACT_CASE(kActGelu)
+    QG_ACT_CASE(kActSwiglu)
     default: return cudaErrorInvalidValue;
   }
-  return cudaGetLastError();
+#undef QG_ACT_CASE
 }
 
 cudaError_t launch_transpose_mxfp8(const ActBackwardParams& p, cudaStream_t stream) {
-  const int grid = act_grid(p, 1);
-  if (small_grid(grid))
-    act_backward_kernel<-1, false, kGroupsSmall><<<grid, 512, 0, stream>>>(p);
-  else
-    act_backward_kernel<-1, false, 1><<<grid, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_act<-1, false>(p, act_grid(p, 1), stream);
 }
 
 }  // namespace qg

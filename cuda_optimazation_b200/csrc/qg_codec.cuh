@@ -90,6 +90,18 @@ __device__ __forceinline__ float e8m0_decode(uint32_t code) {
   return __uint_as_float(code ? (code == 255u ? 0x7fc00000u : code << 23) : 0x00400000u);
 }
 
+// max(|a|, |b|, |c|) without the NaN among them (NaN if all are).
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;

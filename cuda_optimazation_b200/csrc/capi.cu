@@ -174,7 +174,7 @@ struct Requant {
 struct PreparedGemm {
   GemmParams p;
   int fmt = 1;
-  bool fp4 = true, pair = true, out_bf16 = false;
+  bool fp4 = true, pair = true, out_bf16 = false, rows = false;
   int variant = 1, out_kind = 0, grid = 0;
   void* memset_ptr = nullptr;  // scale padding to clear before each launch
   size_t memset_bytes = 0;
@@ -185,6 +185,7 @@ cudaError_t gemm_launch(const PreparedGemm& g, cudaStream_t stream) {
     cudaError_t e = cudaMemsetAsync(g.memset_ptr, 0, g.memset_bytes, stream);
     if (e != cudaSuccess) return e;
   }
+  if (g.rows) return launch_gemm_fused_rows(g.p, g.fmt, stream);
   if (g.pair) return launch_gemm_pair(g.p, g.fmt, g.out_kind, g.grid, stream);
   return g.variant == 2 ? launch_gemm_blockscaled(g.p, g.fp4, g.out_bf16, g.grid, stream)
                         : launch_gemm_solo(g.p, g.fp4, g.out_bf16, g.grid, stream);
@@ -212,6 +213,33 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
   const int sv = fmt == 1 ? 16 : 32;
   const int variant = (gather.nranks > 0 || rq || epi || fmt == 2) ? 1 : gemm_variant(fp4, m);
   const bool pair = variant == 1;
+  if (epi && m <= 128) {
+    // Few rows: the weights stream past them (gemm_fused_rows.cu).  Against the
+    // pair kernel, whose 256-row tile would be mostly empty: MXFP8 1 x 28672 x
+    // 4096 gated and 64 x 4096 x 14336 (see the kernel's file for the figures).
+    GemmParams& p = out->p;
+    std::memset(&p, 0, sizeof(p));
+    const int sets = epi->act == QG_ACT_SWIGLU ? 2 : 1;
+    const int chunks = pair_sf_chunks_per_stage(fmt);
+    if (!make_operand_map(&p.tm_a, b_q, n, row_bytes, 128 * sets) ||
+        !make_operand_map(&p.tm_b, a_q, m, row_bytes, rows_mma_n(m)) ||
+        !make_scale_map(&p.tm_sfa, b_sf, n, k, sv, sf_layout, sets, chunks) ||
+        !make_scale_map(&p.tm_sfb, a_sf, m, k, sv, sf_layout, 1, chunks))
+      return QG_ERR_CUDA;
+    p.m = static_cast<int>(m);
+    p.n = static_cast<int>(n);
+    p.k = static_cast<int>(k);
+    p.num_n_tiles = static_cast<int>((n + 128 * sets - 1) / (128 * sets));
+    p.num_k_blocks = static_cast<int>((row_bytes + 127) / 128);
+    p.epi = *epi;
+    p.a_ts = fmt == 1 ? a_ts : nullptr;
+    p.b_ts = fmt == 1 ? b_ts : nullptr;
+    p.status = status;
+    p.timeout_ns = default_timeout_ns();
+    out->fmt = fmt;
+    out->rows = true;
+    return QG_OK;
+  }
   // Tile of one scheduling unit (a CTA pair: 256 x 256; one CTA: 128 x 256)
   // and the rows each CTA's TMA boxes cover.
   const int tm = pair ? pair_tile_m() : gemm_tile_m();

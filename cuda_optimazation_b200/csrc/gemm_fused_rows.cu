@@ -1,0 +1,438 @@
+// gemm_fused_rows.cu -- the fused-epilogue block-scaled GEMM for few rows
+// (m <= 128: single tokens, decoding batches).
+//
+// The product is bound by streaming the weights B [n][k] once, so they are the
+// MMA's M side: D[128 weight rows][kN activation rows] in TMEM, one weight tile
+// (the gated form: the 128 gate rows and their 128 factor rows) per cluster.  The
+// clusters' CTAs split K, as many as keep every SM streaming (two CTAs an SM
+// where their accumulators and rings fit, one otherwise): a CTA's ring holds
+// ~100 KB, twice what HBM's latency asks of an SM.  The partial sums meet in
+// the cluster's shared memory, where every CTA sums and finishes its share
+// of the rows in a fixed order: no workspace, no atomics, one launch.
+//
+// Scales reach TMEM by tcgen05.cp: its fixed cost per 512-byte chunk, which the
+// large-m kernel avoids, hides behind the weight stream here.
+//
+// The epilogue runs across lanes (lane = column): 32 columns of a row, one MX
+// block, are one warp's, so a block's peak is one warp reduction.
+//
+// Roles (8 warps): warp 0 TMA producer, warp 1 MMA issuer (and TMEM owner),
+// warps 2..5 read the accumulator (one TMEM lane quadrant each); all eight finish
+// rows.  Every wait is bounded (qg_ptx.cuh).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "gemm_epilogue.cuh"
+#include "qg_codec.cuh"
+#include "qg_gemm.h"
+#include "qg_ptx.cuh"
+
+namespace qg {
+
+namespace {
+
+constexpr int kRowsFmtMxfp8 = 0, kRowsFmtNvfp4 = 1, kRowsFmtMxfp4 = 2;
+
+constexpr int pow2_at_least(int v) {
+  int p = 32;
+  while (p < v) p *= 2;
+  return p;
+}
+
+template <int kFmt, int kN, bool kGated>
+struct RowsCfg {
+  static constexpr int kSets = kGated ? 2 : 1;
+  static constexpr int kChunks = kFmt == kRowsFmtNvfp4 ? 4 : (kFmt == kRowsFmtMxfp4 ? 2 : 1);
+  static constexpr int kWBytes = kSets * 128 * 128;
+  static constexpr int kXBytes = kN * 128;
+  static constexpr int kSfwBytes = kSets * kChunks * 512;
+  static constexpr int kSfxBytes = kChunks * 512;
+  static constexpr int kTx = kWBytes + kXBytes + kSfwBytes + kSfxBytes;
+  static constexpr int kStageBytes = (kTx + 1023) / 1024 * 1024;
+  static constexpr int kSfCols = (kSets + 1) * kChunks * 4;  // scale columns of a stage
+  static constexpr int kAccCols = kSets * kN;
+  // Two CTAs an SM if both fit its 512 TMEM columns (more CTAs than TMEM for
+  // them would wait for one another inside their clusters).
+  static constexpr int kExtra = 256 + 1024;  // barriers, alignment
+  static constexpr int kStagesTwo = (228 * 1024 / 2 - 1024 - kExtra) / kStageBytes;
+  static constexpr bool kTwo = kAccCols + kStagesTwo * kSfCols <= 256;
+  static constexpr int kStagesOne =
+      (216 * 1024) / kStageBytes < (512 - kAccCols) / kSfCols ? (216 * 1024) / kStageBytes
+                                                              : (512 - kAccCols) / kSfCols;
+  static constexpr int kStages = kTwo ? kStagesTwo : kStagesOne;
+  static_assert(kStages >= 2, "ring");
+  static constexpr int kTmemCols = pow2_at_least(kAccCols + kStages * kSfCols);
+  // Rows whose partial sums are exchanged at a time (in the ring's memory).
+  static constexpr int kPass =
+      kSets * kN * 512 <= kStages * kStageBytes ? kN : kN / 2;
+  static_assert(kSets * kPass * 512 <= kStages * kStageBytes, "exchange buffer");
+  static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
+  // Never three CTAs on an SM, whose TMEM would not do.
+  static_assert(3 * (kSmemBytes + 1024) > 228 * 1024 && kTmemCols <= (kTwo ? 256 : 512),
+                "residency");
+  static constexpr int kPerSm = kTwo ? 2 : 1;
+};
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint32_t cluster_nctas() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+
+// One value per lane: the lane's byte of an MXFP8 row and, from lane 0, the scale
+// of the warp's block.  `in`: the block lies in the matrix.
+__device__ __forceinline__ void lane_store_mx(float v, bool in, uint8_t* q, uint8_t* sf,
+                                              int layout, int sf_blocks, int row, int col, int n,
+                                              int lane) {
+  const uint32_t bits = v == v ? __float_as_uint(fabsf(v)) : 0u;  // NaN has no part in the peak
+  float mul;
+  uint32_t code = mxfp8_scale_code(
+      __uint_as_float(__reduce_max_sync(0xffffffffu, in ? bits : 0u)), mul);
+  if (in) q[static_cast<int64_t>(row) * n + col] = static_cast<uint8_t>(cvt_e4m3x2(v * mul, 0.0f));
+  if (lane == 0) {
+    const int sc = col / 32;
+    if (layout == 0) {
+      if (in) sf[row * (n / 32) + sc] = static_cast<uint8_t>(code);
+    } else if (sc < sf_blocks * 4) {  // rows fit one 128-row block: both MMA orders agree
+      sf[mma_scale_offset(row, sc, 1, sf_blocks, layout)] = static_cast<uint8_t>(code);
+    }
+  }
+}
+
+// Zero scales of rows [m, 128) in the chunk of columns [col0, col0 + 128).
+__device__ __forceinline__ void pad_rows(uint8_t* sf, int layout, int sf_blocks, int col0, int m) {
+  const int w = threadIdx.x;
+  if (layout == 0 || w >= 128 || (w >> 2) + (w & 3) * 32 < m || col0 / 128 >= sf_blocks) return;
+  reinterpret_cast<uint32_t*>(sf + mma_scale_offset(0, col0 / 32, 1, sf_blocks, layout))[w] = 0u;
+}
+
+template <int kFmt, int kN, bool kGated>
+__global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
+    gemm_fused_rows_kernel(const __grid_constant__ GemmParams p) {
+  using Cfg = RowsCfg<kFmt, kN, kGated>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::kStages * Cfg::kStageBytes);
+  uint64_t* empty_bar = full_bar + Cfg::kStages;
+  uint64_t* acc_full = empty_bar + Cfg::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  static_assert(16 * Cfg::kStages + 16 <= 256, "barrier space");
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = static_cast<int>(cluster_ctarank()), ranks = static_cast<int>(cluster_nctas());
+  const int tile = static_cast<int>(cluster_id_x());
+  const int kb0 = static_cast<int>(static_cast<int64_t>(p.num_k_blocks) * rank / ranks);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(p.num_k_blocks) * (rank + 1) / ranks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0u;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int col0 = tile * Cfg::kSets * 128;  // first column of z
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA
+    if (lane == 0) {
+      const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+      uint32_t issued_mask = 0, issued_parity = 0, phase = 0;
+      int stage = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, p.timeout_ns, abort_flag, p.status,
+                               kDevTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        uint8_t* sw = smem + stage * Cfg::kStageBytes;
+        uint8_t* sx = sw + Cfg::kWBytes;
+        uint8_t* ssw = sx + Cfg::kXBytes;
+        uint8_t* ssx = ssw + Cfg::kSfwBytes;
+        mbar_arrive_expect_tx(&full_bar[stage], Cfg::kTx);
+        tma_load_2d(sw, &p.tm_a, &full_bar[stage], kb * 128, col0, pol_w);
+        tma_load_3d(ssw, &p.tm_sfa, &full_bar[stage], 0, col0 / 128, kb * Cfg::kChunks, pol_w);
+        tma_load_2d(sx, &p.tm_b, &full_bar[stage], kb * 128, 0, pol_x);
+        tma_load_3d(ssx, &p.tm_sfb, &full_bar[stage], 0, 0, kb * Cfg::kChunks, pol_x);
+        issued_mask |= 1u << stage;
+        issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == Cfg::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) {
+        uint32_t dummy = 0;
+        for (int s = 0; s < Cfg::kStages; ++s)
+          if (issued_mask & (1u << s))
+            mbar_wait_bounded(&full_bar[s], (issued_parity >> s) & 1u, p.timeout_ns, &dummy,
+                              nullptr, 0);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA
+    if (lane == 0) {
+      const uint32_t idesc_base =
+          kFmt == kRowsFmtMxfp8
+              ? make_idesc_block_scaled(128, kN, 0u, 1u, 0u, 0u)
+              : make_idesc_block_scaled(128, kN, 1u, kFmt == kRowsFmtMxfp4 ? 1u : 0u, 0u, 0u);
+      int stage = 0;
+      uint32_t phase = 0, acc = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_bounded(&full_bar[stage], phase, p.timeout_ns, abort_flag, p.status,
+                               kDevTimeoutMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint8_t* sw = smem + stage * Cfg::kStageBytes;
+        uint8_t* ssw = sw + Cfg::kWBytes + Cfg::kXBytes;
+        uint8_t* ssx = ssw + Cfg::kSfwBytes;
+        const uint32_t sfx_col = tmem_base + Cfg::kAccCols + stage * Cfg::kSfCols;
+        const uint32_t sfw_col = sfx_col + Cfg::kChunks * 4;
+#pragma unroll
+        for (int c = 0; c < Cfg::kChunks; ++c) {
+          tmem_cp_32x128b_warpx4(sfx_col + c * 4,
+                                 make_smem_desc(smem_u32(ssx + c * 512), 0, 128, kSwizzleNone));
+#pragma unroll
+          for (int s = 0; s < Cfg::kSets; ++s)
+            tmem_cp_32x128b_warpx4(
+                sfw_col + (s * Cfg::kChunks + c) * 4,
+                make_smem_desc(smem_u32(ssw + (c * Cfg::kSets + s) * 512), 0, 128, kSwizzleNone));
+        }
+        const uint64_t xdesc = make_smem_desc(smem_u32(sw + Cfg::kWBytes), 16, 1024, kSwizzle128B);
+#pragma unroll
+        for (int s = 0; s < Cfg::kSets; ++s) {
+          const uint64_t wdesc = make_smem_desc(smem_u32(sw + s * 16384), 16, 1024, kSwizzle128B);
+          const uint32_t d = tmem_base + s * kN;
+          const uint32_t sfw = sfw_col + s * Cfg::kChunks * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint64_t koff = static_cast<uint64_t>(j * 2);  // +32 B of K
+            const uint32_t on = acc | (j > 0 ? 1u : 0u);
+            if (kFmt == kRowsFmtMxfp8) {
+              const uint32_t id = idesc_base | (static_cast<uint32_t>(j) << 29) |
+                                  (static_cast<uint32_t>(j) << 4);
+              mma_mxf8f6f4(d, wdesc + koff, xdesc + koff, id, sfw, sfx_col, on);
+            } else if (kFmt == kRowsFmtMxfp4) {
+              const uint32_t sid = static_cast<uint32_t>((j & 1) * 2);
+              mma_mxf4(d, wdesc + koff, xdesc + koff, idesc_base | (sid << 29) | (sid << 4),
+                       sfw + (j / 2) * 4, sfx_col + (j / 2) * 4, on);
+            } else {
+              mma_mxf4nvf4(d, wdesc + koff, xdesc + koff, idesc_base, sfw + j * 4,
+                           sfx_col + j * 4, on);
+            }
+          }
+        }
+        acc = 1u;
+        tc_commit(&empty_bar[stage]);
+        if (++stage == Cfg::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      tc_commit(acc_full);
+      if (!ok) {
+        // Let the MMAs that were issued finish before the roles meet.
+        uint32_t dummy = 0;
+        mbar_wait_bounded(acc_full, 0, p.timeout_ns, &dummy, nullptr, 0);
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ epilogue
+  float alpha = 1.0f;
+  if (p.a_ts) alpha *= *p.a_ts;
+  if (p.b_ts) alpha *= *p.b_ts;
+  const EpiParams& e = p.epi;
+  const int f = threadIdx.x & 127;
+  const int n_out = kGated ? p.n / 2 : p.n;
+  const int out_col = (kGated ? tile * 128 : col0) + f;
+  const bool in_z = col0 + f < p.n;  // gated: n is a multiple of 256, so both sets are in
+  float bias[Cfg::kSets];
+#pragma unroll
+  for (int s = 0; s < Cfg::kSets; ++s) {
+    bias[s] = 0.0f;
+    if (e.bias && in_z) {
+      const int c = col0 + s * 128 + f;
+      bias[s] = e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[c])
+                            : static_cast<const float*>(e.bias)[c];
+    }
+  }
+  float* part = reinterpret_cast<float*>(smem);  // [set][row of the pass][128]
+  const uint32_t part_addr = smem_u32(part);
+  bool ok = true;
+  if (warp >= 2 && warp <= 5) {
+    if (lane == 0)
+      ok = mbar_wait_bounded<false, 32>(acc_full, 0, p.timeout_ns, abort_flag, p.status,
+                                        kDevTimeoutEpilogue);
+    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    if (ok) mbar_try_wait(acc_full, 0);
+    tc_fence_after();
+  }
+#pragma unroll 1
+  for (int t0 = 0; t0 < kN && t0 < p.m; t0 += Cfg::kPass) {
+    if (warp >= 2 && warp <= 5 && ok) {
+      const int quad = warp % 4;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+#pragma unroll 1
+      for (int s = 0; s < Cfg::kSets; ++s) {
+#pragma unroll 1
+        for (int c = 0; c < Cfg::kPass && t0 + c < p.m; c += 16) {
+          uint32_t r[16];
+          __syncwarp();
+          tmem_ld_32x32b_x16(t_row + s * kN + t0 + c, r);
+          tmem_wait_ld();
+          float* to = part + (s * Cfg::kPass + c) * 128 + quad * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) to[j * 128] = __uint_as_float(r[j]);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // every CTA's partial sums are in place
+    for (int i = rank * 2 + (threadIdx.x >> 7); i < Cfg::kPass && t0 + i < p.m; i += 2 * ranks) {
+      const int row = t0 + i;
+      float z[Cfg::kSets];
+#pragma unroll
+      for (int s = 0; s < Cfg::kSets; ++s) {
+        z[s] = 0.0f;
+        for (int r = 0; r < ranks; ++r)
+          z[s] += ld_cluster_f32(
+              mapa_shared(part_addr + ((s * Cfg::kPass + i) * 128 + f) * 4, static_cast<uint32_t>(r)));
+        z[s] = z[s] * alpha + bias[s];
+        if (e.z_q)
+          lane_store_mx(z[s], in_z, e.z_q, e.z_sf, e.z_layout, e.z_sf_blocks, row,
+                        col0 + s * 128 + f, p.n, lane);
+      }
+      float y;
+      if constexpr (kGated) {
+        y = act_fwd<kActSilu>(z[0]) * z[1];
+      } else {
+        y = z[0];
+        if (e.act == kActRelu) y = act_fwd<kActRelu>(y);
+        else if (e.act == kActSilu) y = act_fwd<kActSilu>(y);
+        else if (e.act == kActGelu) y = act_fwd<kActGelu>(y);
+      }
+      if (e.res && in_z) {
+        const int64_t at = row * e.ldr + out_col;
+        y += e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at])
+                        : static_cast<const float*>(e.res)[at];
+      }
+      if (e.out_kind == kEpiMxfp8) {
+        lane_store_mx(y, in_z, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout,
+                      e.out_sf_blocks, row, out_col, n_out, lane);
+      } else if (in_z) {
+        const int64_t at = row * e.ldc + out_col;
+        if (e.out_kind == kEpiBf16)
+          static_cast<__nv_bfloat16*>(e.out)[at] = __float2bfloat16_rn(y);
+        else
+          static_cast<float*>(e.out)[at] = y;
+      }
+    }
+    cluster_sync();  // the sums have been read: reuse the buffer, or exit
+  }
+  if (rank == 0) {
+    if (e.out_kind == kEpiMxfp8)
+      pad_rows(e.out_sf, e.out_layout, e.out_sf_blocks, out_col - f, p.m);
+    if (e.z_q) {
+#pragma unroll
+      for (int s = 0; s < Cfg::kSets; ++s)
+        pad_rows(e.z_sf, e.z_layout, e.z_sf_blocks, col0 + s * 128, p.m);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+// CTAs per cluster: as many (a power of two, 8 at most) as find a place on the
+// SMs at once, with at least two K blocks each.
+int cluster_size(int tiles, int k_blocks, int slots) {
+  int c = 1;
+  while (c < 8 && tiles * 2 * c <= slots && k_blocks >= 4 * c) c *= 2;
+  return c;
+}
+
+template <int kFmt, int kN, bool kGated>
+cudaError_t launch_rows(const GemmParams& p, cudaStream_t stream) {
+  using Cfg = RowsCfg<kFmt, kN, kGated>;
+  auto kernel = gemm_fused_rows_kernel<kFmt, kN, kGated>;
+  static bool done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
+    return cudaErrorInvalidDevice;
+  if (!done[dev]) {
+    const cudaError_t err =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (err != cudaSuccess) return err;
+    done[dev] = true;
+  }
+  const int tiles = p.num_n_tiles;
+  const int c = cluster_size(tiles, p.num_k_blocks, num_sms() * Cfg::kPerSm);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * c);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(c);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int kFmt, bool kGated>
+cudaError_t launch_rows_n(const GemmParams& p, cudaStream_t stream) {
+  switch (rows_mma_n(p.m)) {
+    case 16: return launch_rows<kFmt, 16, kGated>(p, stream);
+    case 32: return launch_rows<kFmt, 32, kGated>(p, stream);
+    case 64: return launch_rows<kFmt, 64, kGated>(p, stream);
+    default: return launch_rows<kFmt, 128, kGated>(p, stream);
+  }
+}
+
+}  // namespace
+
+int rows_mma_n(int64_t m) { return m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128)); }
+
+cudaError_t launch_gemm_fused_rows(const GemmParams& p, int fmt, cudaStream_t stream) {
+  const bool gated = p.epi.act == kActSwiglu;
+  if (fmt == kRowsFmtNvfp4)
+    return gated ? launch_rows_n<kRowsFmtNvfp4, true>(p, stream)
+                 : launch_rows_n<kRowsFmtNvfp4, false>(p, stream);
+  if (fmt == kRowsFmtMxfp4)
+    return gated ? launch_rows_n<kRowsFmtMxfp4, true>(p, stream)
+                 : launch_rows_n<kRowsFmtMxfp4, false>(p, stream);
+  return gated ? launch_rows_n<kRowsFmtMxfp8, true>(p, stream)
+               : launch_rows_n<kRowsFmtMxfp8, false>(p, stream);
+}
+
+}  // namespace qg

@@ -142,6 +142,11 @@ cudaError_t launch_gemm_blockscaled(const GemmParams& p, bool fp4, bool out_bf16
 cudaError_t launch_gemm_pair(const GemmParams& p, int fmt, int out_kind, int grid,
                              cudaStream_t stream);
 int pair_sf_chunks_per_stage(int fmt);
+// The fused-epilogue GEMM for m <= 128 rows (gemm_fused_rows.cu): tm_a / tm_sfa
+// are the weights B (box 128 rows, 256 for the gated activation), tm_b /
+// tm_sfb the rows A (box rows_mma_n(m)); num_n_tiles tiles of the weights' boxes.
+cudaError_t launch_gemm_fused_rows(const GemmParams& p, int fmt, cudaStream_t stream);
+int rows_mma_n(int64_t m);
 cudaError_t launch_gemm_solo(const GemmParams& p, bool fp4, bool out_bf16, int grid,
                              cudaStream_t stream);
 int pair_tile_m();

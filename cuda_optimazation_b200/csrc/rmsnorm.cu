@@ -109,14 +109,16 @@ __device__ __forceinline__ void store8(void* base, int64_t elem, const Vec8& x) 
 // vectors and then (fp32) the second ones, so that a warp's accesses are
 // contiguous.
 template <bool kBf16>
-__device__ __forceinline__ void ring_copy(uint8_t* slot, const void* base, int64_t elem, int v,
-                                          int nvec) {
-  const uint8_t* g = static_cast<const uint8_t*>(base) + (elem + v * 8) * kElem<kBf16>;
+__device__ __forceinline__ const uint8_t* at_row(const void* base, int64_t row, int64_t ld) {
+  return static_cast<const uint8_t*>(base) + row * ld * kElem<kBf16>;
+}
+template <bool kBf16>
+__device__ __forceinline__ void ring_copy(uint8_t* slot, const uint8_t* row, int v, int nvec) {
 #pragma unroll
   for (int i = 0; i < Raw8<kBf16>::kChunks; ++i)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
                      smem_u32(slot + (i * nvec + v) * 16)),
-                 "l"(g + 16 * i)
+                 "l"(row + v * 8 * kElem<kBf16> + 16 * i)
                  : "memory");
 }
 template <bool kBf16>
@@ -150,49 +152,67 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
-__device__ __forceinline__ float sum4(float2 a, float2 b, float2 c, float2 d) {
-  const float2 s = add2(add2(a, b), add2(c, d));
-  return s.x + s.y;
-}
-
-__device__ __forceinline__ float square_sum(const Vec8& h) {
-  return sum4(mul2(h.v[0], h.v[0]), mul2(h.v[1], h.v[1]), mul2(h.v[2], h.v[2]),
-              mul2(h.v[3], h.v[3]));
-}
-
-// y of one vector, quantised and stored.  Every lane of the warp takes part;
-// `in` says whether the vector lies in the row.
-__device__ __forceinline__ void store_y(const RmsNormParams& p, int64_t row, int v, bool in,
-                                        const Vec8& h, const Vec8& w, float rstd, int lane) {
-  Vec8 y;
-  float amax = 0.0f;
-  if (in) {
+__device__ __forceinline__ void add_to(Vec8& a, const Vec8& b) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y.v[i] = mul2(mul2(h.v[i], both(rstd)), w.v[i]);
-      amax = fmaxf(fmaxf(amax, fabsf(y.v[i].x)), fabsf(y.v[i].y));
-    }
-  }
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  for (int i = 0; i < 4; ++i) a.v[i] = add2(a.v[i], b.v[i]);
+}
+__device__ __forceinline__ void add_squares(float2& s, const Vec8& h) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = fma2(h.v[i], h.v[i], s);
+}
+
+// Where a row's scale words go: `at` for its first four blocks, `step` bytes
+// further for each four more (the MMA layouts).
+struct ScaleRow {
+  uint8_t* at;
+  int64_t step;
+};
+__device__ __forceinline__ ScaleRow scale_row(const RmsNormParams& p, int64_t row) {
+  const int64_t in_chunk = (row & 31) * 16 + (row >> 5 & 3) * 4, br = row >> 7;
+  if (p.layout == 1) return {p.sf + br * 512 + in_chunk, p.row_blocks * 512};
+  if (p.layout == 2) return {p.sf + br * p.sf_blocks * 512 + in_chunk, 512};
+  return {p.sf + row * (p.k / 32), 0};
+}
+
+// t = h * w of one vector (y without rstd) and the peak |t| of its MX block.
+// Formed before the row's sum is known, so that little is left after it; the
+// peak of y is the peak of t times rstd (rounding is monotonic).  Every lane of
+// the warp takes part; a lane beyond the row brings zeros.
+__device__ __forceinline__ float weighted(const Vec8& h, const Vec8& w, Vec8& t) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t.v[i] = mul2(h.v[i], w.v[i]);
+  float peak = max3_abs(t.v[0].x, t.v[0].y, t.v[1].x);
+  peak = max3_abs(peak, t.v[1].y, t.v[2].x);
+  peak = max3_abs(peak, t.v[2].y, t.v[3].x);
+  return max3_abs(peak, t.v[3].y, 0.0f);
+}
+__device__ __forceinline__ float block_peak(float peak) {
+  peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+  return fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+}
+
+// y = t * rstd of vector v, quantised and stored (q: the row's values).
+__device__ __forceinline__ void store_y(const RmsNormParams& p, uint8_t* q, const ScaleRow& sr,
+                                        int v, bool in, const Vec8& t, float peak, float rstd,
+                                        int lane) {
   float mul;
-  const uint32_t code = mxfp8_scale_code(amax, mul);  // 0 beyond the row: padding
+  const uint32_t code = mxfp8_scale_code(fmaxf(peak * rstd, 0.0f), mul);  // 0 beyond the row: padding
   if (in) {
+    // Two products: rstd * mul may overflow where t is 0.
+    float2 y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y.v[i] = mul2(y.v[i], both(mul));
-    *reinterpret_cast<uint2*>(p.q + row * p.k + v * 8) =
-        make_uint2(cvt_e4m3x4(y.v[0].x, y.v[0].y, y.v[1].x, y.v[1].y),
-                   cvt_e4m3x4(y.v[2].x, y.v[2].y, y.v[3].x, y.v[3].y));
+    for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(t.v[i], both(rstd)), both(mul));
+    *reinterpret_cast<uint2*>(q + v * 8) = make_uint2(
+        cvt_e4m3x4(y[0].x, y[0].y, y[1].x, y[1].y), cvt_e4m3x4(y[2].x, y[2].y, y[3].x, y[3].y));
   }
   if (p.layout == 0) {
-    if (in && (lane & 3) == 0) p.sf[row * (p.k / 32) + v / 4] = static_cast<uint8_t>(code);
+    if (in && (lane & 3) == 0) sr.at[v / 4] = static_cast<uint8_t>(code);
   } else {
     // Codes of the word's four blocks, joined over lanes 0, 4, 8, 12 of 16.
     uint32_t word = code | __shfl_down_sync(0xffffffffu, code, 4) << 8;
     word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
     if (in && (lane & 15) == 0)
-      *reinterpret_cast<uint32_t*>(
-          p.sf + mma_scale_offset(row, v / 4, p.row_blocks, p.sf_blocks, p.layout)) = word;
+      *reinterpret_cast<uint32_t*>(sr.at + (v / 16) * sr.step) = word;
   }
 }
 
@@ -224,30 +244,30 @@ __global__ void __launch_bounds__(1024) rmsnorm_direct_kernel(const RmsNormParam
     return;
   }
   const int nvec = static_cast<int>(p.k / 8);
-  Vec8 h[kVec];
-  Raw8<kWBf16> w[kVec];
-  float ss = 0.0f;
+  Vec8 t[kVec];
+  float peak[kVec];
+  float2 ss = make_float2(0.0f, 0.0f);
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
+    peak[i] = 0.0f;
     if (v < nvec) {
-      h[i] = load_once<kBf16>(p.x, row * p.ldx + v * 8).decode();
-      w[i] = load_kept<kWBf16>(p.weight, v * 8);
-      if (p.residual) {
-        const Vec8 r = load_once<kBf16>(p.residual, row * p.ldr + v * 8).decode();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[i].v[j] = add2(h[i].v[j], r.v[j]);
-      }
-      if (p.h) store8<kBf16>(p.h, row * p.ldh + v * 8, h[i]);
-      ss += square_sum(h[i]);
+      Vec8 h = load_once<kBf16>(p.x, row * p.ldx + v * 8).decode();
+      const Vec8 w = load_kept<kWBf16>(p.weight, v * 8).decode();
+      if (p.residual) add_to(h, load_once<kBf16>(p.residual, row * p.ldr + v * 8).decode());
+      if (p.h) store8<kBf16>(p.h, row * p.ldh + v * 8, h);
+      add_squares(ss, h);
+      peak[i] = weighted(h, w, t[i]);
     }
+    peak[i] = block_peak(peak[i]);
   }
-  const float rstd = rsqrtf(row_sum(ss, red) / static_cast<float>(p.k) + p.eps);
+  const float rstd = rsqrtf(row_sum(ss.x + ss.y, red) / static_cast<float>(p.k) + p.eps);
   if (threadIdx.x == 0 && p.rstd) p.rstd[row] = rstd;
+  const ScaleRow sr = scale_row(p, row);
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    store_y(p, row, v, v < nvec, h[i], w[i].decode(), rstd, threadIdx.x & 31);
+    store_y(p, p.q + row * p.k, sr, v, v < nvec, t[i], peak[i], rstd, threadIdx.x & 31);
   }
 }
 
@@ -262,56 +282,67 @@ __global__ void __launch_bounds__(512) rmsnorm_ring_kernel(const RmsNormParams p
   uint8_t* mine = ring + threadIdx.y * kStages * slot_bytes;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-  auto fetch = [&](int64_t row, int stage) {
+  const uint8_t* x_next = at_row<kBf16>(p.x, first, p.ldx);
+  const uint8_t* r_next = at_row<kBf16>(p.residual, first, p.ldr);
+  const int64_t x_step = step * p.ldx * kElem<kBf16>, r_step = step * p.ldr * kElem<kBf16>;
+  // Starts copying row `row`, and moves on by `step` rows.
+  auto fetch = [&](int64_t row, uint8_t* slot) {
     if (row < p.rows) {
-      uint8_t* slot = mine + stage * slot_bytes;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
         const int v = threadIdx.x + i * blockDim.x;
         if (v < nvec) {
-          ring_copy<kBf16>(slot, p.x, row * p.ldx, v, nvec);
-          if (p.residual) ring_copy<kBf16>(slot + row_bytes, p.residual, row * p.ldr, v, nvec);
+          ring_copy<kBf16>(slot, x_next, v, nvec);
+          if (p.residual) ring_copy<kBf16>(slot + row_bytes, r_next, v, nvec);
         }
       }
     }
+    x_next += x_step;
+    r_next += r_step;
     ring_commit();
   };
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) fetch(first + s * step, s);
-  int stage = 0;
+  for (int s = 0; s < kStages; ++s) fetch(first + s * step, mine + s * slot_bytes);
+  Raw8<kWBf16> w[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) w[i] = load_kept<kWBf16>(p.weight, v * 8);
+  }
+  uint8_t* slot = mine;
+  uint8_t* q = p.q + first * p.k;
+  uint8_t* h_out = static_cast<uint8_t*>(p.h) + first * p.ldh * kElem<kBf16>;
   for (int64_t row = first; row < p.rows; row += step) {
     ring_wait<kStages - 1>();
-    const uint8_t* slot = mine + stage * slot_bytes;
-    Vec8 h[kVec];
-    float ss = 0.0f;
+    Vec8 t[kVec];
+    float peak[kVec];
+    float2 ss = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
+      peak[i] = 0.0f;
       if (v < nvec) {
-        h[i] = ring_read<kBf16>(slot, v, nvec).decode();
-        if (p.residual) {
-          const Vec8 r = ring_read<kBf16>(slot + row_bytes, v, nvec).decode();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) h[i].v[j] = add2(h[i].v[j], r.v[j]);
-        }
-        ss += square_sum(h[i]);
+        Vec8 h = ring_read<kBf16>(slot, v, nvec).decode();
+        if (p.residual) add_to(h, ring_read<kBf16>(slot + row_bytes, v, nvec).decode());
+        if (p.h) store8<kBf16>(h_out, v * 8, h);
+        add_squares(ss, h);
+        peak[i] = weighted(h, w[i].decode(), t[i]);
       }
+      peak[i] = block_peak(peak[i]);
     }
-    fetch(row + kStages * step, stage);
-    if (++stage == kStages) stage = 0;
-    const float rstd = rsqrtf(row_sum(ss, red) / static_cast<float>(p.k) + p.eps);
+    fetch(row + kStages * step, slot);
+    slot += slot_bytes;
+    if (slot == mine + kStages * slot_bytes) slot = mine;
+    const float rstd = rsqrtf(row_sum(ss.x + ss.y, red) / static_cast<float>(p.k) + p.eps);
     if (threadIdx.x == 0 && p.rstd) p.rstd[row] = rstd;
+    const ScaleRow sr = scale_row(p, row);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
-      const bool in = v < nvec;
-      Vec8 w;
-      if (in) {
-        if (p.h) store8<kBf16>(p.h, row * p.ldh + v * 8, h[i]);
-        w = load_kept<kWBf16>(p.weight, v * 8).decode();
-      }
-      store_y(p, row, v, in, h[i], w, rstd, threadIdx.x & 31);
+      store_y(p, q, sr, v, v < nvec, t[i], peak[i], rstd, threadIdx.x & 31);
     }
+    q += step * p.k;
+    h_out += step * p.ldh * kElem<kBf16>;
   }
   ring_wait<0>();
   const int t = threadIdx.y * blockDim.x + threadIdx.x, n = blockDim.x * blockDim.y;
@@ -377,11 +408,7 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_direct_kernel(const RmsN
       const int v = threadIdx.x + i * blockDim.x;
       if (v < nvec) {
         Vec8 d = bwd_dx(dy[i].decode(), h[i].decode(), w[i].decode(), rstd, c);
-        if (p.dres) {
-          const Vec8 r = load_once<kBf16>(p.dres, row * p.lddres + v * 8).decode();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) d.v[j] = add2(d.v[j], r.v[j]);
-        }
+        if (p.dres) add_to(d, load_once<kBf16>(p.dres, row * p.lddres + v * 8).decode());
         store8<kBf16>(p.dx, row * p.lddx + v * 8, d);
       }
     }
@@ -408,19 +435,26 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNor
   uint8_t* mine = ring + threadIdx.y * kStages * slot_bytes;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-  auto fetch = [&](int64_t row, int stage) {
+  const uint8_t* dy_next = at_row<kBf16>(p.dy, first, p.lddy);
+  const uint8_t* h_next = at_row<kBf16>(p.h, first, p.ldh);
+  const uint8_t* r_next = at_row<kBf16>(p.dres, first, p.lddres);
+  const int64_t dy_step = step * p.lddy * kElem<kBf16>, h_step = step * p.ldh * kElem<kBf16>,
+                r_step = step * p.lddres * kElem<kBf16>;
+  auto fetch = [&](int64_t row, uint8_t* slot) {
     if (row < p.rows) {
-      uint8_t* slot = mine + stage * slot_bytes;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
         const int v = threadIdx.x + i * blockDim.x;
         if (v < nvec) {
-          ring_copy<kBf16>(slot, p.dy, row * p.lddy, v, nvec);
-          ring_copy<kBf16>(slot + row_bytes, p.h, row * p.ldh, v, nvec);
-          if (p.dres) ring_copy<kBf16>(slot + 2 * row_bytes, p.dres, row * p.lddres, v, nvec);
+          ring_copy<kBf16>(slot, dy_next, v, nvec);
+          ring_copy<kBf16>(slot + row_bytes, h_next, v, nvec);
+          if (p.dres) ring_copy<kBf16>(slot + 2 * row_bytes, r_next, v, nvec);
         }
       }
     }
+    dy_next += dy_step;
+    h_next += h_step;
+    r_next += r_step;
     ring_commit();
   };
   Vec8 dw[kVec];
@@ -433,12 +467,12 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNor
     if (v < nvec) w[i] = load_kept<kWBf16>(p.weight, v * 8);
   }
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) fetch(first + s * step, s);
-  int stage = 0;
+  for (int s = 0; s < kStages; ++s) fetch(first + s * step, mine + s * slot_bytes);
+  uint8_t* slot = mine;
+  uint8_t* out = static_cast<uint8_t*>(p.dx) + first * p.lddx * kElem<kBf16>;
   for (int64_t row = first; row < p.rows; row += step) {
     const float rstd = __ldg(p.rstd + row);
     ring_wait<kStages - 1>();
-    const uint8_t* slot = mine + stage * slot_bytes;
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
@@ -456,16 +490,14 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNor
         Vec8 d = bwd_dx(ring_read<kBf16>(slot, v, nvec).decode(),
                         ring_read<kBf16>(slot + row_bytes, v, nvec).decode(), w[i].decode(), rstd,
                         c);
-        if (p.dres) {
-          const Vec8 r = ring_read<kBf16>(slot + 2 * row_bytes, v, nvec).decode();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) d.v[j] = add2(d.v[j], r.v[j]);
-        }
-        store8<kBf16>(p.dx, row * p.lddx + v * 8, d);
+        if (p.dres) add_to(d, ring_read<kBf16>(slot + 2 * row_bytes, v, nvec).decode());
+        store8<kBf16>(out, v * 8, d);
       }
     }
-    fetch(row + kStages * step, stage);
-    if (++stage == kStages) stage = 0;
+    fetch(row + kStages * step, slot);
+    slot += slot_bytes;
+    if (slot == mine + kStages * slot_bytes) slot = mine;
+    out += step * p.lddx * kElem<kBf16>;
   }
   ring_wait<0>();
   if (!p.dw_part) return;

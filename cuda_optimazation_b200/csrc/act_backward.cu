@@ -127,8 +127,11 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
   const int warp = (threadIdx.x >> 5) & 3, group = threadIdx.x >> 7, lane = threadIdx.x & 31;
   const int rg = lane >> 2, cg = lane & 3;
   const int col_tiles = static_cast<int>((p.n + kSets * kTile - 1) / (kSets * kTile));
-  const int tm = static_cast<int>(blockIdx.x) / col_tiles;
-  const int tc = static_cast<int>(blockIdx.x) % col_tiles;
+  const int row_tiles = static_cast<int>((p.m + kTile - 1) / kTile);
+  // All groups at once: the row tiles of a column tile are neighbours, and one
+  // cluster where p.cluster_rows says so.
+  const int tm = static_cast<int>(kGroups > 1 ? blockIdx.x % row_tiles : blockIdx.x / col_tiles);
+  const int tc = static_cast<int>(kGroups > 1 ? blockIdx.x / row_tiles : blockIdx.x % col_tiles);
   const int64_t m0 = static_cast<int64_t>(tm) * kTile;
   const int rows = static_cast<int>(p.m - m0 < kTile ? p.m - m0 : kTile);
   // This lane's first column of z (of the gate set) and of dout.
@@ -370,11 +373,26 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
     }
   }
   if constexpr (kGrad && kGroups > 1) {
-    const int64_t col = static_cast<int64_t>(tc) * kSets * kTile + threadIdx.x;
-    if (p.dbias_part && threadIdx.x < kSets * kTile && col < p.n) {
-      float t = part[0][threadIdx.x];
-      for (int g = 1; g < kGroups && g * 32 < rows; ++g) t += part[g][threadIdx.x];
-      p.dbias_part[tm * p.n + col] = t;
+    if (p.dbias_part) {
+      const int64_t col = static_cast<int64_t>(tc) * kSets * kTile + threadIdx.x;
+      const bool in = threadIdx.x < kSets * kTile && col < p.n;
+      float t = 0.0f;
+      if (in)
+        for (int g = 0; g < kGroups && g * 32 < rows; ++g) t += part[g][threadIdx.x];
+      if (!p.cluster_rows) {
+        if (in) p.dbias_part[tm * p.n + col] = t;
+      } else {
+        // The column tile's row tiles are this cluster: the first sums them up.
+        if (in) part[0][threadIdx.x] = t;
+        cluster_sync();
+        if (tm == 0 && in) {
+          for (int r = 1; r < row_tiles; ++r)
+            t += ld_cluster_f32(
+                mapa_shared(smem_u32(&part[0][threadIdx.x]), static_cast<uint32_t>(r)));
+          p.dbias_part[col] = t;
+        }
+        cluster_sync();  // the others' shared memory has been read
+      }
     }
   }
 }
@@ -382,7 +400,9 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
 // Few tiles: all four row groups of a tile at once, for latency; enough tiles to
 // fill the SMs with 128-thread CTAs several times: one group after the other.
 constexpr int kGroupsSmall = 4;
-bool small_grid(int grid) { return grid < 4 * num_sms(); }
+bool small_grid(int64_t grid) { return grid < 4 * num_sms(); }
+// Row tiles that a cluster may join (the portable size).
+constexpr int kClusterRows = 8;
 
 template <int kAct, bool kBf16, int kGroups>
 cudaError_t launch_one(const ActBackwardParams& p, int grid, cudaStream_t stream) {
@@ -398,6 +418,21 @@ cudaError_t launch_one(const ActBackwardParams& p, int grid, cudaStream_t stream
     if (e != cudaSuccess) return e;
     done[dev] = true;
   }
+  if (p.cluster_rows) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(128 * kGroups);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>((p.m + kTile - 1) / kTile);
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+  }
   kernel<<<grid, 128 * kGroups, kSmem, stream>>>(p);
   return cudaGetLastError();
 }
@@ -408,16 +443,23 @@ cudaError_t launch_act(const ActBackwardParams& p, int grid, cudaStream_t stream
                           : launch_one<kAct, kBf16, 1>(p, grid, stream);
 }
 
-int act_grid(const ActBackwardParams& p, int sets) {
-  return static_cast<int>(((p.m + kTile - 1) / kTile) *
-                          ((p.n + sets * kTile - 1) / (sets * kTile)));
+int64_t act_grid(int64_t m, int64_t n, int sets) {
+  return ((m + kTile - 1) / kTile) * ((n + sets * kTile - 1) / (sets * kTile));
 }
 
 }  // namespace
 
-cudaError_t launch_act_backward(const ActBackwardParams& p, int act, bool bf16,
+bool act_backward_joins(int64_t m, int64_t n, int act) {
+  const int64_t parts = (m + kTile - 1) / kTile;
+  return parts == 1 ||
+         (parts <= kClusterRows && small_grid(act_grid(m, n, act == kActSwiglu ? 2 : 1)));
+}
+
+cudaError_t launch_act_backward(const ActBackwardParams& in, int act, bool bf16,
                                 cudaStream_t stream) {
-  const int grid = act_grid(p, act == kActSwiglu ? 2 : 1);
+  ActBackwardParams p = in;
+  p.cluster_rows = p.dbias_part && p.m > kTile && act_backward_joins(p.m, p.n, act);
+  const int grid = static_cast<int>(act_grid(p.m, p.n, act == kActSwiglu ? 2 : 1));
 #define QG_ACT_CASE(a) \
   case a:              \
     return bf16 ? launch_act<a, true>(p, grid, stream) : launch_act<a, false>(p, grid, stream);
@@ -433,7 +475,7 @@ cudaError_t launch_act_backward(const ActBackwardParams& p, int act, bool bf16,
 }
 
 cudaError_t launch_transpose_mxfp8(const ActBackwardParams& p, cudaStream_t stream) {
-  return launch_act<-1, false>(p, act_grid(p, 1), stream);
+  return launch_act<-1, false>(p, static_cast<int>(act_grid(p.m, p.n, 1)), stream);
 }
 
 }  // namespace qg

@@ -614,7 +614,7 @@ int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh
                         int64_t lddres, int64_t rows, int64_t k, void* dx, int64_t lddx,
                         float* dweight, void* workspace, size_t workspace_bytes,
                         qg_stream_t stream) {
-  if (!dy || !h || !rstd || !weight || !dx) return QG_ERR_ARG;
+  if (!dy || !h || !rstd || !weight || !dx || dx == dy || dx == h) return QG_ERR_ARG;
   if (!float_dtype(x_dtype) || !float_dtype(w_dtype)) return QG_ERR_DTYPE;
   if (rows < 1 || rows > (1ll << 31) - 256 || k < 32 || k % 32 != 0 || k > kMaxNormK ||
       lddy < k || ldh < k || lddx < k || (dres && lddres < k))
@@ -624,9 +624,9 @@ int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh
       !aligned16(weight) || !aligned_to(rstd, 4) || !aligned_to(dweight, 4))
     return QG_ERR_ALIGN;
   if (dweight) {
-    if (!workspace || workspace_bytes < qg_rmsnorm_backward_workspace_bytes(rows, k))
-      return QG_ERR_ARG;
-    if (!aligned16(workspace)) return QG_ERR_ALIGN;
+    const size_t need = qg_rmsnorm_backward_workspace_bytes(rows, k);
+    if (need && (!workspace || workspace_bytes < need)) return QG_ERR_ARG;
+    if (need && !aligned16(workspace)) return QG_ERR_ALIGN;
   }
   if (int d = check_device()) return d;
   RmsNormBwdParams p{};
@@ -636,14 +636,15 @@ int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh
   p.dres = dres;
   p.rstd = rstd;
   p.dx = dx;
-  p.dw_part = dweight ? static_cast<float*>(workspace) : nullptr;
+  p.dw_part = static_cast<float*>(workspace);
+  p.dw = dweight;
   p.lddy = lddy;
   p.ldh = ldh;
   p.lddres = lddres;
   p.lddx = lddx;
   p.rows = rows;
   p.k = k;
-  return launch_rmsnorm_backward(p, x_dtype == QG_DTYPE_BF16, w_dtype == QG_DTYPE_BF16, dweight,
+  return launch_rmsnorm_backward(p, x_dtype == QG_DTYPE_BF16, w_dtype == QG_DTYPE_BF16,
                                  reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess
              ? QG_OK
              : QG_ERR_CUDA;
@@ -704,7 +705,8 @@ int qg_gemm_fused(int format, const void* a_q, const void* a_sf, const float* a_
 }
 
 size_t qg_act_backward_workspace_bytes(int64_t m, int64_t n) {
-  if (m < 1 || n < 1) return 0;
+  // QG_ACT_NONE's tiles are the most; what joins them joins every activation's.
+  if (m < 1 || n < 1 || act_backward_joins(m, n, QG_ACT_NONE)) return 0;
   return static_cast<size_t>((m + 127) / 128) * static_cast<size_t>(n) * 4;
 }
 
@@ -727,7 +729,8 @@ int qg_act_backward_mxfp8(const void* dout, int dout_dtype, int64_t ldd, const v
       !aligned16(dz_q) ||
       !aligned16(dz_sf) || !aligned16(dzt_q) || !aligned16(dzt_sf) || !aligned_to(dbias, 4))
     return QG_ERR_ALIGN;
-  if (dbias) {
+  const bool parts = dbias && !act_backward_joins(m, n, act);
+  if (parts) {
     if (!workspace || workspace_bytes < qg_act_backward_workspace_bytes(m, n)) return QG_ERR_ARG;
     if (!aligned16(workspace)) return QG_ERR_ALIGN;
   }
@@ -746,13 +749,12 @@ int qg_act_backward_mxfp8(const void* dout, int dout_dtype, int64_t ldd, const v
   p.dzt_sf = static_cast<uint8_t*>(dzt_sf);
   p.mt = (m + 31) / 32 * 32;
   p.out_layout = out_layout;
-  const int parts = static_cast<int>((m + 127) / 128);  // one row tile: its sums are dbias
-  p.dbias_part = dbias ? (parts > 1 ? static_cast<float*>(workspace) : dbias) : nullptr;
+  p.dbias_part = parts ? static_cast<float*>(workspace) : dbias;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (launch_act_backward(p, act, dout_dtype == QG_DTYPE_BF16, s) != cudaSuccess)
     return QG_ERR_CUDA;
-  if (dbias && parts > 1 &&
-      launch_column_sum(p.dbias_part, parts, n, dbias, s) != cudaSuccess)
+  if (parts && launch_column_sum(p.dbias_part, static_cast<int>((m + 127) / 128), n, dbias, s) !=
+                   cudaSuccess)
     return QG_ERR_CUDA;
   return QG_OK;
 }

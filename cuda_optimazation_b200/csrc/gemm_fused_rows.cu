@@ -74,12 +74,6 @@ struct RowsCfg {
   static constexpr int kPerSm = kTwo ? 2 : 1;
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 __device__ __forceinline__ uint32_t cluster_nctas() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));

@@ -200,14 +200,16 @@ struct RmsNormBwdParams {
   const void* dres;  // may be null
   const float* rstd;
   void* dx;
-  float* dw_part;    // [rmsnorm_backward_parts(rows, k)][k] at most; null: no dw
+  float* dw_part;    // [rmsnorm_backward_parts(rows, k)][k] at most
+  float* dw;         // [k]; null: not wanted
   int64_t lddy, ldh, lddres, lddx;
   int64_t rows, k;
 };
 cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
                                  cudaStream_t stream);
+// Rows of partial sums; 0 where the kernel writes dw itself.
 int rmsnorm_backward_parts(int64_t rows, int64_t k);
-cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16, float* dw,
+cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16,
                                     cudaStream_t stream);
 // out[c] = sum over r < parts of part[r][c], in a fixed order.
 cudaError_t launch_column_sum(const float* part, int parts, int64_t k, float* out,
@@ -228,8 +230,12 @@ struct ActBackwardParams {
   uint8_t* dzt_sf;
   int64_t mt;            // m rounded up to 32
   int out_layout;
-  float* dbias_part;     // [ceil(m / 128)][n]; null: no dbias
+  float* dbias_part;     // [ceil(m / 128)][n], or dbias itself where
+                         // act_backward_joins(); null: no dbias
+  int cluster_rows;      // set by the launch: a column tile's CTAs are one cluster
 };
+// Whether the kernel finishes dbias by itself (one row tile, or a cluster's).
+bool act_backward_joins(int64_t m, int64_t n, int act);
 cudaError_t launch_act_backward(const ActBackwardParams& p, int act, bool bf16,
                                 cudaStream_t stream);
 // dzt = z turned (dout, dz and dbias unused).

@@ -374,12 +374,58 @@ __device__ __forceinline__ Vec8 bwd_dx(const Vec8& dy, const Vec8& h, const Vec8
   return d;
 }
 
-// CTA b takes rows b, b + grid, ...; each thread owns the same columns of all
-// of them, so its share of dw stays in registers and is written once, to row b
-// of the partial sums.
-template <bool kBf16, bool kWBf16, int kVec>
+// dw of the 64 columns from col0 on, by one CTA: its warps take every
+// (warps)-th row, two columns a lane, and are joined in order.
+template <bool kBf16>
+__device__ __forceinline__ void column_dw(const RmsNormBwdParams& p, int64_t col0) {
+  __shared__ float2 sums[16][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int64_t col = col0 + 2 * lane;
+  float2 s = make_float2(0.0f, 0.0f);
+  if (col < p.k) {
+#pragma unroll 8
+    for (int row = warp; row < static_cast<int>(p.rows); row += warps) {
+      float2 d, h;
+      if constexpr (kBf16) {
+        const uint32_t a = __ldg(reinterpret_cast<const uint32_t*>(
+            static_cast<const __nv_bfloat16*>(p.dy) + row * p.lddy + col));
+        const uint32_t b = __ldg(reinterpret_cast<const uint32_t*>(
+            static_cast<const __nv_bfloat16*>(p.h) + row * p.ldh + col));
+        d = make_float2(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+        h = make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
+      } else {
+        d = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.dy) + row * p.lddy +
+                                                  col));
+        h = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.h) + row * p.ldh +
+                                                  col));
+      }
+      s = fma2(d, mul2(h, both(__ldg(p.rstd + row))), s);
+    }
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && col < p.k) {
+    for (int w = 1; w < warps; ++w) s = add2(s, sums[w][lane]);
+    p.dw[col] = s.x;
+    p.dw[col + 1] = s.y;
+  }
+}
+
+// kColumns (few rows): CTA b takes row b, and CTAs past the rows the columns of
+// dw, which need no row's sum: dy and h are read twice, the second time from
+// L2, and nothing is left to join.  dx may not be dy then.
+// Otherwise CTA b takes rows b, b + grid, ...; each thread owns the same columns
+// of all of them, so its share of dw stays in registers and is written once, to
+// row b of the partial sums.
+template <bool kBf16, bool kWBf16, int kVec, bool kColumns>
 __global__ void __launch_bounds__(512) rmsnorm_backward_direct_kernel(const RmsNormBwdParams p) {
   __shared__ float red[32];
+  if constexpr (kColumns) {
+    if (blockIdx.x >= p.rows) {
+      column_dw<kBf16>(p, (blockIdx.x - p.rows) * 64);
+      return;
+    }
+  }
   const int nvec = static_cast<int>(p.k / 8);
   const float inv_k = 1.0f / static_cast<float>(p.k);
   Vec8 dw[kVec];
@@ -412,8 +458,9 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_direct_kernel(const RmsN
         store8<kBf16>(p.dx, row * p.lddx + v * 8, d);
       }
     }
+    if constexpr (kColumns) return;
   }
-  if (p.dw_part) {
+  if (!kColumns && p.dw) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
@@ -500,7 +547,7 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNor
     out += step * p.lddx * kElem<kBf16>;
   }
   ring_wait<0>();
-  if (!p.dw_part) return;
+  if (!p.dw) return;
   if (blockDim.y == 1) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
@@ -626,6 +673,24 @@ int backward_direct_grid(int64_t rows) {
   return static_cast<int>(rows < most ? rows : most);
 }
 
+// Few rows whose dy and h stay in L2: dw by columns (see the kernel).
+bool backward_by_columns(int64_t rows, int64_t k) { return rows <= 512 && rows * k <= 4 << 20; }
+
+template <bool kBf16, bool kWBf16, bool kColumns>
+void launch_bwd_direct(const RmsNormBwdParams& p, int grid, cudaStream_t stream) {
+  RowShape s = row_shape(p.k, 512);
+  if (kColumns) s.threads = 512;
+  if (s.vec == 1)
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 1, kColumns><<<grid, s.threads, 0, stream>>>(p);
+  else if (s.vec == 2)
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 2, kColumns><<<grid, s.threads, 0, stream>>>(p);
+  else if (s.vec == 4)
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4, kColumns><<<grid, s.threads, 0, stream>>>(p);
+  else
+    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8, kColumns><<<grid, s.threads, 0, stream>>>(p);
+}
+
+// Returns the rows of partial sums that were written (0: dw is done).
 template <bool kBf16, bool kWBf16>
 int launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
   const RingShape r = ring_shape(p.rows, p.k, p.k * kElem<kBf16> * (p.dres ? 3 : 2));
@@ -634,19 +699,16 @@ int launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
       launch_ring(rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 3>, p, r, stream);
     else
       launch_ring(rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 2>, p, r, stream);
-    return r.grid;
+    return p.dw ? r.grid : 0;
   }
-  const RowShape s = row_shape(p.k, 512);
+  if (backward_by_columns(p.rows, p.k)) {
+    const int64_t columns = p.dw ? (p.k + 63) / 64 : 0;
+    launch_bwd_direct<kBf16, kWBf16, true>(p, static_cast<int>(p.rows + columns), stream);
+    return 0;
+  }
   const int grid = backward_direct_grid(p.rows);
-  if (s.vec == 1)
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 1><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 2)
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 2><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 4)
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4><<<grid, s.threads, 0, stream>>>(p);
-  else
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8><<<grid, s.threads, 0, stream>>>(p);
-  return grid;
+  launch_bwd_direct<kBf16, kWBf16, false>(p, grid, stream);
+  return p.dw ? grid : 0;
 }
 
 }  // namespace
@@ -659,7 +721,7 @@ cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
 }
 
 int rmsnorm_backward_parts(int64_t rows, int64_t k) {
-  int most = backward_direct_grid(rows);
+  int most = backward_by_columns(rows, k) ? 0 : backward_direct_grid(rows);
   for (int64_t inputs = 2; inputs <= 3; ++inputs)
     for (int64_t elem = 2; elem <= 4; elem += 2) {
       const RingShape r = ring_shape(rows, k, k * elem * inputs);
@@ -668,7 +730,7 @@ int rmsnorm_backward_parts(int64_t rows, int64_t k) {
   return most;
 }
 
-cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16, float* dw,
+cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16,
                                     cudaStream_t stream) {
   int parts;
   if (bf16)
@@ -677,8 +739,8 @@ cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w
     parts = w_bf16 ? launch_norm_bwd<false, true>(p, stream)
                    : launch_norm_bwd<false, false>(p, stream);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || !dw) return e;
-  return launch_column_sum(p.dw_part, parts, p.k, dw, stream);
+  if (e != cudaSuccess || !parts) return e;
+  return launch_column_sum(p.dw_part, parts, p.k, p.dw, stream);
 }
 
 cudaError_t launch_column_sum(const float* part, int parts, int64_t k, float* out,

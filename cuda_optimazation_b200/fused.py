@@ -26,6 +26,12 @@ from .qgemm import (
     Mxfp8Result, Nvfp4Result, _check, lib,
 )
 
+try:  # the stream's handle without a Stream object (3.5 us a call)
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
 ACTIVATIONS = {"none": ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU, "gelu": ACT_GELU,
                "swiglu": ACT_SWIGLU}
 GATE_COLUMNS = 128  # columns of a gate block of the gated activation
@@ -53,23 +59,21 @@ def _code(t: torch.Tensor, what: str) -> int:
     return c
 
 
-def _matrix(t: torch.Tensor, what: str, rows: int, cols: int, device, dtype=None) -> None:
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+def _matrix(t: torch.Tensor, what: str, rows: int, cols: int, device, dtype=None) -> int:
+    """Checks a matrix and returns its row stride."""
+    if t.shape != (rows, cols):
         raise ValueError(f"{what} must be {rows} x {cols}, got {tuple(t.shape)}")
-    if t.device != device or (cols > 1 and t.stride(1) != 1):
+    ld, step = t.stride()
+    if t.device != device or (step != 1 and cols > 1):
         raise ValueError(f"{what} must be on {device} with unit column stride")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    return ld if rows > 1 else cols  # the stride of a single row is arbitrary in torch
 
 
 def _vector(t: torch.Tensor, what: str, n: int, device) -> None:
-    if t.dim() != 1 or t.shape[0] != n or t.device != device or (n > 1 and t.stride(0) != 1):
+    if t.shape != (n,) or t.device != device or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{what} must be a contiguous vector of {n} values on {device}")
-
-
-def _ld(t: torch.Tensor) -> int:
-    # The stride of a single row is arbitrary in torch.
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _sf_bytes(rows: int, k: int, layout: int) -> int:
@@ -84,27 +88,29 @@ def _new_mxfp8(rows: int, k: int, layout: int, device) -> Mxfp8Result:
                        rows, k, layout)
 
 
-def _held(a: Operand, what: str) -> None:
-    """A quantised operand's buffers against its shape."""
-    nv, mx4 = isinstance(a, Nvfp4Result), isinstance(a, Mxfp4Result)
-    values = a.rows * a.k // 2 if nv or mx4 else a.rows * a.k
-    sv = 16 if nv else 32
+def _held(a: Operand, what: str) -> torch.device:
+    """Checks a quantised operand's buffers against its shape; their device."""
+    q, sf, rows, k = a.quantized, a.block_scales, a.rows, a.k
+    kind = type(a)
+    sv = 16 if kind is Nvfp4Result else 32
     if a.layout == LAYOUT_REF_LINEAR:
-        scales = a.rows * (a.k // sv)
+        scales = rows * (k // sv)
     else:
-        scales = ((a.rows + 127) // 128) * ((a.k // sv + 3) // 4) * 512
-    if a.quantized.numel() < values or a.block_scales.numel() < scales:
-        raise ValueError(f"{what}: buffers are smaller than the shape {a.rows} x {a.k} needs")
-    if not (a.quantized.is_contiguous() and a.block_scales.is_contiguous()):
+        scales = ((rows + 127) // 128) * ((k // sv + 3) // 4) * 512
+    if q.numel() < (rows * k if kind is Mxfp8Result else rows * k // 2) or sf.numel() < scales:
+        raise ValueError(f"{what}: buffers are smaller than the shape {rows} x {k} needs")
+    if not (q.is_contiguous() and sf.is_contiguous()):
         raise ValueError(f"{what}: buffers must be contiguous")
-    if not a.quantized.is_cuda or a.block_scales.device != a.quantized.device:
+    dev = q.device
+    if dev.type != "cuda" or sf.device != dev:
         raise ValueError(f"{what}: buffers must be on one CUDA device")
+    return dev
 
 
-def _mxfp8(a, what: str) -> None:
+def _mxfp8(a, what: str) -> torch.device:
     if not isinstance(a, Mxfp8Result):
         raise TypeError(f"{what} must be an Mxfp8Result")
-    _held(a, what)
+    return _held(a, what)
 
 
 # ------------------------------------------------------------------ RMS norm
@@ -128,24 +134,25 @@ def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torc
     rows, k = x.shape
     dev = x.device
     code = _code(x, "x")
-    _matrix(x, "x", rows, k, dev)
+    ldx = _matrix(x, "x", rows, k, dev)
     _vector(weight, "weight", k, dev)
+    rp = hp = None
+    ldr = ldh = 0
     if residual is not None:
-        _matrix(residual, "residual", rows, k, dev, x.dtype)
+        ldr, rp = _matrix(residual, "residual", rows, k, dev, x.dtype), residual.data_ptr()
     if h is not None:
-        _matrix(h, "h", rows, k, dev, x.dtype)
+        ldh = _matrix(h, "h", rows, k, dev, x.dtype)
     with _scope(dev, stream):
         y = _new_mxfp8(rows, k, layout, dev)
         rstd = torch.empty(rows, dtype=torch.float32, device=dev)
         if h is None and residual is not None:
-            h = torch.empty(rows, k, dtype=x.dtype, device=dev)
+            h, ldh = torch.empty(rows, k, dtype=x.dtype, device=dev), k
+        if h is not None:
+            hp = h.data_ptr()
         rc = lib().qg_rmsnorm_mxfp8(
-            x.data_ptr(), code, _ld(x), residual.data_ptr() if residual is not None else None,
-            _ld(residual) if residual is not None else 0, weight.data_ptr(),
-            _code(weight, "weight"), eps, rows, k, layout, y.quantized.data_ptr(),
-            y.block_scales.data_ptr(), h.data_ptr() if h is not None else None,
-            _ld(h) if h is not None else 0, rstd.data_ptr(),
-            torch.cuda.current_stream().cuda_stream)
+            x.data_ptr(), code, ldx, rp, ldr, weight.data_ptr(), _code(weight, "weight"), eps,
+            rows, k, layout, y.quantized.data_ptr(), y.block_scales.data_ptr(), hp, ldh,
+            rstd.data_ptr(), _raw_stream(dev.index))
     _check(rc, "qg_rmsnorm_mxfp8")
     return RmsNormResult(y, x if h is None else h, rstd)
 
@@ -163,29 +170,30 @@ def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weig
     rows, k = h.shape
     dev = h.device
     code = _code(h, "h")
-    _matrix(h, "h", rows, k, dev)
-    _matrix(dy, "dy", rows, k, dev, h.dtype)
+    ldh = _matrix(h, "h", rows, k, dev)
+    lddy = _matrix(dy, "dy", rows, k, dev, h.dtype)
     _vector(rstd, "rstd", rows, dev)
     _vector(weight, "weight", k, dev)
     if rstd.dtype != torch.float32:
         raise TypeError("rstd must be float32")
+    rp, ldr = None, 0
     if dres is not None:
-        _matrix(dres, "dres", rows, k, dev, h.dtype)
+        ldr, rp = _matrix(dres, "dres", rows, k, dev, h.dtype), dres.data_ptr()
     with _scope(dev, stream):
         dx = torch.empty(rows, k, dtype=h.dtype, device=dev)
-        dw = ws = None
+        dw = dwp = wsp = None
         need = 0
         if want_dweight:
             dw = torch.empty(k, dtype=torch.float32, device=dev)
+            dwp = dw.data_ptr()
             need = lib().qg_rmsnorm_backward_workspace_bytes(rows, k)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            if need:
+                ws = torch.empty(need, dtype=torch.uint8, device=dev)
+                wsp = ws.data_ptr()
         rc = lib().qg_rmsnorm_backward(
-            dy.data_ptr(), _ld(dy), h.data_ptr(), _ld(h), code, rstd.data_ptr(),
-            weight.data_ptr(), _code(weight, "weight"),
-            dres.data_ptr() if dres is not None else None, _ld(dres) if dres is not None else 0,
-            rows, k, dx.data_ptr(), k, dw.data_ptr() if dw is not None else None,
-            ws.data_ptr() if ws is not None else None, need,
-            torch.cuda.current_stream().cuda_stream)
+            dy.data_ptr(), lddy, h.data_ptr(), ldh, code, rstd.data_ptr(), weight.data_ptr(),
+            _code(weight, "weight"), rp, ldr, rows, k, dx.data_ptr(), k, dwp, wsp, need,
+            _raw_stream(dev.index))
     _check(rc, "qg_rmsnorm_backward")
     return dx, dw
 
@@ -223,52 +231,50 @@ def gemm_fused(a: Operand, b: Operand, bias: Optional[torch.Tensor] = None, act:
         raise ValueError("operands must share the format")
     if a.k != b.k or a.layout != b.layout:
         raise ValueError("operands must share K and layout")
-    if act not in ACTIVATIONS:
+    code = ACTIVATIONS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(ACTIVATIONS)}")
-    _held(a, "a")
-    _held(b, "b")
-    m, n, k = a.rows, b.rows, a.k
-    dev = a.quantized.device
-    if b.quantized.device != dev:
+    dev = _held(a, "a")
+    if _held(b, "b") != dev:
         raise ValueError("operands must be on one device")
-    cols = n // 2 if act == "swiglu" else n
-    e = Epilogue()
-    e.act = ACTIVATIONS[act]
+    m, n = a.rows, b.rows
+    cols = n // 2 if code == ACT_SWIGLU else n
+    bp = rp = ats = bts = zq = zsf = out_sf = None
+    bias_code = res_code = ldr = ldc = 0
     if bias is not None:
         _vector(bias, "bias", n, dev)
-        e.bias, e.bias_dtype = bias.data_ptr(), _code(bias, "bias")
+        bp, bias_code = bias.data_ptr(), _code(bias, "bias")
     if residual is not None:
-        _matrix(residual, "residual", m, cols, dev)
-        e.residual, e.residual_dtype = residual.data_ptr(), _code(residual, "residual")
-        e.ldr = _ld(residual)
+        ldr = _matrix(residual, "residual", m, cols, dev)
+        rp, res_code = residual.data_ptr(), _code(residual, "residual")
+    kind = type(a)
+    fmt = FORMAT_MXFP8
+    if kind is Nvfp4Result:
+        fmt, ats, bts = FORMAT_NVFP4, a.tensor_scale.data_ptr(), b.tensor_scale.data_ptr()
+    elif kind is Mxfp4Result:
+        fmt = FORMAT_MXFP4
     with _scope(dev, stream):
         if isinstance(out, torch.Tensor):
-            _matrix(out, "out", m, cols, dev)
-            to, e.out, e.out_dtype, e.ldc = out, out.data_ptr(), _code(out, "out"), _ld(out)
+            to, ldc = out, _matrix(out, "out", m, cols, dev)
+            op, out_code = out.data_ptr(), _code(out, "out")
         elif out == "mxfp8":
-            to = _new_mxfp8(m, cols, layout, dev)
-            e.out, e.out_sf = to.quantized.data_ptr(), to.block_scales.data_ptr()
-            e.out_dtype, e.out_layout = DTYPE_MXFP8, layout
+            to, out_code = _new_mxfp8(m, cols, layout, dev), DTYPE_MXFP8
+            op, out_sf = to.quantized.data_ptr(), to.block_scales.data_ptr()
         elif out in _TORCH:
-            to = torch.empty(m, cols, dtype=_TORCH[out], device=dev)
-            e.out, e.out_dtype, e.ldc = to.data_ptr(), _OUTPUTS[out], cols
+            to, out_code = torch.empty(m, cols, dtype=_TORCH[out], device=dev), _OUTPUTS[out]
+            op, ldc = to.data_ptr(), cols
         else:
             raise ValueError(f"out must be a tensor or one of {sorted(_OUTPUTS)}")
         z = None
         if checkpoint:
             z = _new_mxfp8(m, n, checkpoint_layout, dev)
-            e.ckpt_q, e.ckpt_sf = z.quantized.data_ptr(), z.block_scales.data_ptr()
-            e.ckpt_layout = checkpoint_layout
-        fmt, ats, bts = FORMAT_MXFP8, None, None
-        if isinstance(a, Nvfp4Result):
-            fmt, ats, bts = FORMAT_NVFP4, a.tensor_scale.data_ptr(), b.tensor_scale.data_ptr()
-        elif isinstance(a, Mxfp4Result):
-            fmt = FORMAT_MXFP4
+            zq, zsf = z.quantized.data_ptr(), z.block_scales.data_ptr()
+        e = Epilogue(code, bias_code, bp, rp, ldr, res_code, out_code, op, ldc, out_sf, zq, zsf,
+                     layout, checkpoint_layout)
         rc = lib().qg_gemm_fused(
             fmt, a.quantized.data_ptr(), a.block_scales.data_ptr(), ats, b.quantized.data_ptr(),
-            b.block_scales.data_ptr(), bts, m, n, k, a.layout, ctypes.addressof(e),
-            status.data_ptr() if status is not None else None,
-            torch.cuda.current_stream().cuda_stream)
+            b.block_scales.data_ptr(), bts, m, n, a.k, a.layout, ctypes.addressof(e),
+            status.data_ptr() if status is not None else None, _raw_stream(dev.index))
     _check(rc, "qg_gemm_fused")
     return GemmFusedResult(to, z)
 
@@ -288,39 +294,39 @@ def act_backward(dout: torch.Tensor, checkpoint: Optional[Mxfp8Result], act: str
     quantised for both gradient products, and its column sums
     (qg_act_backward_mxfp8).  dout: fp32/bf16 [m, n] ([m, n / 2] for "swiglu").
     checkpoint may be None for act="none"."""
-    if act not in ACTIVATIONS:
+    code = ACTIVATIONS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(ACTIVATIONS)}")
     if dout.dim() != 2 or not dout.is_cuda:
         raise ValueError("dout must be a 2-D CUDA tensor")
     dev = dout.device
     m, cols = dout.shape
-    n = 2 * cols if act == "swiglu" else cols
-    if act != "none" and checkpoint is None:
-        raise ValueError(f"act={act!r} needs the checkpoint")
+    n = 2 * cols if code == ACT_SWIGLU else cols
+    zq = zsf = None
+    z_layout = LAYOUT_MMA
     if checkpoint is not None:
-        _mxfp8(checkpoint, "checkpoint")
-        if (checkpoint.rows, checkpoint.k) != (m, n) or checkpoint.quantized.device != dev:
+        if _mxfp8(checkpoint, "checkpoint") != dev or (checkpoint.rows, checkpoint.k) != (m, n):
             raise ValueError(f"checkpoint must be {m} x {n} on {dev}")
-    _matrix(dout, "dout", m, cols, dev)
+        zq, zsf = checkpoint.quantized.data_ptr(), checkpoint.block_scales.data_ptr()
+        z_layout = checkpoint.layout
+    elif code != ACT_NONE:
+        raise ValueError(f"act={act!r} needs the checkpoint")
+    ldd = _matrix(dout, "dout", m, cols, dev)
     with _scope(dev, stream):
-        mt = (m + 31) // 32 * 32
-        dz, dz_t = _new_mxfp8(m, n, layout, dev), _new_mxfp8(n, mt, layout, dev)
-        db = ws = None
+        dz, dz_t = _new_mxfp8(m, n, layout, dev), _new_mxfp8(n, (m + 31) // 32 * 32, layout, dev)
+        db = dbp = wsp = None
         need = 0
         if want_dbias:
             db = torch.empty(n, dtype=torch.float32, device=dev)
+            dbp = db.data_ptr()
             need = lib().qg_act_backward_workspace_bytes(m, n)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        z = checkpoint
+            if need:
+                ws = torch.empty(need, dtype=torch.uint8, device=dev)
+                wsp = ws.data_ptr()
         rc = lib().qg_act_backward_mxfp8(
-            dout.data_ptr(), _code(dout, "dout"), _ld(dout),
-            z.quantized.data_ptr() if z is not None else None,
-            z.block_scales.data_ptr() if z is not None else None,
-            z.layout if z is not None else LAYOUT_MMA, ACTIVATIONS[act], m, n,
+            dout.data_ptr(), _code(dout, "dout"), ldd, zq, zsf, z_layout, code, m, n,
             dz.quantized.data_ptr(), dz.block_scales.data_ptr(), dz_t.quantized.data_ptr(),
-            dz_t.block_scales.data_ptr(), layout, db.data_ptr() if db is not None else None,
-            ws.data_ptr() if ws is not None else None, need,
-            torch.cuda.current_stream().cuda_stream)
+            dz_t.block_scales.data_ptr(), layout, dbp, wsp, need, _raw_stream(dev.index))
     _check(rc, "qg_act_backward_mxfp8")
     return ActBackwardResult(dz, dz_t, db)
 
@@ -330,13 +336,12 @@ def transpose_mxfp8(a: Mxfp8Result, layout: int = LAYOUT_MMA,
     """A's transpose (k x rows rounded up to 32, zeros beyond) requantised with
     scales along A's rows (qg_transpose_mxfp8): the kept 8-bit input of a product
     as the operand of its weight gradient."""
-    _mxfp8(a, "a")
-    dev = a.quantized.device
+    dev = _mxfp8(a, "a")
     with _scope(dev, stream):
         t = _new_mxfp8(a.k, (a.rows + 31) // 32 * 32, layout, dev)
         rc = lib().qg_transpose_mxfp8(
             a.quantized.data_ptr(), a.block_scales.data_ptr(), a.layout, a.rows, a.k,
             t.quantized.data_ptr(), t.block_scales.data_ptr(), layout,
-            torch.cuda.current_stream().cuda_stream)
+            _raw_stream(dev.index))
     _check(rc, "qg_transpose_mxfp8")
     return t

@@ -296,14 +296,15 @@ int qg_rmsnorm_mxfp8(const void* x, int x_dtype, int64_t ldx, const void* residu
  *   dx = rstd * (g - xh * mean(g * xh)) + dres,   dweight = sum_rows dy * xh.
  * dy, h, dres (NULL: none) and dx have x_dtype; dx is the gradient of x and of
  * the residual alike.  dweight (k floats) may be NULL, and workspace with it.
- * dx may be dy or dres itself.  Deterministic: sums run in a fixed order. */
+ * dx may be dres itself, but not dy or h.  Deterministic: sums run in a fixed
+ * order. */
 int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, int x_dtype,
                         const float* rstd, const void* weight, int w_dtype, const void* dres,
                         int64_t lddres, int64_t rows, int64_t k, void* dx, int64_t lddx,
                         float* dweight, void* workspace, size_t workspace_bytes,
                         qg_stream_t stream);
 
-/* Workspace bytes qg_rmsnorm_backward needs for dweight. */
+/* Workspace bytes qg_rmsnorm_backward needs for dweight (0: none, NULL will do). */
 size_t qg_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t k);
 
 /* Activations: gelu is the tanh form, relu's slope at 0 is 0.  QG_ACT_SWIGLU gates: of every 256
@@ -359,15 +360,15 @@ int qg_gemm_fused(int format, const void* a_q, const void* a_sf, const float* a_
  *     gradient dz^T . x;
  *   - dbias (n floats, NULL: none): the column sums of dz.
  * Scales in out_layout, an MMA layout.  With QG_ACT_NONE z_q and z_sf may be
- * NULL.  n % 32 == 0.  workspace: qg_act_backward_workspace_bytes bytes (0, and
- * NULL, without dbias).  Deterministic. */
+ * NULL.  n % 32 == 0.  workspace: qg_act_backward_workspace_bytes bytes (NULL
+ * without dbias).  Deterministic. */
 int qg_act_backward_mxfp8(const void* dout, int dout_dtype, int64_t ldd, const void* z_q,
                           const void* z_sf, int z_layout, int act, int64_t m, int64_t n,
                           void* dz_q, void* dz_sf, void* dzt_q, void* dzt_sf, int out_layout,
                           float* dbias, void* workspace, size_t workspace_bytes,
                           qg_stream_t stream);
 
-/* Workspace bytes qg_act_backward_mxfp8 needs for dbias. */
+/* Workspace bytes qg_act_backward_mxfp8 needs for dbias (0: none, NULL will do). */
 size_t qg_act_backward_workspace_bytes(int64_t m, int64_t n);
 
 /* An MXFP8 matrix (rows x k, k % 32 == 0, any layout) turned: k x rt with rt =

@@ -33,7 +33,7 @@ def test_rmsnorm_refusals(qlib):
 
 
 def norm_bwd(L, dy=A, lddy=256, h=A, ldh=256, dt=0, rstd=A, w=A, wdt=0, dres=None, lddres=0,
-             rows=4, k=256, dx=A, lddx=256, dw=A, ws=A, wsb=BIG):
+             rows=600, k=256, dx=2 * A, lddx=256, dw=A, ws=A, wsb=BIG):
     return L.qg_rmsnorm_backward(dy, lddy, h, ldh, dt, rstd, w, wdt, dres, lddres, rows, k, dx,
                                  lddx, dw, ws, wsb, None)
 
@@ -42,14 +42,17 @@ def test_rmsnorm_backward_refusals(qlib):
     L = qlib.lib()
     for bad in ("dy", "h", "rstd", "w", "dx", "ws"):
         assert norm_bwd(L, **{bad: None}) == qlib.ERR_ARG, bad
-    need = L.qg_rmsnorm_backward_workspace_bytes(4, 256)
-    assert need == 4 * 256 * 4 and L.qg_rmsnorm_backward_workspace_bytes(0, 256) == 0
+    assert norm_bwd(L, dx=A) == qlib.ERR_ARG  # dy's own buffer
+    need = L.qg_rmsnorm_backward_workspace_bytes(600, 256)
+    assert need > 0 and need % (256 * 4) == 0
+    assert L.qg_rmsnorm_backward_workspace_bytes(0, 256) == 0
+    assert L.qg_rmsnorm_backward_workspace_bytes(4, 256) == 0  # few rows join by themselves
     assert norm_bwd(L, wsb=need - 1) == qlib.ERR_ARG
     assert norm_bwd(L, dt=3) == qlib.ERR_DTYPE
     for bad in (dict(rows=0), dict(k=40), dict(lddy=8), dict(ldh=8), dict(lddx=8),
                 dict(dres=A, lddres=8)):
         assert norm_bwd(L, **bad) == qlib.ERR_SHAPE, bad
-    for bad in (dict(dy=MIS), dict(h=MIS), dict(dx=MIS), dict(w=MIS), dict(ws=MIS), dict(lddx=257),
+    for bad in (dict(dy=MIS), dict(h=MIS), dict(dx=A + 8 * 1001), dict(w=MIS), dict(ws=MIS), dict(lddx=257),
                 dict(dres=MIS, lddres=256), dict(dw=A + 1)):
         assert norm_bwd(L, **bad) == qlib.ERR_ALIGN, bad
 
@@ -88,7 +91,7 @@ def test_gemm_refusals(qlib):
         assert gemm(qlib, **bad) == qlib.ERR_ALIGN, bad
 
 
-def act_bwd(L, d=A, dt=1, ldd=256, zq=A, zsf=A, zl=1, act=2, m=64, n=256, dz=A, dzs=A, t=A, ts=A,
+def act_bwd(L, d=A, dt=1, ldd=256, zq=A, zsf=A, zl=1, act=2, m=2000, n=256, dz=A, dzs=A, t=A, ts=A,
             lay=1, db=A, ws=A, wsb=BIG):
     return L.qg_act_backward_mxfp8(d, dt, ldd, zq, zsf, zl, act, m, n, dz, dzs, t, ts, lay, db, ws,
                                    wsb, None)
@@ -99,7 +102,8 @@ def test_act_backward_refusals(qlib):
     for bad in ("d", "zq", "zsf", "dz", "dzs", "t", "ts", "ws"):
         assert act_bwd(L, **{bad: None}) == qlib.ERR_ARG, bad
     assert act_bwd(L, act=5) == qlib.ERR_ARG
-    assert act_bwd(L, wsb=L.qg_act_backward_workspace_bytes(64, 256) - 1) == qlib.ERR_ARG
+    assert act_bwd(L, wsb=L.qg_act_backward_workspace_bytes(2000, 256) - 1) == qlib.ERR_ARG
+    assert L.qg_act_backward_workspace_bytes(64, 256) == 0  # one row tile
     assert act_bwd(L, dt=2) == qlib.ERR_DTYPE
     for bad in (dict(zl=3), dict(lay=0), dict(lay=3)):
         assert act_bwd(L, **bad) == qlib.ERR_LAYOUT, bad

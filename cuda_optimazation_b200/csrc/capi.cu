@@ -291,7 +291,15 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
     p.rq_row_blocks = static_cast<int>((m + 127) / 128);
     p.rq_sf_blocks = static_cast<int>((n / 16 + 3) / 4);
   }
-  if (epi) p.epi = *epi;
+  if (epi) {
+    p.epi = *epi;
+    if (epi->out_kind == kEpiBf16 && epi->out_vec) {
+      if (!make_output_map(&p.tm_out[0], epi->out, m, epi->act == QG_ACT_SWIGLU ? n / 2 : n,
+                           epi->ldc))
+        return QG_ERR_CUDA;
+      p.n_out = 1;
+    }
+  }
   p.a_ts = fmt == 1 ? a_ts : nullptr;
   p.b_ts = fmt == 1 ? b_ts : nullptr;
   p.status = status;

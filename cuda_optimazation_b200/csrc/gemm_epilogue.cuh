@@ -22,7 +22,12 @@ __device__ __forceinline__ void epi_affine(const EpiParams& e, const uint32_t (&
                                            float alpha, int col0, int n, int lane,
                                            float (&z)[32]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(acc[j]) * alpha;
+  for (int j = 0; j < 32; j += 2) {
+    const float2 t = mul2(make_float2(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1])),
+                          both(alpha));
+    z[j] = t.x;
+    z[j + 1] = t.y;
+  }
   if (e.bias) {
     float b = 0.0f;
     if (col0 + lane < n)
@@ -56,7 +61,7 @@ __device__ __forceinline__ void epi_store_mx(const float (&v)[32], uint8_t* q, u
   if (in) {
     float amax = 0.0f, mul;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) amax = fmaxf(amax, fabsf(v[j]));
+    for (int j = 0; j < 32; j += 2) amax = max3_abs(amax, v[j], v[j + 1]);
     code = mxfp8_scale_code(amax, mul);
     uint4* dst = reinterpret_cast<uint4*>(q + static_cast<int64_t>(row) * n + col0);
 #pragma unroll
@@ -65,7 +70,9 @@ __device__ __forceinline__ void epi_store_mx(const float (&v)[32], uint8_t* q, u
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = 16 * h + 4 * i;
-        w[i] = cvt_e4m3x4(v[j] * mul, v[j + 1] * mul, v[j + 2] * mul, v[j + 3] * mul);
+        const float2 a = mul2(make_float2(v[j], v[j + 1]), both(mul));
+        const float2 b = mul2(make_float2(v[j + 2], v[j + 3]), both(mul));
+        w[i] = cvt_e4m3x4(a.x, a.y, b.x, b.y);
       }
       dst[h] = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -78,12 +85,11 @@ __device__ __forceinline__ void epi_store_mx(const float (&v)[32], uint8_t* q, u
   }
 }
 
-// y += residual, then the output (n: its columns).
-__device__ __forceinline__ void epi_finish(const EpiParams& e, float (&y)[32], int row, int col0,
-                                           int m, int n) {
-  const bool in = row < m && col0 < n;
+// y += residual (n: the output's columns).
+__device__ __forceinline__ void epi_residual(const EpiParams& e, float (&y)[32], int row, int col0,
+                                             int m, int n) {
   const bool full = col0 + 32 <= n;
-  if (in && e.res) {
+  if (e.res && row < m && col0 < n) {
     const int64_t at = row * e.ldr + col0;
     if (e.res_bf16) {
       const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(e.res) + at;
@@ -121,6 +127,22 @@ __device__ __forceinline__ void epi_finish(const EpiParams& e, float (&y)[32], i
       }
     }
   }
+}
+
+// 32 values as 16 words of bf16.
+__device__ __forceinline__ void epi_pack(const float (&y)[32], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+}
+
+// The output, straight to global memory.
+__device__ __forceinline__ void epi_store(const EpiParams& e, const float (&y)[32], int row,
+                                          int col0, int m, int n) {
+  const bool in = row < m && col0 < n;
+  const bool full = col0 + 32 <= n;
   if (e.out_kind == kEpiMxfp8) {
     epi_store_mx(y, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout, e.row_blocks,
                  e.out_sf_blocks, row, col0, m, n);
@@ -129,16 +151,12 @@ __device__ __forceinline__ void epi_finish(const EpiParams& e, float (&y)[32], i
     if (e.out_kind == kEpiBf16) {
       __nv_bfloat16* c = static_cast<__nv_bfloat16*>(e.out) + at;
       if (full && e.out_vec) {
+        uint32_t w[16];
+        epi_pack(y, w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(y[8 * i + 2 * j], y[8 * i + 2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&b);
-          }
-          reinterpret_cast<uint4*>(c)[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int i = 0; i < 4; ++i)
+          reinterpret_cast<uint4*>(c)[i] =
+              make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j)

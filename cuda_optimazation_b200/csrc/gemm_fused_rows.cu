@@ -32,6 +32,8 @@ namespace qg {
 
 namespace {
 
+constexpr int kTogether = 4;  // rows that a thread finishes at a time
+constexpr int kMaxRanks = 8;  // CTAs per cluster (the portable size)
 constexpr int kRowsFmtMxfp8 = 0, kRowsFmtNvfp4 = 1, kRowsFmtMxfp4 = 2;
 
 constexpr int pow2_at_least(int v) {
@@ -127,6 +129,19 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.num_k_blocks) * rank / ranks);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.num_k_blocks) * (rank + 1) / ranks);
 
+  const int col0 = tile * Cfg::kSets * 128;  // first column of z
+  // One stage's loads (the producer thread).
+  auto load_stage = [&](int stage, int kb, uint64_t pol_w, uint64_t pol_x) {
+    uint8_t* sw = smem + stage * Cfg::kStageBytes;
+    uint8_t* sx = sw + Cfg::kWBytes;
+    uint8_t* ssw = sx + Cfg::kXBytes;
+    uint8_t* ssx = ssw + Cfg::kSfwBytes;
+    mbar_arrive_expect_tx(&full_bar[stage], Cfg::kTx);
+    tma_load_2d(sw, &p.tm_a, &full_bar[stage], kb * 128, col0, pol_w);
+    tma_load_3d(ssw, &p.tm_sfa, &full_bar[stage], 0, col0 / 128, kb * Cfg::kChunks, pol_w);
+    tma_load_2d(sx, &p.tm_b, &full_bar[stage], kb * 128, 0, pol_x);
+    tma_load_3d(ssx, &p.tm_sfb, &full_bar[stage], 0, 0, kb * Cfg::kChunks, pol_x);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -135,6 +150,10 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
     mbar_init(acc_full, 1);
     *abort_flag = 0u;
     fence_barrier_init();
+    // The first stages need no one's leave: on their way before the TMEM
+    // allocation and the CTA's barrier.
+    const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+    for (int s = 0; s < Cfg::kStages && kb0 + s < kb1; ++s) load_stage(s, kb0 + s, pol_w, pol_x);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
@@ -144,31 +163,23 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int col0 = tile * Cfg::kSets * 128;  // first column of z
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
     if (lane == 0) {
       const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      uint32_t issued_mask = 0, issued_parity = 0, phase = 0;
+      // Stages loaded above: round 0, parity 0.
+      const int early = kb1 - kb0 < Cfg::kStages ? kb1 - kb0 : Cfg::kStages;
+      uint32_t issued_mask = (1u << early) - 1u, issued_parity = 0, phase = 1;
       int stage = 0;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0 + Cfg::kStages; kb < kb1; ++kb) {
         if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, p.timeout_ns, abort_flag, p.status,
                                kDevTimeoutProducer)) {
           ok = false;
           break;
         }
-        uint8_t* sw = smem + stage * Cfg::kStageBytes;
-        uint8_t* sx = sw + Cfg::kWBytes;
-        uint8_t* ssw = sx + Cfg::kXBytes;
-        uint8_t* ssx = ssw + Cfg::kSfwBytes;
-        mbar_arrive_expect_tx(&full_bar[stage], Cfg::kTx);
-        tma_load_2d(sw, &p.tm_a, &full_bar[stage], kb * 128, col0, pol_w);
-        tma_load_3d(ssw, &p.tm_sfa, &full_bar[stage], 0, col0 / 128, kb * Cfg::kChunks, pol_w);
-        tma_load_2d(sx, &p.tm_b, &full_bar[stage], kb * 128, 0, pol_x);
-        tma_load_3d(ssx, &p.tm_sfb, &full_bar[stage], 0, 0, kb * Cfg::kChunks, pol_x);
-        issued_mask |= 1u << stage;
+        load_stage(stage, kb, pol_w, pol_x);
         issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
         if (++stage == Cfg::kStages) {
           stage = 0;
@@ -306,43 +317,65 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
     }
     __syncwarp();
     cluster_sync();  // every CTA's partial sums are in place
-    for (int i = rank * 2 + (threadIdx.x >> 7); i < Cfg::kPass && t0 + i < p.m; i += 2 * ranks) {
-      const int row = t0 + i;
-      float z[Cfg::kSets];
+    // A CTA half finishes every (2 ranks)-th row of the pass, kTogether rows at
+    // a time: all their remote loads and residuals are in flight at once.
+    for (int i0 = rank * 2 + (threadIdx.x >> 7); i0 < Cfg::kPass && t0 + i0 < p.m;
+         i0 += 2 * ranks * kTogether) {
+      float z[kTogether][Cfg::kSets], res[kTogether];
 #pragma unroll
-      for (int s = 0; s < Cfg::kSets; ++s) {
-        z[s] = 0.0f;
-        for (int r = 0; r < ranks; ++r)
-          z[s] += ld_cluster_f32(
-              mapa_shared(part_addr + ((s * Cfg::kPass + i) * 128 + f) * 4, static_cast<uint32_t>(r)));
-        z[s] = z[s] * alpha + bias[s];
-        if (e.z_q)
-          lane_store_mx(z[s], in_z, e.z_q, e.z_sf, e.z_layout, e.z_sf_blocks, row,
-                        col0 + s * 128 + f, p.n, lane);
+      for (int u = 0; u < kTogether; ++u) {
+        const int i = i0 + u * 2 * ranks;
+        const bool on = i < Cfg::kPass && t0 + i < p.m;
+        res[u] = 0.0f;
+        if (on && e.res && in_z) {
+          const int64_t at = (t0 + i) * e.ldr + out_col;
+          res[u] = e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at])
+                              : static_cast<const float*>(e.res)[at];
+        }
+#pragma unroll
+        for (int s = 0; s < Cfg::kSets; ++s) {
+          float v[kMaxRanks];
+          const uint32_t at = part_addr + ((s * Cfg::kPass + (on ? i : 0)) * 128 + f) * 4;
+#pragma unroll
+          for (int r = 0; r < kMaxRanks; ++r)
+            v[r] = r < ranks ? ld_cluster_f32(mapa_shared(at, static_cast<uint32_t>(r))) : 0.0f;
+          z[u][s] = v[0];
+#pragma unroll
+          for (int r = 1; r < kMaxRanks; ++r) z[u][s] += v[r];
+        }
       }
-      float y;
-      if constexpr (kGated) {
-        y = act_fwd<kActSilu>(z[0]) * z[1];
-      } else {
-        y = z[0];
-        if (e.act == kActRelu) y = act_fwd<kActRelu>(y);
-        else if (e.act == kActSilu) y = act_fwd<kActSilu>(y);
-        else if (e.act == kActGelu) y = act_fwd<kActGelu>(y);
-      }
-      if (e.res && in_z) {
-        const int64_t at = row * e.ldr + out_col;
-        y += e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at])
-                        : static_cast<const float*>(e.res)[at];
-      }
-      if (e.out_kind == kEpiMxfp8) {
-        lane_store_mx(y, in_z, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout,
-                      e.out_sf_blocks, row, out_col, n_out, lane);
-      } else if (in_z) {
-        const int64_t at = row * e.ldc + out_col;
-        if (e.out_kind == kEpiBf16)
-          static_cast<__nv_bfloat16*>(e.out)[at] = __float2bfloat16_rn(y);
-        else
-          static_cast<float*>(e.out)[at] = y;
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const int i = i0 + u * 2 * ranks;
+        if (i >= Cfg::kPass || t0 + i >= p.m) break;
+        const int row = t0 + i;
+#pragma unroll
+        for (int s = 0; s < Cfg::kSets; ++s) {
+          z[u][s] = z[u][s] * alpha + bias[s];
+          if (e.z_q)
+            lane_store_mx(z[u][s], in_z, e.z_q, e.z_sf, e.z_layout, e.z_sf_blocks, row,
+                          col0 + s * 128 + f, p.n, lane);
+        }
+        float y;
+        if constexpr (kGated) {
+          y = act_fwd<kActSilu>(z[u][0]) * z[u][1];
+        } else {
+          y = z[u][0];
+          if (e.act == kActRelu) y = act_fwd<kActRelu>(y);
+          else if (e.act == kActSilu) y = act_fwd<kActSilu>(y);
+          else if (e.act == kActGelu) y = act_fwd<kActGelu>(y);
+        }
+        if (e.res) y += res[u];
+        if (e.out_kind == kEpiMxfp8) {
+          lane_store_mx(y, in_z, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout,
+                        e.out_sf_blocks, row, out_col, n_out, lane);
+        } else if (in_z) {
+          const int64_t at = row * e.ldc + out_col;
+          if (e.out_kind == kEpiBf16)
+            static_cast<__nv_bfloat16*>(e.out)[at] = __float2bfloat16_rn(y);
+          else
+            static_cast<float*>(e.out)[at] = y;
+        }
       }
     }
     cluster_sync();  // the sums have been read: reuse the buffer, or exit
@@ -368,7 +401,7 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
 // SMs at once, with at least two K blocks each.
 int cluster_size(int tiles, int k_blocks, int slots) {
   int c = 1;
-  while (c < 8 && tiles * 2 * c <= slots && k_blocks >= 4 * c) c *= 2;
+  while (c < kMaxRanks && tiles * 2 * c <= slots && k_blocks >= 4 * c) c *= 2;
   return c;
 }
 

@@ -227,8 +227,30 @@ __device__ __forceinline__ void tile_coords(int tile, int num_m_tiles, int num_n
 // warps (11..14, one per TMEM lane quadrant).
 template <int kOut>
 constexpr int pair_threads() {
-  return kOut >= 2 ? 480 : 352;
+  return kOut >= 4 ? 512 : (kOut >= 2 ? 480 : 352);
 }
+
+// Warp roles.  The fused epilogues (kOut >= 4) hold a tile's 128 accumulator
+// columns of a row in registers, so that the accumulator goes back to the MMA
+// issuer before any of the epilogue's arithmetic: their warps are ordered by
+// warpgroup (producer and issuer; stagers; two of epilogue warps) and hand
+// registers over.  512 threads start with 128 registers each:
+// 64 + 64 + 192 + 192 = 4 x 128.
+template <int kOut>
+struct PairRoles {
+  static constexpr bool kWide = kOut >= 4;
+  // The warps (a whole warpgroup, where registers change hands) of the producer
+  // and the issuers.
+  __device__ static bool feeder(int warp) { return kWide ? warp < 4 : warp == 0 || mma(warp); }
+  __device__ static bool mma(int warp) { return warp == 1 || (!kWide && warp == 10); }
+  __device__ static bool stager(int warp) {
+    return kWide ? warp >= 4 && warp < 8 : warp >= 6 && warp <= 9;
+  }
+  __device__ static bool epilogue(int warp) {
+    return kWide ? warp >= 8 : (warp >= 2 && warp <= 5) || warp >= 11;
+  }
+  static constexpr int kRegsAtLaunch = 128, kRegsFew = 64, kRegsEpilogue = 192;
+};
 
 // ------------------------------------------------------------------ tile scheduler
 // The grid holds one CTA pair per output tile; the pairs that fit run
@@ -386,10 +408,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
   // the first is the cluster's own index, later ones come from the
   // leader's producer through cluster launch control (see TileRing).
   TileRing ring{tile_ids, tile_full, tile_empty, leader};
-
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA
-    if (lane == 0) {
+  using Roles = PairRoles<kOut>;
+  if (Roles::feeder(warp)) {
+    if constexpr (Roles::kWide) reg_dealloc<Roles::kRegsFew>();
+    if (warp == 0 && lane == 0) {
+      // -------------------------------------------------------------- TMA
       const uint64_t pol = l2_policy_evict_last();
       // B tiles (and their scales): within a group of kGroupM m-tiles the
       // pairs working at one time share a B tile once, A slices are reused
@@ -512,7 +535,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         if (!leader) spin_ns(200000);
       }
     }
-  } else if (warp == 1 || warp == 10) {
     // ---------------------------------------------------------------- MMA
     // Issuer h (warp 1: h = 0, warp 10: h = 1) accumulates output columns of
     // its N half into TMEM columns [h * kIssueN, (h + 1) * kIssueN).  The
@@ -520,7 +542,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
     // stage, phase, descriptors and scale columns are stepped by constants
     // and the diagnostic switches are read once.
     const int h = warp == 1 ? 0 : 1;
-    if (leader && lane == 0 && h < Cfg::kIssuers) {
+    if (Roles::mma(warp) && leader && lane == 0 && h < Cfg::kIssuers) {
       const uint32_t idesc_base =
           kFp4 ? make_idesc_block_scaled(2 * Cfg::kBM, Cfg::kIssueN, 1u,
                                          kFmt == kFmtMxfp4 ? 1u : 0u, 0u, 0u)
@@ -610,8 +632,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
       uint32_t dummy = 0;
       mbar_wait_bounded(&drain_bar[h], 0, p.timeout_ns, &dummy, nullptr, 0);
     }
-  } else if (warp >= 6 && warp <= 9) {
+  } else if (Roles::stager(warp)) {
     // ---------------------------------------------------------------- scale stagers
+    if constexpr (Roles::kWide) reg_dealloc<Roles::kRegsFew>();
     const int quad = warp % 4;
     const uint32_t t_quad = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const bool no_wait = (kDiag & 32u) != 0, skip_st = (kDiag & 1u) != 0;
@@ -660,8 +683,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         trace_pair(p, pair == 0 && lane == 0, 11 + (warp - 6) + (leader ? 0 : 4), g);
       }
     }
-  } else {
+  } else if (Roles::epilogue(warp)) {
     // ---------------------------------------------------------------- epilogue
+    if constexpr (Roles::kWide) reg_alloc<Roles::kRegsEpilogue>();
     const int quad = warp % 4;
     // acc_empty[h] (leader) is released as soon as this warp has read issuer
     // h's TMEM columns, so issuer 0 starts the next tile while the second
@@ -775,49 +799,75 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
           }
         }
       } else if constexpr (kOut >= 4) {
-        // Fused epilogue: 32 columns of a row at a time.  The two warps of a
-        // TMEM lane quadrant take the 64-column blocks {sub, 2 + sub}, which
-        // for the gated form are a gate block and its factors.
+        // Fused epilogue.  The two warps of a TMEM lane quadrant take the
+        // 64-column blocks {sub, 2 + sub} (a gate block and its factors, for
+        // the gated form), read them whole, hand the accumulator back and
+        // work from registers while the next tile's MMAs run, 32 columns
+        // (one MX block) at a time.  bf16 rows that TMA can store leave
+        // through the warp's swizzled box, as in kind 3.
         static_assert(Cfg::kIssuers == 1 || kOut < 4, "one issuer: TMEM column = tile column");
-        const int sub = warp >= 11 ? 1 : 0;
-        auto release = [&]() {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader0);
+        const int sub = (warp - 8) / 4;
+        const int row0 = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32;
+        uint8_t* box = epi_smem + (quad * 2 + sub) * 4096;
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_ld_32x32b_x32(t_row + ((c / 2) * 2 + sub) * 64 + (c & 1) * 32, r[c]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader0);
+        const EpiParams& e = p.epi;
+        const bool boxed = e.out_kind == kEpiBf16 && p.n_out > 0;
+        // Half h (32 columns) of the warp's 64-column output box at column c0.
+        auto put = [&](const float(&y)[32], int h, int c0, int n_out) {
+          if (!boxed) {
+            epi_store(e, y, row, c0 + 32 * h, p.m, n_out);
+            return;
+          }
+          if (h == 0) {
+            if (lane == 0) tma_store_wait_read<0>();  // the box's previous store has read it
+            __syncwarp();
+          }
+          uint32_t w[16];
+          epi_pack(y, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) * 16)) =
+                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          if (h == 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&p.tm_out[0], box, c0, row0);
+              tma_store_commit();
+            }
+          }
         };
         if constexpr (kOut == 4) {
-#pragma unroll 1
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int tcol = (c / 2 * 2 + sub) * 64 + (c & 1) * 32;
-            uint32_t r[32];
-            __syncwarp();
-            tmem_ld_32x32b_x32(t_row + tcol, r);
-            tmem_wait_ld();
-            if (c == 3) release();
+            const int c0 = n0 + ((c / 2) * 2 + sub) * 64, col0 = c0 + (c & 1) * 32;
             float z[32];
-            epi_affine(p.epi, r, alpha, n0 + tcol, p.n, lane, z);
-            epi_checkpoint(p.epi, z, row, n0 + tcol, p.m, p.n);
-            epi_act(p.epi.act, z);
-            epi_finish(p.epi, z, row, n0 + tcol, p.m, p.n);
+            epi_affine(e, r[c], alpha, col0, p.n, lane, z);
+            epi_checkpoint(e, z, row, col0, p.m, p.n);
+            epi_act(e.act, z);
+            epi_residual(e, z, row, col0, p.m, p.n);
+            put(z, c & 1, c0, p.n);
           }
         } else {
-#pragma unroll 1
+#pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int tcol = sub * 64 + c * 32;
-            uint32_t r[32], f[32];
-            __syncwarp();
-            tmem_ld_32x32b_x32(t_row + tcol, r);
-            tmem_ld_32x32b_x32(t_row + kGateCols + tcol, f);
-            tmem_wait_ld();
-            if (c == 1) release();
             float z[32], u[32];
-            epi_affine(p.epi, r, alpha, n0 + tcol, p.n, lane, z);
-            epi_checkpoint(p.epi, z, row, n0 + tcol, p.m, p.n);
-            epi_affine(p.epi, f, alpha, n0 + kGateCols + tcol, p.n, lane, u);
-            epi_checkpoint(p.epi, u, row, n0 + kGateCols + tcol, p.m, p.n);
+            epi_affine(e, r[c], alpha, n0 + tcol, p.n, lane, z);
+            epi_checkpoint(e, z, row, n0 + tcol, p.m, p.n);
+            epi_affine(e, r[2 + c], alpha, n0 + kGateCols + tcol, p.n, lane, u);
+            epi_checkpoint(e, u, row, n0 + kGateCols + tcol, p.m, p.n);
 #pragma unroll
             for (int j = 0; j < 32; ++j) z[j] = act_fwd<kActSilu>(z[j]) * u[j];
-            epi_finish(p.epi, z, row, n0 / 2 + tcol, p.m, p.n / 2);
+            epi_residual(e, z, row, n0 / 2 + tcol, p.m, p.n / 2);
+            put(z, c, n0 / 2 + sub * 64, p.n / 2);
           }
         }
       } else if constexpr (kOut == 3) {
@@ -1016,7 +1066,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
     }
   }
 
-  if (Cfg::kEpiBytes > 0 && ((warp >= 2 && warp <= 5) || warp >= 11) && (threadIdx.x % 32) == 0)
+  if (Cfg::kEpiBytes > 0 && Roles::epilogue(warp) && (threadIdx.x % 32) == 0)
     tma_store_wait_all<0>();  // output stores done before shared memory is released
   tc_fence_before();
   cluster_sync();  // the leader's MMAs into both TMEMs are drained
@@ -1039,6 +1089,14 @@ static cudaError_t launch_pair_one(const GemmParams& p, int grid, cudaStream_t s
     cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
+    if constexpr (PairRoles<kOut>::kWide) {
+      // The register hand-over waits for good if its shares exceed what the
+      // CTA was launched with.
+      cudaFuncAttributes a{};
+      e = cudaFuncGetAttributes(&a, kern);
+      if (e != cudaSuccess) return e;
+      if (a.numRegs < PairRoles<kOut>::kRegsAtLaunch) return cudaErrorInvalidConfiguration;
+    }
     attr_done[dev] = true;
   }
   kern<<<grid, kOut >= 2 ? pair_threads<kOut>() : Cfg::kThreads, Cfg::kSmemBytes, stream>>>(p);

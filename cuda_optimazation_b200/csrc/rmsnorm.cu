@@ -374,58 +374,76 @@ __device__ __forceinline__ Vec8 bwd_dx(const Vec8& dy, const Vec8& h, const Vec8
   return d;
 }
 
-// dw of the 64 columns from col0 on, by one CTA: its warps take every
-// (warps)-th row, two columns a lane, and are joined in order.
+// dw of 128 bytes' worth of columns by one CTA of 16 warps: eight lanes span the
+// columns (16 bytes each), the warp's four such groups and the warps take the
+// rows in turn; the sums are joined in a fixed order.
 template <bool kBf16>
 __device__ __forceinline__ void column_dw(const RmsNormBwdParams& p, int64_t col0) {
-  __shared__ float2 sums[16][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int64_t col = col0 + 2 * lane;
-  float2 s = make_float2(0.0f, 0.0f);
+  constexpr int kPairs = kBf16 ? 4 : 2;  // column pairs of a lane
+  __shared__ float2 sums[16][8][kPairs];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t col = col0 + (lane & 7) * 2 * kPairs;
+  float2 s[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) s[i] = make_float2(0.0f, 0.0f);
   if (col < p.k) {
-#pragma unroll 8
-    for (int row = warp; row < static_cast<int>(p.rows); row += warps) {
-      float2 d, h;
-      if constexpr (kBf16) {
-        const uint32_t a = __ldg(reinterpret_cast<const uint32_t*>(
-            static_cast<const __nv_bfloat16*>(p.dy) + row * p.lddy + col));
-        const uint32_t b = __ldg(reinterpret_cast<const uint32_t*>(
-            static_cast<const __nv_bfloat16*>(p.h) + row * p.ldh + col));
-        d = make_float2(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
-        h = make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
-      } else {
-        d = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.dy) + row * p.lddy +
-                                                  col));
-        h = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.h) + row * p.ldh +
-                                                  col));
+    const uint8_t* dy = static_cast<const uint8_t*>(p.dy) + col * kElem<kBf16>;
+    const uint8_t* h = static_cast<const uint8_t*>(p.h) + col * kElem<kBf16>;
+#pragma unroll 4
+    for (int row = warp * 4 + (lane >> 3); row < static_cast<int>(p.rows); row += 64) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(dy + row * p.lddy * kElem<kBf16>));
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(h + row * p.ldh * kElem<kBf16>));
+      const float2 r = both(__ldg(p.rstd + row));
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        if constexpr (kBf16)
+          s[i] = fma2(make_float2(__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xffff0000u)),
+                      mul2(make_float2(__uint_as_float(y[i] << 16),
+                                       __uint_as_float(y[i] & 0xffff0000u)), r), s[i]);
+        else
+          s[i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])),
+                      mul2(make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])),
+                           r), s[i]);
       }
-      s = fma2(d, mul2(h, both(__ldg(p.rstd + row))), s);
     }
   }
-  sums[warp][lane] = s;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+#pragma unroll
+    for (int o = 8; o <= 16; o *= 2)
+      s[i] = add2(s[i], make_float2(__shfl_xor_sync(0xffffffffu, s[i].x, o),
+                                    __shfl_xor_sync(0xffffffffu, s[i].y, o)));
+    if (lane < 8) sums[warp][lane][i] = s[i];
+  }
   __syncthreads();
-  if (warp == 0 && col < p.k) {
-    for (int w = 1; w < warps; ++w) s = add2(s, sums[w][lane]);
-    p.dw[col] = s.x;
-    p.dw[col + 1] = s.y;
+  if (warp == 0 && lane < 8 && col < p.k) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      for (int w = 1; w < 16; ++w) s[i] = add2(s[i], sums[w][lane][i]);
+      p.dw[col + 2 * i] = s[i].x;
+      p.dw[col + 2 * i + 1] = s[i].y;
+    }
   }
 }
 
-// kColumns (few rows): CTA b takes row b, and CTAs past the rows the columns of
-// dw, which need no row's sum: dy and h are read twice, the second time from
-// L2, and nothing is left to join.  dx may not be dy then.
+// kColumns (few rows): the first CTAs take the columns of dw, which need no row's
+// sum, the others one row each: dy and h are read twice, the second time mostly
+// from L2, and nothing is left to join.  dx may not be dy then.
 // Otherwise CTA b takes rows b, b + grid, ...; each thread owns the same columns
 // of all of them, so its share of dw stays in registers and is written once, to
 // row b of the partial sums.
 template <bool kBf16, bool kWBf16, int kVec, bool kColumns>
-__global__ void __launch_bounds__(512) rmsnorm_backward_direct_kernel(const RmsNormBwdParams p) {
+__global__ void __launch_bounds__(512, kColumns && kVec <= 2 ? 2 : 1)
+    rmsnorm_backward_direct_kernel(const RmsNormBwdParams p) {
   __shared__ float red[32];
   if constexpr (kColumns) {
-    if (blockIdx.x >= p.rows) {
-      column_dw<kBf16>(p, (blockIdx.x - p.rows) * 64);
+    if (blockIdx.x + p.rows < gridDim.x) {
+      column_dw<kBf16>(p, static_cast<int64_t>(blockIdx.x) * (128 / kElem<kBf16>));
       return;
     }
   }
+  const int64_t first = kColumns ? blockIdx.x + p.rows - gridDim.x : blockIdx.x;
   const int nvec = static_cast<int>(p.k / 8);
   const float inv_k = 1.0f / static_cast<float>(p.k);
   Vec8 dw[kVec];
@@ -433,7 +451,7 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_direct_kernel(const RmsN
   for (int i = 0; i < kVec; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[i].v[j] = make_float2(0.0f, 0.0f);
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  for (int64_t row = first; row < p.rows; row += gridDim.x) {
     const float rstd = __ldg(p.rstd + row);
     Raw8<kBf16> dy[kVec], h[kVec];
     Raw8<kWBf16> w[kVec];
@@ -453,6 +471,8 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_direct_kernel(const RmsN
     for (int i = 0; i < kVec; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
       if (v < nvec) {
+        // By columns two CTAs share an SM's registers: w once more, from L1.
+        if (kColumns) w[i] = load_kept<kWBf16>(p.weight, v * 8);
         Vec8 d = bwd_dx(dy[i].decode(), h[i].decode(), w[i].decode(), rstd, c);
         if (p.dres) add_to(d, load_once<kBf16>(p.dres, row * p.lddres + v * 8).decode());
         store8<kBf16>(p.dx, row * p.lddx + v * 8, d);
@@ -702,7 +722,7 @@ int launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
     return p.dw ? r.grid : 0;
   }
   if (backward_by_columns(p.rows, p.k)) {
-    const int64_t columns = p.dw ? (p.k + 63) / 64 : 0;
+    const int64_t per = 128 / kElem<kBf16>, columns = p.dw ? (p.k + per - 1) / per : 0;
     launch_bwd_direct<kBf16, kWBf16, true>(p, static_cast<int>(p.rows + columns), stream);
     return 0;
   }

@@ -115,6 +115,18 @@ bool make_output_map(CUtensorMap* map, void* base, int64_t rows, int64_t cols, i
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Dense e4m3 output [rows][cols] as 64-column x 32-row TMA store boxes.
+bool make_mx_output_map(CUtensorMap* map, void* base, int64_t rows, int64_t cols) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols)};
+  const cuuint32_t box[2] = {64u, 32u};
+  const cuuint32_t estr[2] = {1u, 1u};
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                     CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 uint64_t default_timeout_ns() {
   static uint64_t t = [] {
     const char* e = std::getenv("QG_WAIT_TIMEOUT_NS");
@@ -293,12 +305,13 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
   }
   if (epi) {
     p.epi = *epi;
-    if (epi->out_kind == kEpiBf16 && epi->out_vec) {
-      if (!make_output_map(&p.tm_out[0], epi->out, m, epi->act == QG_ACT_SWIGLU ? n / 2 : n,
-                           epi->ldc))
-        return QG_ERR_CUDA;
-      p.n_out = 1;
+    const int64_t cols = epi->act == QG_ACT_SWIGLU ? n / 2 : n;
+    if (epi->out_kind == kEpiMxfp8) {
+      if (!make_mx_output_map(&p.tm_out[0], epi->out, m, cols)) return QG_ERR_CUDA;
+    } else if (epi->out_kind == kEpiBf16 && epi->out_vec) {
+      if (!make_output_map(&p.tm_out[0], epi->out, m, cols, epi->ldc)) return QG_ERR_CUDA;
     }
+    if (epi->z_q && !make_mx_output_map(&p.tm_out[1], epi->z_q, m, n)) return QG_ERR_CUDA;
   }
   p.a_ts = fmt == 1 ? a_ts : nullptr;
   p.b_ts = fmt == 1 ? b_ts : nullptr;

@@ -16,25 +16,26 @@
 
 namespace qg {
 
-// z of columns [col0, col0 + 32); lane j of the warp fetches bias[col0 + j]
-// for all of them.
-__device__ __forceinline__ void epi_affine(const EpiParams& e, const uint32_t (&acc)[32],
-                                           float alpha, int col0, int n, int lane,
-                                           float (&z)[32]) {
+// bias[col] (0 without one, or beyond it).
+__device__ __forceinline__ float epi_bias(const EpiParams& e, int col, int n) {
+  if (!e.bias || col >= n) return 0.0f;
+  return e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[col])
+                     : static_cast<const float*>(e.bias)[col];
+}
+
+// z = alpha acc + bias of 32 columns, in place; lane j of the warp holds the
+// bias of column j for all of them.
+__device__ __forceinline__ void epi_affine(const EpiParams& e, float (&z)[32], float alpha,
+                                           float bias) {
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
-    const float2 t = mul2(make_float2(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1])),
-                          both(alpha));
+    const float2 t = mul2(make_float2(z[j], z[j + 1]), both(alpha));
     z[j] = t.x;
     z[j + 1] = t.y;
   }
   if (e.bias) {
-    float b = 0.0f;
-    if (col0 + lane < n)
-      b = e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[col0 + lane])
-                      : static_cast<const float*>(e.bias)[col0 + lane];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) z[j] += __shfl_sync(0xffffffffu, b, j);
+    for (int j = 0; j < 32; ++j) z[j] += __shfl_sync(0xffffffffu, bias, j);
   }
 }
 
@@ -50,32 +51,22 @@ __device__ __forceinline__ void epi_act(int act, float (&z)[32]) {
   else if (act == kActGelu) epi_act_all<kActGelu>(z);
 }
 
-// One MX block of an MXFP8 matrix with n columns: 32 value bytes and its scale.
-// Rows and columns of the last scale chunks that lie beyond the matrix get
-// code 0.
-__device__ __forceinline__ void epi_store_mx(const float (&v)[32], uint8_t* q, uint8_t* sf,
-                                             int layout, int row_blocks, int sf_blocks, int row,
-                                             int col0, int m, int n) {
+// One MX block of an MXFP8 matrix with n columns: its scale goes to `sf`, its 32
+// value bytes to w.  Rows and columns of the last scale chunks that lie beyond
+// the matrix get code 0.
+__device__ __forceinline__ void epi_quantise(const float (&v)[32], uint8_t* sf, int layout,
+                                             int row_blocks, int sf_blocks, int row, int col0,
+                                             int m, int n, uint32_t (&w)[8]) {
   const bool in = row < m && col0 < n;
-  uint32_t code = 0;
-  if (in) {
-    float amax = 0.0f, mul;
+  float amax = 0.0f, mul;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) amax = max3_abs(amax, v[j], v[j + 1]);
-    code = mxfp8_scale_code(amax, mul);
-    uint4* dst = reinterpret_cast<uint4*>(q + static_cast<int64_t>(row) * n + col0);
+  for (int j = 0; j < 32; j += 2) amax = max3_abs(amax, v[j], v[j + 1]);
+  const uint32_t code = mxfp8_scale_code(in ? amax : 0.0f, mul);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 16 * h + 4 * i;
-        const float2 a = mul2(make_float2(v[j], v[j + 1]), both(mul));
-        const float2 b = mul2(make_float2(v[j + 2], v[j + 3]), both(mul));
-        w[i] = cvt_e4m3x4(a.x, a.y, b.x, b.y);
-      }
-      dst[h] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float2 a = mul2(make_float2(v[4 * i], v[4 * i + 1]), both(mul));
+    const float2 b = mul2(make_float2(v[4 * i + 2], v[4 * i + 3]), both(mul));
+    w[i] = cvt_e4m3x4(a.x, a.y, b.x, b.y);
   }
   if (layout == 0) {
     if (in) sf[static_cast<int64_t>(row) * (n / 32) + col0 / 32] = static_cast<uint8_t>(code);
@@ -85,47 +76,52 @@ __device__ __forceinline__ void epi_store_mx(const float (&v)[32], uint8_t* q, u
   }
 }
 
-// y += residual (n: the output's columns).
-__device__ __forceinline__ void epi_residual(const EpiParams& e, float (&y)[32], int row, int col0,
-                                             int m, int n) {
-  const bool full = col0 + 32 <= n;
-  if (e.res && row < m && col0 < n) {
-    const int64_t at = row * e.ldr + col0;
-    if (e.res_bf16) {
-      const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(e.res) + at;
-      if (full && e.res_vec) {
+// The residual of 32 columns of a row: fetched ahead of its use where 16-byte
+// loads can (the last columns of an odd row are read when they are added).
+struct EpiResidual {
+  uint4 v[8];
+};
+__device__ __forceinline__ void epi_fetch_residual(const EpiParams& e, EpiResidual& r, int row,
+                                                   int col0, int m, int n) {
+  if (!e.res || !e.res_vec || row >= m || col0 + 32 > n) return;
+  const uint8_t* at =
+      static_cast<const uint8_t*>(e.res) + (row * e.ldr + col0) * (e.res_bf16 ? 2 : 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 a = __ldg(reinterpret_cast<const uint4*>(r) + i);
-          const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  for (int i = 0; i < 4; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+  if (!e.res_bf16) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            y[8 * i + 2 * j] += __uint_as_float(w[j] << 16);
-            y[8 * i + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
-          }
-        }
-      } else {
+    for (int i = 4; i < 8; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+  }
+}
+__device__ __forceinline__ void epi_add_residual(const EpiParams& e, const EpiResidual& r,
+                                                 float (&y)[32], int row, int col0, int m, int n) {
+  if (!e.res || row >= m || col0 >= n) return;
+  const bool fetched = e.res_vec && col0 + 32 <= n;
+  if (fetched && e.res_bf16) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (col0 + j < n) y[j] += __bfloat162float(r[j]);
-      }
-    } else {
-      const float* r = static_cast<const float*>(e.res) + at;
-      if (full && e.res_vec) {
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w[4] = {r.v[i].x, r.v[i].y, r.v[i].z, r.v[i].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(r) + i);
-          y[4 * i] += a.x;
-          y[4 * i + 1] += a.y;
-          y[4 * i + 2] += a.z;
-          y[4 * i + 3] += a.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (col0 + j < n) y[j] += r[j];
+      for (int j = 0; j < 4; ++j) {
+        y[8 * i + 2 * j] += __uint_as_float(w[j] << 16);
+        y[8 * i + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
       }
     }
+  } else if (fetched) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[4 * i] += __uint_as_float(r.v[i].x);
+      y[4 * i + 1] += __uint_as_float(r.v[i].y);
+      y[4 * i + 2] += __uint_as_float(r.v[i].z);
+      y[4 * i + 3] += __uint_as_float(r.v[i].w);
+    }
+  } else {
+    const int64_t at = row * e.ldr + col0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < n)
+        y[j] += e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at + j])
+                           : static_cast<const float*>(e.res)[at + j];
   }
 }
 
@@ -138,30 +134,17 @@ __device__ __forceinline__ void epi_pack(const float (&y)[32], uint32_t (&w)[16]
   }
 }
 
-// The output, straight to global memory.
+// An fp32 output, or bf16 rows that TMA cannot store, straight to global memory.
 __device__ __forceinline__ void epi_store(const EpiParams& e, const float (&y)[32], int row,
                                           int col0, int m, int n) {
-  const bool in = row < m && col0 < n;
   const bool full = col0 + 32 <= n;
-  if (e.out_kind == kEpiMxfp8) {
-    epi_store_mx(y, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout, e.row_blocks,
-                 e.out_sf_blocks, row, col0, m, n);
-  } else if (in) {
+  if (row < m && col0 < n) {
     const int64_t at = row * e.ldc + col0;
     if (e.out_kind == kEpiBf16) {
       __nv_bfloat16* c = static_cast<__nv_bfloat16*>(e.out) + at;
-      if (full && e.out_vec) {
-        uint32_t w[16];
-        epi_pack(y, w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          reinterpret_cast<uint4*>(c)[i] =
-              make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (col0 + j < n) c[j] = __float2bfloat16_rn(y[j]);
-      }
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j < n) c[j] = __float2bfloat16_rn(y[j]);
     } else {
       float* c = static_cast<float*>(e.out) + at;
       if (full && e.out_vec) {
@@ -176,12 +159,6 @@ __device__ __forceinline__ void epi_store(const EpiParams& e, const float (&y)[3
       }
     }
   }
-}
-
-__device__ __forceinline__ void epi_checkpoint(const EpiParams& e, const float (&z)[32], int row,
-                                               int col0, int m, int n) {
-  if (e.z_q)
-    epi_store_mx(z, e.z_q, e.z_sf, e.z_layout, e.row_blocks, e.z_sf_blocks, row, col0, m, n);
 }
 
 }  // namespace qg

@@ -278,12 +278,7 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
   float bias[Cfg::kSets];
 #pragma unroll
   for (int s = 0; s < Cfg::kSets; ++s) {
-    bias[s] = 0.0f;
-    if (e.bias && in_z) {
-      const int c = col0 + s * 128 + f;
-      bias[s] = e.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[c])
-                            : static_cast<const float*>(e.bias)[c];
-    }
+    bias[s] = epi_bias(e, col0 + s * 128 + f, p.n);
   }
   float* part = reinterpret_cast<float*>(smem);  // [set][row of the pass][128]
   const uint32_t part_addr = smem_u32(part);

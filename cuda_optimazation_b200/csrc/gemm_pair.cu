@@ -235,7 +235,7 @@ constexpr int pair_threads() {
 // issuer before any of the epilogue's arithmetic: their warps are ordered by
 // warpgroup (producer and issuer; stagers; two of epilogue warps) and hand
 // registers over.  512 threads start with 128 registers each:
-// 64 + 64 + 192 + 192 = 4 x 128.
+// 80 + 64 + 184 + 184 = 4 x 128.
 template <int kOut>
 struct PairRoles {
   static constexpr bool kWide = kOut >= 4;
@@ -249,7 +249,8 @@ struct PairRoles {
   __device__ static bool epilogue(int warp) {
     return kWide ? warp >= 8 : (warp >= 2 && warp <= 5) || warp >= 11;
   }
-  static constexpr int kRegsAtLaunch = 128, kRegsFew = 64, kRegsEpilogue = 192;
+  static constexpr int kRegsAtLaunch = 128, kRegsFeeder = 48, kRegsStager = 64, kRegsEpilogue = 200;
+  static_assert(kRegsFeeder + kRegsStager + 2 * kRegsEpilogue <= 4 * kRegsAtLaunch, "shares");
 };
 
 // ------------------------------------------------------------------ tile scheduler
@@ -410,7 +411,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
   TileRing ring{tile_ids, tile_full, tile_empty, leader};
   using Roles = PairRoles<kOut>;
   if (Roles::feeder(warp)) {
-    if constexpr (Roles::kWide) reg_dealloc<Roles::kRegsFew>();
+    if constexpr (Roles::kWide) reg_dealloc<Roles::kRegsFeeder>();
     if (warp == 0 && lane == 0) {
       // -------------------------------------------------------------- TMA
       const uint64_t pol = l2_policy_evict_last();
@@ -634,7 +635,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
     }
   } else if (Roles::stager(warp)) {
     // ---------------------------------------------------------------- scale stagers
-    if constexpr (Roles::kWide) reg_dealloc<Roles::kRegsFew>();
+    if constexpr (Roles::kWide) reg_dealloc<Roles::kRegsStager>();
     const int quad = warp % 4;
     const uint32_t t_quad = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const bool no_wait = (kDiag & 32u) != 0, skip_st = (kDiag & 1u) != 0;
@@ -704,12 +705,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
     // NVFP4 output: 1 / tensor scale (IEEE division, as the reference's host
     // quantizer forms it) and the running amax of this lane's outputs.
     float rq_inv_ts = 1.0f, rq_max = 0.0f;
+    int half = 0;  // fused epilogues: the half of the warp's memory to write next
     if constexpr (kOut == 2) rq_inv_ts = __fdiv_rn(1.0f, p.rq_ts ? *p.rq_ts : 1.0f);
     for (int it = 0;; ++it) {
       const int tile = ring.next_warp(p, abort_flag, lane);
       if (tile < 0) break;
       int mt, nt;
       tile_coords(tile, p.num_m_tiles, p.num_n_tiles, mt, nt);
+      float bias[4];  // fused epilogues: of this lane's column of each 32-column run
+      if constexpr (kOut >= 4) {
+        // What the epilogue reads, on its way while the tile's MMAs run.
+        const int sub = (warp - 8) / 4, n_out = kOut == 5 ? p.n / 2 : p.n;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          bias[c] = epi_bias(p.epi, nt * Cfg::kBN + ((c / 2) * 2 + sub) * 64 + (c & 1) * 32 + lane,
+                             p.n);
+        const int row = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32 + lane;
+        if (p.epi.res && row < p.m) {
+#pragma unroll
+          for (int b = 0; b < (kOut == 5 ? 1 : 2); ++b) {
+            const int col = kOut == 5 ? nt * kGateCols + sub * 64
+                                      : nt * Cfg::kBN + (2 * b + sub) * 64;
+            if (col < n_out) prefetch_l2(static_cast<const uint8_t*>(p.epi.res) +
+                                         (row * p.epi.ldr + col) * (p.epi.res_bf16 ? 2 : 4));
+          }
+        }
+      }
       bool ok = true;
       if (lane == 0)
         ok = mbar_wait_bounded<false, 32>(acc_full, it & 1, p.timeout_ns, abort_flag, p.status,
@@ -803,71 +824,120 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         // 64-column blocks {sub, 2 + sub} (a gate block and its factors, for
         // the gated form), read them whole, hand the accumulator back and
         // work from registers while the next tile's MMAs run, 32 columns
-        // (one MX block) at a time.  bf16 rows that TMA can store leave
-        // through the warp's swizzled box, as in kind 3.
+        // (one MX block) at a time.  MXFP8 values and bf16 rows that TMA can
+        // store leave through the warp's 4 KB of shared memory: a lane's own
+        // stores would touch a line each and hold up the stagers' loads.
         static_assert(Cfg::kIssuers == 1 || kOut < 4, "one issuer: TMEM column = tile column");
         const int sub = (warp - 8) / 4;
         const int row0 = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32;
-        uint8_t* box = epi_smem + (quad * 2 + sub) * 4096;
-        uint32_t r[4][32];
+        uint8_t* boxes = epi_smem + (quad * 2 + sub) * 4096;
+        float z[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          tmem_ld_32x32b_x32(t_row + ((c / 2) * 2 + sub) * 64 + (c & 1) * 32, r[c]);
+          tmem_ld_32x32b_x32(t_row + ((c / 2) * 2 + sub) * 64 + (c & 1) * 32,
+                             reinterpret_cast<uint32_t(&)[32]>(z[c]));
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader0);
         const EpiParams& e = p.epi;
-        const bool boxed = e.out_kind == kEpiBf16 && p.n_out > 0;
-        // Half h (32 columns) of the warp's 64-column output box at column c0.
-        auto put = [&](const float(&y)[32], int h, int c0, int n_out) {
-          if (!boxed) {
-            epi_store(e, y, row, c0 + 32 * h, p.m, n_out);
-            return;
-          }
+        // z of 64-column block b of the warp starts at tile column:
+        auto zcol = [&](int b) { return n0 + (2 * b + sub) * 64; };
+        // MXFP8: 64 columns x 32 rows, 64 bytes a row (SWIZZLE_64B), in the two
+        // halves of the warp's memory by turns; before a half is written the
+        // store before the last has read it (all stores, beside bf16 boxes).
+        auto mx_half = [&](const float(&v)[32], int h, uint8_t* sf, int layout, int sf_blocks,
+                           int c0, int cols, const CUtensorMap* map) {
+          uint8_t* box = boxes + half * 2048;
           if (h == 0) {
-            if (lane == 0) tma_store_wait_read<0>();  // the box's previous store has read it
+            if (lane == 0) {
+              if (e.out_kind == kEpiMxfp8) tma_store_wait_read<1>();
+              else tma_store_wait_read<0>();
+            }
             __syncwarp();
           }
-          uint32_t w[16];
-          epi_pack(y, w);
+          uint32_t w[8];
+          epi_quantise(v, sf, layout, e.row_blocks, sf_blocks, row, c0 + 32 * h, p.m, cols, w);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(box + lane * 128 + (((4 * h + i) ^ (lane & 7)) * 16)) =
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(box + lane * 64 + (((2 * h + i) ^ ((lane >> 1) & 3)) * 16)) =
                 make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
           if (h == 1) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&p.tm_out[0], box, c0, row0);
+              tma_store_2d(map, box, c0, row0);
               tma_store_commit();
             }
+            half ^= 1;
           }
         };
-        if constexpr (kOut == 4) {
+        // Half h (32 columns) of the 64 output columns from c0 on.
+        auto put = [&](const float(&y)[32], int h, int c0, int cols) {
+          if (e.out_kind == kEpiMxfp8) {
+            mx_half(y, h, e.out_sf, e.out_layout, e.out_sf_blocks, c0, cols, &p.tm_out[0]);
+          } else if (e.out_kind == kEpiBf16 && e.out_vec) {
+            if (h == 0) {
+              if (lane == 0) tma_store_wait_read<0>();
+              __syncwarp();
+            }
+            uint32_t w[16];
+            epi_pack(y, w);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int c0 = n0 + ((c / 2) * 2 + sub) * 64, col0 = c0 + (c & 1) * 32;
-            float z[32];
-            epi_affine(e, r[c], alpha, col0, p.n, lane, z);
-            epi_checkpoint(e, z, row, col0, p.m, p.n);
-            epi_act(e.act, z);
-            epi_residual(e, z, row, col0, p.m, p.n);
-            put(z, c & 1, c0, p.n);
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(boxes + lane * 128 + (((4 * h + i) ^ (lane & 7)) * 16)) =
+                  make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            if (h == 1) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&p.tm_out[0], boxes, c0, row0);
+                tma_store_commit();
+              }
+            }
+          } else {
+            epi_store(e, y, row, c0 + 32 * h, p.m, cols);
+          }
+        };
+        EpiResidual res;
+        if constexpr (kOut == 4) {
+          epi_fetch_residual(e, res, row, zcol(0), p.m, p.n);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              epi_affine(e, z[2 * b + h], alpha, bias[2 * b + h]);
+              if (e.z_q)
+                mx_half(z[2 * b + h], h, e.z_sf, e.z_layout, e.z_sf_blocks, zcol(b), p.n,
+                        &p.tm_out[1]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = 2 * b + h;
+              epi_act(e.act, z[c]);
+              epi_add_residual(e, res, z[c], row, zcol(b) + 32 * h, p.m, p.n);
+              if (c < 3)
+                epi_fetch_residual(e, res, row, zcol((c + 1) / 2) + ((c + 1) & 1) * 32, p.m, p.n);
+              put(z[c], h, zcol(b), p.n);
+            }
           }
         } else {
+          const int c0 = n0 / 2 + sub * 64;
+          epi_fetch_residual(e, res, row, c0, p.m, p.n / 2);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            epi_affine(e, z[c], alpha, bias[c]);
+            if (e.z_q)
+              mx_half(z[c], c & 1, e.z_sf, e.z_layout, e.z_sf_blocks, zcol(c / 2), p.n,
+                      &p.tm_out[1]);
+          }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const int tcol = sub * 64 + c * 32;
-            float z[32], u[32];
-            epi_affine(e, r[c], alpha, n0 + tcol, p.n, lane, z);
-            epi_checkpoint(e, z, row, n0 + tcol, p.m, p.n);
-            epi_affine(e, r[2 + c], alpha, n0 + kGateCols + tcol, p.n, lane, u);
-            epi_checkpoint(e, u, row, n0 + kGateCols + tcol, p.m, p.n);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) z[j] = act_fwd<kActSilu>(z[j]) * u[j];
-            epi_residual(e, z, row, n0 / 2 + tcol, p.m, p.n / 2);
-            put(z, c, n0 / 2 + sub * 64, p.n / 2);
+            for (int j = 0; j < 32; ++j) z[c][j] = act_fwd<kActSilu>(z[c][j]) * z[2 + c][j];
+            epi_add_residual(e, res, z[c], row, c0 + c * 32, p.m, p.n / 2);
+            if (c == 0) epi_fetch_residual(e, res, row, c0 + 32, p.m, p.n / 2);
+            put(z[c], c, c0, p.n / 2);
           }
         }
       } else if constexpr (kOut == 3) {

@@ -40,8 +40,8 @@ namespace {
 
 constexpr int kTile = 128;  // rows, and columns of a set, of a CTA
 
-// Staging: a thread copies its own pieces of the tile into shared memory
-// (cp.async) before it works on any, and reads back only what it copied.
+// Staging: a thread copies its own pieces of a 32-row group into shared memory
+// (cp.async) two groups ahead of its work, and reads back only what it copied.
 template <int kBytes>
 __device__ __forceinline__ void stage_copy(uint8_t* to, const void* from) {
   if constexpr (kBytes == 16)
@@ -54,12 +54,9 @@ __device__ __forceinline__ void stage_copy(uint8_t* to, const void* from) {
 __device__ __forceinline__ void stage_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
-// All but the last `left` of the four row groups have arrived.
-__device__ __forceinline__ void stage_wait(int left) {
-  if (left >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
-  else if (left == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+template <int kLeft>
+__device__ __forceinline__ void stage_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
 // Eight gradients: 16 bytes of bf16, or two 16-byte pieces `second` apart.
@@ -83,9 +80,10 @@ __device__ __forceinline__ void read_grad8(const uint8_t* at, int second, float2
 // Eight values of an MXFP8 row with scale s.
 __device__ __forceinline__ void read_mx8(const uint8_t* at, float s, float2 (&v)[4]) {
   const uint2 w = *reinterpret_cast<const uint2*>(at);
+  e4m3x4_decode(w.x, v[0], v[1]);
+  e4m3x4_decode(w.y, v[2], v[3]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = mul2(e4m3x2_decode((i < 2 ? w.x : w.y) >> (16 * (i & 1))), both(s));
+  for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], both(s));
 }
 
 // Upper halves of two non-negative floats' patterns: b's in the high half.
@@ -140,62 +138,70 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
   const bool active = zc < p.n;  // p.n is a multiple of 32: a warp is in or out as a whole
   const int64_t row_blocks = (p.m + 127) / 128, n_blocks = (p.n + 127) / 128;
   const int64_t sf_blocks = (p.n / 32 + 3) / 4, t_blocks = (p.mt / 32 + 3) / 4;
-  // Staged pieces: [row group][row][gradient pieces, sets] of each thread.
+  // Staged pieces: [row][gradient pieces, sets] of each thread, one slot per row
+  // group where all are worked on at once, else two slots by turns.
+  constexpr int kSlots = kGroups > 1 ? kGroups : 2;
   uint8_t* stage_d = staged + (threadIdx.x & 127) * 16;
-  uint8_t* stage_z = staged + 16 * kGradBytes * 128 + (threadIdx.x & 127) * 8;
-  if (active) {
-    const uint8_t* d = static_cast<const uint8_t*>(p.dout) +
-                       ((m0 + group * 32 + rg * 4) * p.ldd + dc) * (kBf16 ? 2 : 4);
-    const uint8_t* z = p.z_q + (m0 + group * 32 + rg * 4) * p.n + zc;
+  uint8_t* stage_z = staged + kSlots * 4 * kGradBytes * 128 + (threadIdx.x & 127) * 8;
+  const uint8_t* d_next = static_cast<const uint8_t*>(p.dout) +
+                          ((m0 + group * 32 + rg * 4) * p.ldd + dc) * (kBf16 ? 2 : 4);
+  const uint8_t* z_next = p.z_q + (m0 + group * 32 + rg * 4) * p.n + zc;
+  const int64_t d_step = p.ldd * (kBf16 ? 2 : 4);
+  auto fetch = [&](int rb) {
+    const int slot = kGroups > 1 ? rb : rb & 1;
 #pragma unroll
-    for (int rb = group; rb < 4; rb += kGroups) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (rb * 32 + rg * 4 + i < rows) {
-          const int at = rb * 4 + i;
-          if constexpr (kGrad) {
-            stage_copy<16>(stage_d + at * kGradBytes * 128, d);
-            if constexpr (!kBf16) stage_copy<16>(stage_d + (at * 2 + 1) * 2048, d + 16);
-          }
-          if constexpr (kZ) {
-#pragma unroll
-            for (int s = 0; s < kSets; ++s)
-              stage_copy<8>(stage_z + (at * kSets + s) * 1024, z + s * kTile);
-          }
+    for (int i = 0; i < 4; ++i) {
+      if (rb * 32 + rg * 4 + i < rows) {
+        const int at = slot * 4 + i;
+        if constexpr (kGrad) {
+          stage_copy<16>(stage_d + at * kGradBytes * 128, d_next + i * d_step);
+          if constexpr (!kBf16)
+            stage_copy<16>(stage_d + (at * 2 + 1) * 2048, d_next + i * d_step + 16);
         }
-        d += p.ldd * (kBf16 ? 2 : 4);
-        z += p.n;
+        if constexpr (kZ) {
+#pragma unroll
+          for (int s = 0; s < kSets; ++s)
+            stage_copy<8>(stage_z + (at * kSets + s) * 1024, z_next + i * p.n + s * kTile);
+        }
       }
-      d += 28 * p.ldd * (kBf16 ? 2 : 4);
-      z += 28 * p.n;
-      stage_commit();
     }
+    d_next += 32 * d_step;
+    z_next += 32 * p.n;
+    stage_commit();
+  };
+  // Scales first: the CTA's barrier waits for them.
+  uint32_t zw[4] = {0, 0, 0, 0};
+  if (kZ && threadIdx.x < kSets * 32) {
+    // Row i's 16 bytes of the chunk: scales of rows i, i + 32, i + 64, i + 96.
+    const int i = threadIdx.x % 32;
+    const int64_t bs = static_cast<int64_t>(tc) * kSets + threadIdx.x / 32;
+    if (p.z_layout != 0) {
+      const int64_t chunk = p.z_layout == 1 ? bs * row_blocks + tm : tm * sf_blocks + bs;
+      const uint4 c = __ldg(reinterpret_cast<const uint4*>(p.z_sf + chunk * 512) + i);
+      zw[0] = c.x; zw[1] = c.y; zw[2] = c.z; zw[3] = c.w;
+    } else {
+      for (int r = 0; r < 4; ++r)
+        for (int c = 0; c < 4; ++c)
+          if (r * 32 + i < rows && bs * 4 + c < p.n / 32)
+            zw[r] |= static_cast<uint32_t>(
+                         __ldg(p.z_sf + (m0 + r * 32 + i) * (p.n / 32) + bs * 4 + c))
+                     << (8 * c);
+    }
+  }
+  if (active) {
+    fetch(group);
+    if constexpr (kGroups == 1) fetch(1);
   }
   if (threadIdx.x < kSets * 32) {
     const int s = threadIdx.x / 32, i = threadIdx.x % 32;
     row_sf[s][i] = make_uint4(0, 0, 0, 0);
     col_sf[s][i] = make_uint4(0, 0, 0, 0);
     if constexpr (kZ) {
-      // Row i's 16 bytes of the chunk: scales of rows i, i + 32, i + 64, i + 96.
-      const int64_t bs = static_cast<int64_t>(tc) * kSets + s;
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (p.z_layout != 0) {
-        const int64_t chunk = p.z_layout == 1 ? bs * row_blocks + tm : tm * sf_blocks + bs;
-        const uint4 c = __ldg(reinterpret_cast<const uint4*>(p.z_sf + chunk * 512) + i);
-        w[0] = c.x; w[1] = c.y; w[2] = c.z; w[3] = c.w;
-      } else {
-        for (int r = 0; r < 4; ++r)
-          for (int c = 0; c < 4; ++c)
-            if (r * 32 + i < rows && bs * 4 + c < p.n / 32)
-              w[r] |= static_cast<uint32_t>(
-                          __ldg(p.z_sf + (m0 + r * 32 + i) * (p.n / 32) + bs * 4 + c))
-                      << (8 * c);
-      }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          reinterpret_cast<float*>(z_scale[s][r][c])[i] = e8m0_decode(w[r] >> (8 * c) & 0xffu);
+          reinterpret_cast<float*>(z_scale[s][r][c])[i] = e8m0_decode(zw[r] >> (8 * c) & 0xffu);
     }
   }
   __syncthreads();
@@ -210,7 +216,8 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
 #pragma unroll 1
     for (int rb = group; rb * 32 < rows; rb += kGroups) {
       const int r0 = rb * 32 + rg * 4;  // this lane's first row of the tile
-      stage_wait(kGroups > 1 ? 0 : 3 - rb);
+      const int slot = kGroups > 1 ? rb : rb & 1;
+      stage_wait<(kGroups > 1 ? 0 : 1)>();
       float2 v[kSets][4][4];
       float zs[kSets][4];
       if constexpr (kZ) {
@@ -223,7 +230,7 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (r0 + i < rows) {
-          const int at = rb * 4 + i;
+          const int at = slot * 4 + i;
           float2 d[4];
           if constexpr (kGrad)
             read_grad8<kBf16>(stage_d + at * kGradBytes * 128, 2048, d);
@@ -249,6 +256,7 @@ __global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBa
             for (int j = 0; j < 4; ++j) v[s][i][j] = make_float2(0.0f, 0.0f);
         }
       }
+      if constexpr (kGroups == 1) fetch(rb + 2);  // the slot has been read
 #pragma unroll
       for (int s = 0; s < kSets; ++s) {
         float2 (&x)[4][4] = v[s];
@@ -406,7 +414,7 @@ constexpr int kClusterRows = 8;
 
 template <int kAct, bool kBf16, int kGroups>
 cudaError_t launch_one(const ActBackwardParams& p, int grid, cudaStream_t stream) {
-  constexpr int kSmem = staged_bytes<kAct, kBf16>() * 4 * 128;
+  constexpr int kSmem = staged_bytes<kAct, kBf16>() * (kGroups > 1 ? kGroups : 2) * 128;
   auto kernel = act_backward_kernel<kAct, kBf16, kGroups>;
   static bool done[kMaxDevices] = {};
   int dev = 0;

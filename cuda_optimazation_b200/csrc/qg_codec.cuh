@@ -69,8 +69,15 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
   return r;
 }
 
+// Four values -> four bytes, a's the lowest; the second conversion fills the upper
+// half of the first one's register.
 __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float d) {
-  return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16);
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
 }
 
 // ue8m0 code of a block with largest magnitude `amax` (the MXFP8 quantizer's
@@ -129,11 +136,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Two e4m3 bytes -> two floats (exact: every e4m3 value is an f16 value).
-__device__ __forceinline__ float2 e4m3x2_decode(uint32_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
-  return __half22float2(*reinterpret_cast<__half2*>(&h));
+// Four e4m3 bytes -> four floats (exact: every e4m3 value is an f16 value).
+__device__ __forceinline__ void e4m3x4_decode(uint32_t four, float2& lo, float2& hi) {
+  uint32_t a, b;
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+      : "=r"(a), "=r"(b)
+      : "r"(four));
+  lo = __half22float2(*reinterpret_cast<__half2*>(&a));
+  hi = __half22float2(*reinterpret_cast<__half2*>(&b));
 }
 
 template <bool kBf16>

@@ -114,7 +114,8 @@ constexpr int staged_bytes() {
 // kAct < 0: z itself (the transposition).  kGroups: 32-row groups of the tile
 // that are worked on at once, by four warps each.
 template <int kAct, bool kBf16, int kGroups>
-__global__ void __launch_bounds__(128 * kGroups) act_backward_kernel(const ActBackwardParams p) {
+__global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwiglu ? 4 : 0)
+    act_backward_kernel(const ActBackwardParams p) {
   constexpr int kSets = kAct == kActSwiglu ? 2 : 1;
   constexpr bool kGrad = kAct >= 0, kZ = kAct != kActNone;
   constexpr int kGradBytes = kGrad ? (kBf16 ? 16 : 32) : 0;

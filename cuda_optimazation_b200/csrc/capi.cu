@@ -102,16 +102,18 @@ bool make_scale_map(CUtensorMap* m, const void* base, int64_t mn, int64_t k, int
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// bf16 output [rows][cols] with row stride ldc elements, as 64-column x
-// 32-row TMA store boxes with the 128-byte swizzle of the staging buffer.
-bool make_output_map(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t ldc) {
+// bf16 (f32: fp32) output [rows][cols] with row stride ldc elements, as 64-column
+// (32) x 32-row TMA store boxes with the 128-byte swizzle of the staging buffer.
+bool make_output_map(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t ldc,
+                     bool f32 = false) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldc * 2)};
-  const cuuint32_t box[2] = {64u, 32u};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldc * (f32 ? 4 : 2))};
+  const cuuint32_t box[2] = {f32 ? 32u : 64u, 32u};
   const cuuint32_t estr[2] = {1u, 1u};
-  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                     CU_TENSOR_MAP_L2_PROMOTION_NONE,
+  return encode_fn()(map,
+                     f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                     base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -308,8 +310,9 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
     const int64_t cols = epi->act == QG_ACT_SWIGLU ? n / 2 : n;
     if (epi->out_kind == kEpiMxfp8) {
       if (!make_mx_output_map(&p.tm_out[0], epi->out, m, cols)) return QG_ERR_CUDA;
-    } else if (epi->out_kind == kEpiBf16 && epi->out_vec) {
-      if (!make_output_map(&p.tm_out[0], epi->out, m, cols, epi->ldc)) return QG_ERR_CUDA;
+    } else if (epi->out_vec) {
+      if (!make_output_map(&p.tm_out[0], epi->out, m, cols, epi->ldc, epi->out_kind == kEpiF32))
+        return QG_ERR_CUDA;
     }
     if (epi->z_q && !make_mx_output_map(&p.tm_out[1], epi->z_q, m, n)) return QG_ERR_CUDA;
   }

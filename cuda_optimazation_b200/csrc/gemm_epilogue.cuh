@@ -77,7 +77,7 @@ __device__ __forceinline__ void epi_quantise(const float (&v)[32], uint8_t* sf, 
 }
 
 // The residual of 32 columns of a row: fetched ahead of its use where 16-byte
-// loads can (the last columns of an odd row are read when they are added).
+// loads can.
 struct EpiResidual {
   uint4 v[8];
 };
@@ -93,10 +93,13 @@ __device__ __forceinline__ void epi_fetch_residual(const EpiParams& e, EpiResidu
     for (int i = 4; i < 8; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
   }
 }
+// `turn`: 4 KB of shared memory of the warp, free to use; every lane takes part.
 __device__ __forceinline__ void epi_add_residual(const EpiParams& e, const EpiResidual& r,
-                                                 float (&y)[32], int row, int col0, int m, int n) {
-  if (!e.res || row >= m || col0 >= n) return;
+                                                 float (&y)[32], int row, int col0, int m, int n,
+                                                 float* turn) {
+  if (!e.res || col0 >= n) return;
   const bool fetched = e.res_vec && col0 + 32 <= n;
+  if (fetched && row >= m) return;
   if (fetched && e.res_bf16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -116,12 +119,24 @@ __device__ __forceinline__ void epi_add_residual(const EpiParams& e, const EpiRe
       y[4 * i + 3] += __uint_as_float(r.v[i].w);
     }
   } else {
-    const int64_t at = row * e.ldr + col0;
+    // Rows that start anywhere, or end inside the run: the warp fetches its 32
+    // rows one by one, a lane a column, and turns them in shared memory.
+    const int lane = threadIdx.x & 31, row0 = row - lane;
+    const bool in = col0 + lane < n;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      float v = 0.0f;
+      if (in && row0 + r < m) {
+        const int64_t at = (row0 + r) * e.ldr + col0 + lane;
+        v = e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at])
+                       : static_cast<const float*>(e.res)[at];
+      }
+      turn[r * 32 + (lane ^ r)] = v;
+    }
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col0 + j < n)
-        y[j] += e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at + j])
-                           : static_cast<const float*>(e.res)[at + j];
+    for (int j = 0; j < 32; ++j) y[j] += turn[lane * 32 + (j ^ lane)];
+    __syncwarp();
   }
 }
 
@@ -134,31 +149,24 @@ __device__ __forceinline__ void epi_pack(const float (&y)[32], uint32_t (&w)[16]
   }
 }
 
-// An fp32 output, or bf16 rows that TMA cannot store, straight to global memory.
-__device__ __forceinline__ void epi_store(const EpiParams& e, const float (&y)[32], int row,
-                                          int col0, int m, int n) {
-  const bool full = col0 + 32 <= n;
-  if (row < m && col0 < n) {
-    const int64_t at = row * e.ldc + col0;
-    if (e.out_kind == kEpiBf16) {
-      __nv_bfloat16* c = static_cast<__nv_bfloat16*>(e.out) + at;
+// Output rows that TMA cannot store (not 16-byte aligned): turned in the warp's
+// shared memory, then stored one by one, a lane a column.
+__device__ __forceinline__ void epi_store_turned(const EpiParams& e, const float (&y)[32], int row,
+                                                 int col0, int m, int n, float* turn) {
+  const int lane = threadIdx.x & 31, row0 = row - lane;
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col0 + j < n) c[j] = __float2bfloat16_rn(y[j]);
-    } else {
-      float* c = static_cast<float*>(e.out) + at;
-      if (full && e.out_vec) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          reinterpret_cast<float4*>(c)[i] =
-              make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (col0 + j < n) c[j] = y[j];
-      }
+  for (int j = 0; j < 32; ++j) turn[lane * 32 + (j ^ lane)] = y[j];
+  __syncwarp();
+  if (col0 + lane < n) {
+#pragma unroll 8
+    for (int r = 0; r < 32 && row0 + r < m; ++r) {
+      const float v = turn[r * 32 + (lane ^ r)];
+      const int64_t at = (row0 + r) * e.ldc + col0 + lane;
+      if (e.out_kind == kEpiBf16) static_cast<__nv_bfloat16*>(e.out)[at] = __float2bfloat16_rn(v);
+      else static_cast<float*>(e.out)[at] = v;
     }
   }
+  __syncwarp();
 }
 
 }  // namespace qg

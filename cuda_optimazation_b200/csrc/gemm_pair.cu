@@ -872,32 +872,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
             half ^= 1;
           }
         };
+        auto boxes_free = [&]() {
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+        };
+        auto send = [&](const CUtensorMap* map, int c0) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(map, boxes, c0, row0);
+            tma_store_commit();
+          }
+        };
         // Half h (32 columns) of the 64 output columns from c0 on.
         auto put = [&](const float(&y)[32], int h, int c0, int cols) {
           if (e.out_kind == kEpiMxfp8) {
             mx_half(y, h, e.out_sf, e.out_layout, e.out_sf_blocks, c0, cols, &p.tm_out[0]);
-          } else if (e.out_kind == kEpiBf16 && e.out_vec) {
-            if (h == 0) {
-              if (lane == 0) tma_store_wait_read<0>();
-              __syncwarp();
-            }
+          } else if (!e.out_vec) {
+            boxes_free();
+            epi_store_turned(e, y, row, c0 + 32 * h, p.m, cols, reinterpret_cast<float*>(boxes));
+          } else if (e.out_kind == kEpiBf16) {
+            // 64 columns to a box.
+            if (h == 0) boxes_free();
             uint32_t w[16];
             epi_pack(y, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               *reinterpret_cast<uint4*>(boxes + lane * 128 + (((4 * h + i) ^ (lane & 7)) * 16)) =
                   make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-            if (h == 1) {
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_2d(&p.tm_out[0], boxes, c0, row0);
-                tma_store_commit();
-              }
-            }
+            if (h == 1) send(&p.tm_out[0], c0);
           } else {
-            epi_store(e, y, row, c0 + 32 * h, p.m, cols);
+            // fp32: 32 columns to a box.
+            boxes_free();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(boxes + lane * 128 + ((i ^ (lane & 7)) * 16)) =
+                  make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            send(&p.tm_out[0], c0 + 32 * h);
           }
+        };
+        // The residual's odd rows are turned in the boxes (which hold no output then:
+        // both halves of a block are added before either is put).
+        auto add_residual = [&](const EpiResidual& r, float(&y)[32], int col0, int cols) {
+          if (e.res && !(e.res_vec && col0 + 32 <= cols)) boxes_free();
+          epi_add_residual(e, r, y, row, col0, p.m, cols, reinterpret_cast<float*>(boxes));
         };
         EpiResidual res;
         if constexpr (kOut == 4) {
@@ -915,11 +933,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
             for (int h = 0; h < 2; ++h) {
               const int c = 2 * b + h;
               epi_act(e.act, z[c]);
-              epi_add_residual(e, res, z[c], row, zcol(b) + 32 * h, p.m, p.n);
+              add_residual(res, z[c], zcol(b) + 32 * h, p.n);
               if (c < 3)
                 epi_fetch_residual(e, res, row, zcol((c + 1) / 2) + ((c + 1) & 1) * 32, p.m, p.n);
-              put(z[c], h, zcol(b), p.n);
             }
+            put(z[2 * b], 0, zcol(b), p.n);
+            put(z[2 * b + 1], 1, zcol(b), p.n);
           }
         } else {
           const int c0 = n0 / 2 + sub * 64;
@@ -935,10 +954,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) z[c][j] = act_fwd<kActSilu>(z[c][j]) * z[2 + c][j];
-            epi_add_residual(e, res, z[c], row, c0 + c * 32, p.m, p.n / 2);
+            add_residual(res, z[c], c0 + c * 32, p.n / 2);
             if (c == 0) epi_fetch_residual(e, res, row, c0 + 32, p.m, p.n / 2);
-            put(z[c], c, c0, p.n / 2);
           }
+          put(z[0], 0, c0, p.n / 2);
+          put(z[1], 1, c0, p.n / 2);
         }
       } else if constexpr (kOut == 3) {
         // bf16 through TMA stores with eight epilogue warps (2-5, 11-14; two

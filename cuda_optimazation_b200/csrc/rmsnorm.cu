@@ -655,28 +655,30 @@ RowShape row_shape(int64_t k, int most) {
   return s;
 }
 
-template <typename K, typename P>
-void launch_ring(K kernel, const P& p, const RingShape& s, cudaStream_t stream) {
-  static bool done[kMaxDevices] = {};
+template <auto kKernel, typename P>
+cudaError_t launch_ring(const P& p, const RingShape& s, cudaStream_t stream) {
+  static bool done[kMaxDevices] = {};  // of this kernel
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
+    return cudaErrorInvalidDevice;
   if (!done[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem) !=
-        cudaSuccess)
-      return;
+    const cudaError_t e =
+        cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+    if (e != cudaSuccess) return e;
     done[dev] = true;
   }
-  kernel<<<s.grid, dim3(s.group, s.rows), s.smem, stream>>>(p);
+  kKernel<<<s.grid, dim3(s.group, s.rows), s.smem, stream>>>(p);
+  return cudaGetLastError();
 }
 
 template <bool kBf16, bool kWBf16>
-void launch_norm(const RmsNormParams& p, cudaStream_t stream) {
+cudaError_t launch_norm(const RmsNormParams& p, cudaStream_t stream) {
   const RingShape r =
       ring_shape(p.rows, p.k, p.k * kElem<kBf16> * (p.residual ? 2 : 1));
   if (r.stages == 3)
-    return launch_ring(rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 3>, p, r, stream);
+    return launch_ring<rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream);
   if (r.stages == 2)
-    return launch_ring(rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 2>, p, r, stream);
+    return launch_ring<rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 2>>(p, r, stream);
   const RowShape s = row_shape(p.k, 1024);
   // Padding words of the last chunks, four per thread.
   int pads = 0;
@@ -686,6 +688,7 @@ void launch_norm(const RmsNormParams& p, cudaStream_t stream) {
   if (s.vec == 1) rmsnorm_direct_kernel<kBf16, kWBf16, 1><<<grid, s.threads, 0, stream>>>(p);
   else if (s.vec == 2) rmsnorm_direct_kernel<kBf16, kWBf16, 2><<<grid, s.threads, 0, stream>>>(p);
   else rmsnorm_direct_kernel<kBf16, kWBf16, 4><<<grid, s.threads, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
 int backward_direct_grid(int64_t rows) {
@@ -697,7 +700,7 @@ int backward_direct_grid(int64_t rows) {
 bool backward_by_columns(int64_t rows, int64_t k) { return rows <= 512 && rows * k <= 4 << 20; }
 
 template <bool kBf16, bool kWBf16, bool kColumns>
-void launch_bwd_direct(const RmsNormBwdParams& p, int grid, cudaStream_t stream) {
+cudaError_t launch_bwd_direct(const RmsNormBwdParams& p, int grid, cudaStream_t stream) {
   RowShape s = row_shape(p.k, 512);
   if (kColumns) s.threads = 512;
   if (s.vec == 1)
@@ -708,36 +711,37 @@ void launch_bwd_direct(const RmsNormBwdParams& p, int grid, cudaStream_t stream)
     rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4, kColumns><<<grid, s.threads, 0, stream>>>(p);
   else
     rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8, kColumns><<<grid, s.threads, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
-// Returns the rows of partial sums that were written (0: dw is done).
 template <bool kBf16, bool kWBf16>
-int launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
+cudaError_t launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
   const RingShape r = ring_shape(p.rows, p.k, p.k * kElem<kBf16> * (p.dres ? 3 : 2));
+  int parts;
+  cudaError_t e;
   if (r.stages) {
-    if (r.stages == 3)
-      launch_ring(rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 3>, p, r, stream);
-    else
-      launch_ring(rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 2>, p, r, stream);
-    return p.dw ? r.grid : 0;
-  }
-  if (backward_by_columns(p.rows, p.k)) {
+    parts = r.grid;
+    e = r.stages == 3
+            ? launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream)
+            : launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 2>>(p, r, stream);
+  } else if (backward_by_columns(p.rows, p.k)) {
     const int64_t per = 128 / kElem<kBf16>, columns = p.dw ? (p.k + per - 1) / per : 0;
-    launch_bwd_direct<kBf16, kWBf16, true>(p, static_cast<int>(p.rows + columns), stream);
-    return 0;
+    return launch_bwd_direct<kBf16, kWBf16, true>(p, static_cast<int>(p.rows + columns), stream);
+  } else {
+    parts = backward_direct_grid(p.rows);
+    e = launch_bwd_direct<kBf16, kWBf16, false>(p, parts, stream);
   }
-  const int grid = backward_direct_grid(p.rows);
-  launch_bwd_direct<kBf16, kWBf16, false>(p, grid, stream);
-  return p.dw ? grid : 0;
+  if (e != cudaSuccess || !p.dw) return e;
+  return launch_column_sum(p.dw_part, parts, p.k, p.dw, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
                                  cudaStream_t stream) {
-  if (bf16) w_bf16 ? launch_norm<true, true>(p, stream) : launch_norm<true, false>(p, stream);
-  else w_bf16 ? launch_norm<false, true>(p, stream) : launch_norm<false, false>(p, stream);
-  return cudaGetLastError();
+  if (bf16)
+    return w_bf16 ? launch_norm<true, true>(p, stream) : launch_norm<true, false>(p, stream);
+  return w_bf16 ? launch_norm<false, true>(p, stream) : launch_norm<false, false>(p, stream);
 }
 
 int rmsnorm_backward_parts(int64_t rows, int64_t k) {
@@ -752,15 +756,11 @@ int rmsnorm_backward_parts(int64_t rows, int64_t k) {
 
 cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w_bf16,
                                     cudaStream_t stream) {
-  int parts;
   if (bf16)
-    parts = w_bf16 ? launch_norm_bwd<true, true>(p, stream) : launch_norm_bwd<true, false>(p, stream);
-  else
-    parts = w_bf16 ? launch_norm_bwd<false, true>(p, stream)
-                   : launch_norm_bwd<false, false>(p, stream);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || !parts) return e;
-  return launch_column_sum(p.dw_part, parts, p.k, p.dw, stream);
+    return w_bf16 ? launch_norm_bwd<true, true>(p, stream)
+                  : launch_norm_bwd<true, false>(p, stream);
+  return w_bf16 ? launch_norm_bwd<false, true>(p, stream)
+                : launch_norm_bwd<false, false>(p, stream);
 }
 
 cudaError_t launch_column_sum(const float* part, int parts, int64_t k, float* out,

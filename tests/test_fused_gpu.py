@@ -39,7 +39,8 @@ def close(got, ref, tol):
 
 # ------------------------------------------------------------------ RMS norm
 NORM = [(1, 32), (1, 8192), (3, 96), (127, 160), (128, 4096), (129, 5152), (300, 64), (2, 16416),
-        (5, 32768), (1000, 1024)]
+        (5, 32768), (1000, 1024), (14171, 640), (5000, 2048), (1500, 8192), (700, 13056),
+        (400, 16384), (600, 32768)]
 
 
 @pytest.mark.parametrize("rows,k", NORM)
@@ -212,6 +213,14 @@ SHAPES = [(1, 256, 32), (1, 4096, 2048), (2, 33, 96), (7, 512, 4000), (16, 1000,
 def test_gemm_shapes(F, qlib, m, n, k, fmt):
     gemm_case(F, qlib, m, n, k, fmt, act="gelu", bias="f32", res="bf16",
               out="bf16" if n % 2 else "f32")
+
+
+@pytest.mark.parametrize("m,n", [(150, 1959), (300, 70), (257, 8)])
+@pytest.mark.parametrize("res", [None, "bf16", "f32"])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_gemm_odd_rows(F, qlib, m, n, res, out):
+    """Rows whose starts 16-byte accesses cannot use."""
+    gemm_case(F, qlib, m, n, 96, act="silu", bias="bf16", res=res, out=out)
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "swiglu"])

@@ -76,14 +76,14 @@ __device__ __forceinline__ void epi_quantise(const float (&v)[32], uint8_t* sf, 
   }
 }
 
-// The residual of 32 columns of a row: fetched ahead of its use where 16-byte
-// loads can.
+// The residual of 32 columns of a row of 16-byte aligned rows, fetched ahead of its
+// use.
 struct EpiResidual {
   uint4 v[8];
 };
 __device__ __forceinline__ void epi_fetch_residual(const EpiParams& e, EpiResidual& r, int row,
                                                    int col0, int m, int n) {
-  if (!e.res || !e.res_vec || row >= m || col0 + 32 > n) return;
+  if (!e.res || row >= m || col0 + 32 > n) return;
   const uint8_t* at =
       static_cast<const uint8_t*>(e.res) + (row * e.ldr + col0) * (e.res_bf16 ? 2 : 4);
 #pragma unroll
@@ -93,14 +93,17 @@ __device__ __forceinline__ void epi_fetch_residual(const EpiParams& e, EpiResidu
     for (int i = 4; i < 8; ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
   }
 }
-// `turn`: 4 KB of shared memory of the warp, free to use; every lane takes part.
 __device__ __forceinline__ void epi_add_residual(const EpiParams& e, const EpiResidual& r,
-                                                 float (&y)[32], int row, int col0, int m, int n,
-                                                 float* turn) {
-  if (!e.res || col0 >= n) return;
-  const bool fetched = e.res_vec && col0 + 32 <= n;
-  if (fetched && row >= m) return;
-  if (fetched && e.res_bf16) {
+                                                 float (&y)[32], int row, int col0, int m, int n) {
+  if (!e.res || row >= m || col0 >= n) return;
+  if (col0 + 32 > n) {  // the last columns of a row
+    const int64_t at = row * e.ldr + col0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < n)
+        y[j] += e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at + j])
+                           : static_cast<const float*>(e.res)[at + j];
+  } else if (e.res_bf16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t w[4] = {r.v[i].x, r.v[i].y, r.v[i].z, r.v[i].w};
@@ -110,7 +113,7 @@ __device__ __forceinline__ void epi_add_residual(const EpiParams& e, const EpiRe
         y[8 * i + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
       }
     }
-  } else if (fetched) {
+  } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       y[4 * i] += __uint_as_float(r.v[i].x);
@@ -118,26 +121,37 @@ __device__ __forceinline__ void epi_add_residual(const EpiParams& e, const EpiRe
       y[4 * i + 2] += __uint_as_float(r.v[i].z);
       y[4 * i + 3] += __uint_as_float(r.v[i].w);
     }
-  } else {
-    // Rows that start anywhere, or end inside the run: the warp fetches its 32
-    // rows one by one, a lane a column, and turns them in shared memory.
-    const int lane = threadIdx.x & 31, row0 = row - lane;
-    const bool in = col0 + lane < n;
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-      float v = 0.0f;
-      if (in && row0 + r < m) {
-        const int64_t at = (row0 + r) * e.ldr + col0 + lane;
-        v = e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at])
-                       : static_cast<const float*>(e.res)[at];
-      }
-      turn[r * 32 + (lane ^ r)] = v;
-    }
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] += turn[lane * 32 + (j ^ lane)];
-    __syncwarp();
   }
+}
+
+// The same for rows that start anywhere: the warp fetches its 32 rows at once, a
+// lane a column, and turns them in 4 KB of its shared memory.
+__device__ __forceinline__ void epi_fetch_rows(const EpiParams& e, float (&v)[32], int row0,
+                                               int col0, int m, int n) {
+  if (!e.res) return;
+  const int lane = threadIdx.x & 31;
+  const bool in = col0 + lane < n;
+  if (e.res_bf16) {
+    const __nv_bfloat16* at = static_cast<const __nv_bfloat16*>(e.res) + row0 * e.ldr + col0 + lane;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      v[r] = in && row0 + r < m ? __bfloat162float(at[r * e.ldr]) : 0.0f;
+  } else {
+    const float* at = static_cast<const float*>(e.res) + row0 * e.ldr + col0 + lane;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) v[r] = in && row0 + r < m ? at[r * e.ldr] : 0.0f;
+  }
+}
+__device__ __forceinline__ void epi_add_rows(const EpiParams& e, const float (&v)[32],
+                                             float (&y)[32], float* turn) {
+  if (!e.res) return;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) turn[r * 32 + (lane ^ r)] = v[r];
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) y[j] += turn[lane * 32 + (j ^ lane)];
+  __syncwarp();
 }
 
 // 32 values as 16 words of bf16.
@@ -157,14 +171,18 @@ __device__ __forceinline__ void epi_store_turned(const EpiParams& e, const float
 #pragma unroll
   for (int j = 0; j < 32; ++j) turn[lane * 32 + (j ^ lane)] = y[j];
   __syncwarp();
-  if (col0 + lane < n) {
-#pragma unroll 8
-    for (int r = 0; r < 32 && row0 + r < m; ++r) {
-      const float v = turn[r * 32 + (lane ^ r)];
-      const int64_t at = (row0 + r) * e.ldc + col0 + lane;
-      if (e.out_kind == kEpiBf16) static_cast<__nv_bfloat16*>(e.out)[at] = __float2bfloat16_rn(v);
-      else static_cast<float*>(e.out)[at] = v;
-    }
+  const bool in = col0 + lane < n;
+  const int64_t first = row0 * e.ldc + col0 + lane;
+  if (e.out_kind == kEpiBf16) {
+    __nv_bfloat16* at = static_cast<__nv_bfloat16*>(e.out) + first;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (in && row0 + r < m) at[r * e.ldc] = __float2bfloat16_rn(turn[r * 32 + (lane ^ r)]);
+  } else {
+    float* at = static_cast<float*>(e.out) + first;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (in && row0 + r < m) at[r * e.ldc] = turn[r * 32 + (lane ^ r)];
   }
   __syncwarp();
 }

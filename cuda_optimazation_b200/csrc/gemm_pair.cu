@@ -221,7 +221,8 @@ __device__ __forceinline__ void tile_coords(int tile, int num_m_tiles, int num_n
 // GEMMsm110/include/backends/tc6_nvfp4.cuh:460-503).
 // 3: bf16 C through TMA stores.  4: the fused epilogue (bias, activation,
 // residual, MXFP8 checkpoint; gemm_epilogue.cuh), 5: the same with the gated
-// activation, whose gate columns are a tile's first 128 and factors its last.
+// activation, whose gate columns are a tile's first 128 and factors its last;
+// 6 and 7: the same two for rows that do not start on 16 bytes (see PairRoles).
 // Threads per CTA: 11 warps; the NVFP4-output epilogue (kOut 2), the
 // bf16 TMA-store epilogue (kOut 3) and the fused ones add four more epilogue
 // warps (11..14, one per TMEM lane quadrant).
@@ -230,15 +231,20 @@ constexpr int pair_threads() {
   return kOut >= 4 ? 512 : (kOut >= 2 ? 480 : 352);
 }
 
-// Warp roles.  The fused epilogues (kOut >= 4) hold a tile's 128 accumulator
-// columns of a row in registers, so that the accumulator goes back to the MMA
-// issuer before any of the epilogue's arithmetic: their warps are ordered by
-// warpgroup (producer and issuer; stagers; two of epilogue warps) and hand
-// registers over.  512 threads start with 128 registers each:
-// 80 + 64 + 184 + 184 = 4 x 128.
+// Warp roles.  The fused epilogues 4 and 5 hold a tile's 128 accumulator columns
+// of a row in registers, so that the accumulator goes back to the MMA issuer
+// before any of the epilogue's arithmetic: their warps are ordered by warpgroup
+// (producer and issuer; stagers; two of epilogue warps) and hand registers over.
+// 512 threads start with 128 registers each: 48 + 64 + 200 + 200 = 4 x 128.
+// The fused epilogues 6 and 7, for rows that TMA and 16-byte loads cannot take, go
+// through a row in a loop of 32 columns with the next columns' residual on its
+// way (see the launch rule in capi.cu).
 template <int kOut>
 struct PairRoles {
-  static constexpr bool kWide = kOut >= 4;
+  static constexpr bool kFused = kOut >= 4;
+  static constexpr bool kGated = kOut == 5 || kOut == 7;
+  static constexpr bool kHeld = kOut == 4 || kOut == 5;
+  static constexpr bool kWide = kFused;
   // The warps (a whole warpgroup, where registers change hands) of the producer
   // and the issuers.
   __device__ static bool feeder(int warp) { return kWide ? warp < 4 : warp == 0 || mma(warp); }
@@ -249,6 +255,8 @@ struct PairRoles {
   __device__ static bool epilogue(int warp) {
     return kWide ? warp >= 8 : (warp >= 2 && warp <= 5) || warp >= 11;
   }
+  // Which of a lane quadrant's two epilogue warps (eight-warp epilogues).
+  __device__ static int second(int warp) { return kWide ? (warp - 8) / 4 : (warp >= 11 ? 1 : 0); }
   static constexpr int kRegsAtLaunch = 128, kRegsFeeder = 48, kRegsStager = 64, kRegsEpilogue = 200;
   static_assert(kRegsFeeder + kRegsStager + 2 * kRegsEpilogue <= 4 * kRegsAtLaunch, "shares");
 };
@@ -713,9 +721,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
       int mt, nt;
       tile_coords(tile, p.num_m_tiles, p.num_n_tiles, mt, nt);
       float bias[4];  // fused epilogues: of this lane's column of each 32-column run
-      if constexpr (kOut >= 4) {
+      if constexpr (Roles::kFused) {
         // What the epilogue reads, on its way while the tile's MMAs run.
-        const int sub = (warp - 8) / 4, n_out = kOut == 5 ? p.n / 2 : p.n;
+        const int sub = Roles::second(warp), n_out = Roles::kGated ? p.n / 2 : p.n;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           bias[c] = epi_bias(p.epi, nt * Cfg::kBN + ((c / 2) * 2 + sub) * 64 + (c & 1) * 32 + lane,
@@ -723,11 +731,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         const int row = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32 + lane;
         if (p.epi.res && row < p.m) {
 #pragma unroll
-          for (int b = 0; b < (kOut == 5 ? 1 : 2); ++b) {
-            const int col = kOut == 5 ? nt * kGateCols + sub * 64
+          for (int b = 0; b < (Roles::kGated ? 1 : 2); ++b) {
+            const int col = Roles::kGated ? nt * kGateCols + sub * 64
                                       : nt * Cfg::kBN + (2 * b + sub) * 64;
-            if (col < n_out) prefetch_l2(static_cast<const uint8_t*>(p.epi.res) +
-                                         (row * p.epi.ldr + col) * (p.epi.res_bf16 ? 2 : 4));
+            if (col < n_out) {
+              const int size = p.epi.res_bf16 ? 2 : 4, run = n_out - col < 64 ? n_out - col : 64;
+              const uint8_t* at = static_cast<const uint8_t*>(p.epi.res) +
+                                  (row * p.epi.ldr + col) * size;
+              prefetch_l2(at);
+              if (size == 4 || !Roles::kHeld) prefetch_l2(at + run * size - 1);
+            }
           }
         }
       }
@@ -819,7 +832,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
               if (col0 + 16 * g < p.n) p.rq_sf[so + g] = static_cast<uint8_t>(sbits[g]);
           }
         }
-      } else if constexpr (kOut >= 4) {
+      } else if constexpr (Roles::kHeld) {
         // Fused epilogue.  The two warps of a TMEM lane quadrant take the
         // 64-column blocks {sub, 2 + sub} (a gate block and its factors, for
         // the gated form), read them whole, hand the accumulator back and
@@ -828,7 +841,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         // store leave through the warp's 4 KB of shared memory: a lane's own
         // stores would touch a line each and hold up the stagers' loads.
         static_assert(Cfg::kIssuers == 1 || kOut < 4, "one issuer: TMEM column = tile column");
-        const int sub = (warp - 8) / 4;
+        const int sub = Roles::second(warp);
         const int row0 = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32;
         uint8_t* boxes = epi_smem + (quad * 2 + sub) * 4096;
         float z[4][32];
@@ -888,9 +901,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         auto put = [&](const float(&y)[32], int h, int c0, int cols) {
           if (e.out_kind == kEpiMxfp8) {
             mx_half(y, h, e.out_sf, e.out_layout, e.out_sf_blocks, c0, cols, &p.tm_out[0]);
-          } else if (!e.out_vec) {
-            boxes_free();
-            epi_store_turned(e, y, row, c0 + 32 * h, p.m, cols, reinterpret_cast<float*>(boxes));
           } else if (e.out_kind == kEpiBf16) {
             // 64 columns to a box.
             if (h == 0) boxes_free();
@@ -911,12 +921,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
             send(&p.tm_out[0], c0 + 32 * h);
           }
         };
-        // The residual's odd rows are turned in the boxes (which hold no output then:
-        // both halves of a block are added before either is put).
-        auto add_residual = [&](const EpiResidual& r, float(&y)[32], int col0, int cols) {
-          if (e.res && !(e.res_vec && col0 + 32 <= cols)) boxes_free();
-          epi_add_residual(e, r, y, row, col0, p.m, cols, reinterpret_cast<float*>(boxes));
-        };
         EpiResidual res;
         if constexpr (kOut == 4) {
           epi_fetch_residual(e, res, row, zcol(0), p.m, p.n);
@@ -933,7 +937,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
             for (int h = 0; h < 2; ++h) {
               const int c = 2 * b + h;
               epi_act(e.act, z[c]);
-              add_residual(res, z[c], zcol(b) + 32 * h, p.n);
+              epi_add_residual(e, res, z[c], row, zcol(b) + 32 * h, p.m, p.n);
               if (c < 3)
                 epi_fetch_residual(e, res, row, zcol((c + 1) / 2) + ((c + 1) & 1) * 32, p.m, p.n);
             }
@@ -954,11 +958,94 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) z[c][j] = act_fwd<kActSilu>(z[c][j]) * z[2 + c][j];
-            add_residual(res, z[c], c0 + c * 32, p.n / 2);
+            epi_add_residual(e, res, z[c], row, c0 + c * 32, p.m, p.n / 2);
             if (c == 0) epi_fetch_residual(e, res, row, c0 + 32, p.m, p.n / 2);
           }
           put(z[0], 0, c0, p.n / 2);
           put(z[1], 1, c0, p.n / 2);
+        }
+      } else if constexpr (Roles::kFused) {
+        // The same, 32 columns at a time in a loop; MXFP8 boxes of 32 columns (the
+        // checkpoint's in the first 2 KB of the warp's memory, the output's
+        // behind them), odd rows turned in all 4 KB.
+        static_assert(Cfg::kIssuers == 1 || kOut < 4, "one issuer: TMEM column = tile column");
+        const int sub = Roles::second(warp);
+        const int row0 = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32;
+        uint8_t* boxes = epi_smem + (quad * 2 + sub) * 4096;
+        const EpiParams& e = p.epi;
+        auto boxes_free = [&]() {
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+        };
+        auto send = [&](const CUtensorMap* map, const uint8_t* box, int c0) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(map, box, c0, row0);
+            tma_store_commit();
+          }
+        };
+        auto put_mx = [&](const float(&v)[32], uint8_t* box, uint8_t* sf, int layout, int sf_blocks,
+                          int c0, int cols, const CUtensorMap* map) {
+          uint32_t w[8];
+          epi_quantise(v, sf, layout, e.row_blocks, sf_blocks, row, c0, p.m, cols, w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(box + lane * 32 + ((i ^ ((lane >> 2) & 1)) * 16)) =
+                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          send(map, box, c0);
+        };
+        const int cols = Roles::kGated ? p.n / 2 : p.n;
+        auto tile_col = [&](int c) {
+          return Roles::kGated ? sub * 64 + c * 32 : ((c / 2) * 2 + sub) * 64 + (c & 1) * 32;
+        };
+        auto out_col = [&](int c) { return (Roles::kGated ? n0 / 2 : n0) + tile_col(c); };
+        constexpr int kRuns = Roles::kGated ? 2 : 4;
+        float next[32];
+        epi_fetch_rows(e, next, row0, out_col(0), p.m, cols);
+#pragma unroll 1
+        for (int c = 0; c < kRuns; ++c) {
+          const int tcol = tile_col(c), c0 = out_col(c);
+          float res[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) res[j] = next[j];
+          if (c + 1 < kRuns) epi_fetch_rows(e, next, row0, out_col(c + 1), p.m, cols);
+          float z[32], u[Roles::kGated ? 32 : 1];
+          __syncwarp();
+          tmem_ld_32x32b_x32(t_row + tcol, reinterpret_cast<uint32_t(&)[32]>(z));
+          if constexpr (Roles::kGated)
+            tmem_ld_32x32b_x32(t_row + kGateCols + tcol, reinterpret_cast<uint32_t(&)[32]>(u));
+          tmem_wait_ld();
+          if (c == kRuns - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader0);
+          }
+          boxes_free();
+          epi_affine(e, z, alpha, c == 0 ? bias[0] : c == 1 ? bias[1] : c == 2 ? bias[2] : bias[3]);
+          if (e.z_q)
+            put_mx(z, boxes, e.z_sf, e.z_layout, e.z_sf_blocks, n0 + tcol, p.n, &p.tm_out[1]);
+          if constexpr (Roles::kGated) {
+            epi_affine(e, u, alpha, c == 0 ? bias[2] : bias[3]);
+            if (e.z_q)
+              put_mx(u, boxes + 1024, e.z_sf, e.z_layout, e.z_sf_blocks, n0 + kGateCols + tcol, p.n,
+                     &p.tm_out[1]);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[j] = act_fwd<kActSilu>(z[j]) * u[j];
+          } else {
+            epi_act(e.act, z);
+          }
+          if (e.res) {
+            boxes_free();
+            epi_add_rows(e, res, z, reinterpret_cast<float*>(boxes));
+          }
+          if (e.out_kind == kEpiMxfp8) {
+            put_mx(z, boxes + 2048, e.out_sf, e.out_layout, e.out_sf_blocks, c0, cols,
+                   &p.tm_out[0]);
+          } else {
+            boxes_free();
+            epi_store_turned(e, z, row, c0, p.m, cols, reinterpret_cast<float*>(boxes));
+          }
         }
       } else if constexpr (kOut == 3) {
         // bf16 through TMA stores with eight epilogue warps (2-5, 11-14; two
@@ -1193,18 +1280,21 @@ static cudaError_t launch_pair_one(const GemmParams& p, int grid, cudaStream_t s
   return cudaGetLastError();
 }
 
+template <int kFmt>
+static cudaError_t launch_pair_fused(const GemmParams& p, int out_kind, int grid,
+                                     cudaStream_t stream) {
+  if (out_kind == 4) return launch_pair_one<kFmt, 4>(p, grid, stream);
+  if (out_kind == 5) return launch_pair_one<kFmt, 5>(p, grid, stream);
+  if (out_kind == 6) return launch_pair_one<kFmt, 6>(p, grid, stream);
+  return launch_pair_one<kFmt, 7>(p, grid, stream);
+}
+
 cudaError_t launch_gemm_pair(const GemmParams& p, int fmt, int out_kind, int grid,
                              cudaStream_t stream) {
   if (out_kind >= 4) {
-    const bool gated = out_kind == 5;
-    if (fmt == kFmtNvfp4)
-      return gated ? launch_pair_one<kFmtNvfp4, 5>(p, grid, stream)
-                   : launch_pair_one<kFmtNvfp4, 4>(p, grid, stream);
-    if (fmt == kFmtMxfp4)
-      return gated ? launch_pair_one<kFmtMxfp4, 5>(p, grid, stream)
-                   : launch_pair_one<kFmtMxfp4, 4>(p, grid, stream);
-    return gated ? launch_pair_one<kFmtMxfp8, 5>(p, grid, stream)
-                 : launch_pair_one<kFmtMxfp8, 4>(p, grid, stream);
+    return fmt == kFmtNvfp4   ? launch_pair_fused<kFmtNvfp4>(p, out_kind, grid, stream)
+           : fmt == kFmtMxfp4 ? launch_pair_fused<kFmtMxfp4>(p, out_kind, grid, stream)
+                              : launch_pair_fused<kFmtMxfp8>(p, out_kind, grid, stream);
   }
   if (fmt == kFmtNvfp4) {
     if (out_kind == 3) return launch_pair_one<kFmtNvfp4, 3>(p, grid, stream);

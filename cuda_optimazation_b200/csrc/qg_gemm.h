@@ -79,7 +79,7 @@ struct GemmParams {
   int rq_row_blocks, rq_sf_blocks;
   uint32_t* status;
   uint64_t timeout_ns;
-  EpiParams epi;  // out_kind 4 / 5 of launch_gemm_pair
+  EpiParams epi;  // out_kind 4..7 of launch_gemm_pair, launch_gemm_fused_rows
 };
 
 // Decode-shaped NVFP4 GEMM (gemm_skinny.cu): weights W [n][k] on the MMA's M
@@ -138,7 +138,8 @@ cudaError_t launch_gemm_blockscaled(const GemmParams& p, bool fp4, bool out_bf16
                                     cudaStream_t stream);
 // fmt: 0 MXFP8, 1 NVFP4, 2 MXFP4.  out_kind: 0 fp32 C, 1 bf16 C, 2 NVFP4
 // output (rq_* fields; NVFP4 only), 3 bf16 C through TMA stores (n_out > 0)
-// with eight epilogue warps, 4 the fused epilogue (epi), 5 its gated form.
+// with eight epilogue warps, 4 the fused epilogue (epi), 5 its gated form, 6 and 7
+// these two for rows that do not start on 16 bytes.
 cudaError_t launch_gemm_pair(const GemmParams& p, int fmt, int out_kind, int grid,
                              cudaStream_t stream);
 int pair_sf_chunks_per_stage(int fmt);

@@ -125,29 +125,30 @@ __device__ __forceinline__ void epi_add_residual(const EpiParams& e, const EpiRe
 }
 
 // The same for rows that start anywhere: the warp fetches its 32 rows at once, a
-// lane a column, and turns them in 4 KB of its shared memory.
-__device__ __forceinline__ void epi_fetch_rows(const EpiParams& e, float (&v)[32], int row0,
+// lane a column, and turns them in 4 KB of its shared memory.  Places beyond the
+// matrix read its last row or column (and are never stored): no load is
+// conditional, so that none waits for another.  bf16 arrives as raw bits.
+__device__ __forceinline__ void epi_fetch_rows(const EpiParams& e, uint32_t (&v)[32], int row0,
                                                int col0, int m, int n) {
   if (!e.res) return;
-  const int lane = threadIdx.x & 31;
-  const bool in = col0 + lane < n;
+  const int col = min(col0 + static_cast<int>(threadIdx.x & 31), n - 1);
   if (e.res_bf16) {
-    const __nv_bfloat16* at = static_cast<const __nv_bfloat16*>(e.res) + row0 * e.ldr + col0 + lane;
+    const uint16_t* at = static_cast<const uint16_t*>(e.res) + col;
 #pragma unroll
-    for (int r = 0; r < 32; ++r)
-      v[r] = in && row0 + r < m ? __bfloat162float(at[r * e.ldr]) : 0.0f;
+    for (int r = 0; r < 32; ++r) v[r] = at[min(row0 + r, m - 1) * e.ldr];
   } else {
-    const float* at = static_cast<const float*>(e.res) + row0 * e.ldr + col0 + lane;
+    const uint32_t* at = static_cast<const uint32_t*>(e.res) + col;
 #pragma unroll
-    for (int r = 0; r < 32; ++r) v[r] = in && row0 + r < m ? at[r * e.ldr] : 0.0f;
+    for (int r = 0; r < 32; ++r) v[r] = at[min(row0 + r, m - 1) * e.ldr];
   }
 }
-__device__ __forceinline__ void epi_add_rows(const EpiParams& e, const float (&v)[32],
+__device__ __forceinline__ void epi_add_rows(const EpiParams& e, const uint32_t (&v)[32],
                                              float (&y)[32], float* turn) {
   if (!e.res) return;
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int r = 0; r < 32; ++r) turn[r * 32 + (lane ^ r)] = v[r];
+  for (int r = 0; r < 32; ++r)
+    turn[r * 32 + (lane ^ r)] = __uint_as_float(e.res_bf16 ? v[r] << 16 : v[r]);
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < 32; ++j) y[j] += turn[lane * 32 + (j ^ lane)];

@@ -316,17 +316,20 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
     // a time: all their remote loads and residuals are in flight at once.
     for (int i0 = rank * 2 + (threadIdx.x >> 7); i0 < Cfg::kPass && t0 + i0 < p.m;
          i0 += 2 * ranks * kTogether) {
-      float z[kTogether][Cfg::kSets], res[kTogether];
+      float z[kTogether][Cfg::kSets];
+      uint32_t res[kTogether];  // raw; beyond the matrix its last row or column's
+      if (e.res) {
+#pragma unroll
+        for (int u = 0; u < kTogether; ++u) {
+          const int64_t at = min(t0 + i0 + u * 2 * ranks, p.m - 1) * e.ldr + min(out_col, n_out - 1);
+          if (e.res_bf16) res[u] = static_cast<const uint16_t*>(e.res)[at];
+          else res[u] = static_cast<const uint32_t*>(e.res)[at];
+        }
+      }
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
         const int i = i0 + u * 2 * ranks;
         const bool on = i < Cfg::kPass && t0 + i < p.m;
-        res[u] = 0.0f;
-        if (on && e.res && in_z) {
-          const int64_t at = (t0 + i) * e.ldr + out_col;
-          res[u] = e.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.res)[at])
-                              : static_cast<const float*>(e.res)[at];
-        }
 #pragma unroll
         for (int s = 0; s < Cfg::kSets; ++s) {
           float v[kMaxRanks];
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
           else if (e.act == kActSilu) y = act_fwd<kActSilu>(y);
           else if (e.act == kActGelu) y = act_fwd<kActGelu>(y);
         }
-        if (e.res) y += res[u];
+        if (e.res) y += __uint_as_float(e.res_bf16 ? res[u] << 16 : res[u]);
         if (e.out_kind == kEpiMxfp8) {
           lane_store_mx(y, in_z, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout,
                         e.out_sf_blocks, row, out_col, n_out, lane);

@@ -1001,12 +1001,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         };
         auto out_col = [&](int c) { return (Roles::kGated ? n0 / 2 : n0) + tile_col(c); };
         constexpr int kRuns = Roles::kGated ? 2 : 4;
-        float next[32];
+        uint32_t next[32];
         epi_fetch_rows(e, next, row0, out_col(0), p.m, cols);
 #pragma unroll 1
         for (int c = 0; c < kRuns; ++c) {
           const int tcol = tile_col(c), c0 = out_col(c);
-          float res[32];
+          uint32_t res[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) res[j] = next[j];
           if (c + 1 < kRuns) epi_fetch_rows(e, next, row0, out_col(c + 1), p.m, cols);

@@ -3,9 +3,10 @@
     python -m cuda_optimazation_b200.build
 
 Compiles every .cu under csrc/ with nvcc for sm_100a only and links
-cuda_optimazation_b200/libqgemm_b200.so (C ABI: include/qgemm.h).  The
-library resolves cuTensorMapEncodeTiled through the CUDA runtime's driver
-entry point, so it needs no libcuda at link time.
+cuda_optimazation_b200/libqgemm_b200.so (C ABI: include/qgemm.h), the drop-in
+harness and the torch binding of the layer operators.  The library resolves
+cuTensorMapEncodeTiled through the CUDA runtime's driver entry point, so it
+needs no libcuda at link time.
 """
 from __future__ import annotations
 
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -47,7 +49,7 @@ def needs_build() -> bool:
         return True
     t = OUT.stat().st_mtime
     deps = list(CSRC.glob("*")) + [ROOT / "include" / "qgemm.h", Path(__file__), HARNESS_SRC]
-    if not HARNESS_BIN.exists():
+    if not HARNESS_BIN.exists() or not BINDING.exists():
         return True
     return any(d.stat().st_mtime > t for d in deps if d.is_file())
 
@@ -82,7 +84,33 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError("link failed")
     os.replace(tmp, OUT)
     build_harness()
+    build_binding()
     return OUT
+
+
+BINDING_SRC = CSRC / "torch_binding.cpp"
+BINDING = PKG / ("_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_binding() -> Path:
+    """The torch side of the layer operators (fused.py), a CPython module linked
+    against the library (rpath $ORIGIN); torch's own libraries are loaded with torch."""
+    import torch
+    from torch.utils import cpp_extension
+    includes = [f"-isystem{d}" for d in cpp_extension.include_paths("cuda")]
+    libs = Path(torch.__file__).parent / "lib"
+    tmp = BINDING.with_suffix(".tmp")
+    cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{sysconfig.get_paths()['include']}", *includes, str(BINDING_SRC), "-o", str(tmp),
+           f"-L{PKG}", "-lqgemm_b200", f"-L{libs}", "-ltorch_python", "-ltorch_cuda",
+           "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("binding build failed")
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 HARNESS_SRC = PKG / "harness" / "quant_gemm_bench.cpp"

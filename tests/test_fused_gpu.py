@@ -422,3 +422,35 @@ def test_offsets_past_32_bits(F):
     mt = a.dz_t.k
     assert torch.equal(a.dz.quantized.view(rows, k)[last:], tail.dz.quantized.view(-1, k))
     assert torch.equal(a.dz_t.quantized.view(k, mt)[:, last:], tail.dz_t.quantized.view(k, -1))
+
+
+# ------------------------------------------------------------------ refusals of the wrappers
+def test_wrapper_refusals(F, qlib):
+    x, w = rand(4, 256, seed=111), rand(256, seed=112)
+    z = qlib.make_mxfp8(x)
+    for bad in (lambda: F.rmsnorm_mxfp8(x.half(), w), lambda: F.rmsnorm_mxfp8(x, w, x.bfloat16()),
+                lambda: F.rmsnorm_backward(x.bfloat16(), x, w[:4], w),
+                lambda: F.rmsnorm_backward(x, x, w[:4].bfloat16(), w),
+                lambda: F.gemm_fused(z, z, bias=w[:4].half()), lambda: F.transpose_mxfp8(x),
+                lambda: F.act_backward(x, x, "relu"), lambda: F.act_backward(x.half(), z, "relu"),
+                lambda: F.rmsnorm_mxfp8("x", w)):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: F.rmsnorm_mxfp8(x, w[:255]), lambda: F.rmsnorm_mxfp8(x, w, x[:3]),
+                lambda: F.rmsnorm_mxfp8(x, w, x.cpu()), lambda: F.rmsnorm_mxfp8(x.t(), w[:4]),
+                lambda: F.rmsnorm_mxfp8(x[0], w), lambda: F.rmsnorm_backward(x, x, w, w),
+                lambda: F.gemm_fused(z, z, bias=w), lambda: F.gemm_fused(z, z, residual=x),
+                lambda: F.gemm_fused(z, z, out="fp16"), lambda: F.gemm_fused(z, z, out=x),
+                lambda: F.gemm_fused(z, qlib.make_mxfp4(x)), lambda: F.gemm_fused(x, x),
+                lambda: F.gemm_fused(z, qlib.make_mxfp8(x, 2)), lambda: F.gemm_fused(z, z, act="x"),
+                lambda: F.act_backward(x[:, :32], z, "relu"), lambda: F.act_backward(x, None, "relu"),
+                lambda: F.act_backward(x, qlib.make_mxfp8(x), "swiglu")):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: F.rmsnorm_mxfp8(x[:, :40], w[:40]), lambda: F.rmsnorm_mxfp8(x, w, eps=-1),
+                lambda: F.rmsnorm_mxfp8(x, w, layout=3), lambda: F.rmsnorm_mxfp8(x[:, 1:33], w[:32]),
+                lambda: F.gemm_fused(z, z, out="mxfp8"), lambda: F.gemm_fused(z, z, act="swiglu"),
+                lambda: F.transpose_mxfp8(z, 0), lambda: F.act_backward(x, z, "relu", layout=0),
+                lambda: F.act_backward(x[:0], None, "none")):
+        with pytest.raises(qlib.QGemmError):
+            bad()

@@ -32,6 +32,7 @@ namespace qg {
 
 namespace {
 
+constexpr int kPrefetch = 4;  // K blocks of weights prefetched into L2 before the wait
 constexpr int kTogether = 4;  // rows that a thread finishes at a time
 constexpr int kMaxRanks = 8;  // CTAs per cluster (the portable size)
 constexpr int kRowsFmtMxfp8 = 0, kRowsFmtNvfp4 = 1, kRowsFmtMxfp4 = 2;
@@ -150,6 +151,13 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
     mbar_init(acc_full, 1);
     *abort_flag = 0u;
     fence_barrier_init();
+    // While the stream's previous kernel ends: this CTA's first weights into L2
+    // (which stays coherent, should that kernel be writing them).
+    for (int kb = kb0; kb < kb1 && kb < kb0 + kPrefetch; ++kb) {
+      tma_prefetch_l2_2d(&p.tm_a, kb * 128, col0);
+      tma_prefetch_l2_3d(&p.tm_sfa, 0, col0 / 128, kb * Cfg::kChunks);
+    }
+    griddep_wait();
     // The first stages need no one's leave: on their way before the TMEM
     // allocation and the CTA's barrier.
     const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
@@ -159,6 +167,7 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish();
   }
+  griddep_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -186,6 +195,7 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
           phase ^= 1u;
         }
       }
+      griddep_launch_dependents();  // all loads are on their way
       if (!ok) {
         uint32_t dummy = 0;
         for (int s = 0; s < Cfg::kStages; ++s)
@@ -395,43 +405,44 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
   }
 }
 
-// CTAs per cluster: as many (a power of two, 8 at most) as find a place on the
-// SMs at once, with at least two K blocks each.
-int cluster_size(int tiles, int k_blocks, int slots) {
-  int c = 1;
-  while (c < kMaxRanks && tiles * 2 * c <= slots && k_blocks >= 4 * c) c *= 2;
-  return c;
-}
-
 template <int kFmt, int kN, bool kGated>
 cudaError_t launch_rows(const GemmParams& p, cudaStream_t stream) {
   using Cfg = RowsCfg<kFmt, kN, kGated>;
   auto kernel = gemm_fused_rows_kernel<kFmt, kN, kGated>;
-  static bool done[kMaxDevices] = {};
+  // Clusters of each size that find a place on the device at once.
+  static int places[kMaxDevices][kMaxRanks + 1] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
     return cudaErrorInvalidDevice;
-  if (!done[dev]) {
-    const cudaError_t err =
+  if (!places[dev][1]) {
+    cudaError_t err =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (err != cudaSuccess) return err;
-    done[dev] = true;
+    for (int c = kMaxRanks; c >= 2; --c) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(static_cast<unsigned>(c));
+      cfg.blockDim = dim3(256);
+      cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = static_cast<unsigned>(c);
+      attr.val.clusterDim.y = 1;
+      attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      err = cudaOccupancyMaxActiveClusters(&places[dev][c], kernel, &cfg);
+      if (err != cudaSuccess) return err;
+    }
+    places[dev][1] = num_sms() * Cfg::kPerSm;
   }
+  // As many CTAs to a cluster as let every tile's find its place at once, with at
+  // least two K blocks each (64 x 4736 x 14336: 37 clusters of 8 do not, and took
+  // 26.8 us in two rounds; one round of smaller ones takes 22.4).
   const int tiles = p.num_n_tiles;
-  const int c = cluster_size(tiles, p.num_k_blocks, num_sms() * Cfg::kPerSm);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * c);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(c);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  int c = kMaxRanks;
+  while (c > 1 && (tiles > places[dev][c] || p.num_k_blocks < 2 * c)) --c;
+  return launch_overlapped(kernel, dim3(static_cast<unsigned>(tiles) * c), dim3(256),
+                           Cfg::kSmemBytes, stream, c, p);
 }
 
 template <int kFmt, bool kGated>

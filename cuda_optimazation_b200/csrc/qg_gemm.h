@@ -7,6 +7,30 @@
 
 namespace qg {
 
+// Launch with programmatic stream serialization: the grid may start while the
+// stream's previous one is ending (its CTAs past griddep_launch_dependents), so
+// the kernel calls griddep_wait before it reads or writes global memory.
+// `cluster`: CTAs of a cluster along x.
+template <typename... P>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
+                              cudaStream_t stream, int cluster, P... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Devices a process may drive (per-device launch state is kept in arrays).
 constexpr int kMaxDevices = 64;
 

@@ -238,6 +238,8 @@ template <bool kBf16, bool kWBf16, int kVec>
 __global__ void __launch_bounds__(1024) rmsnorm_direct_kernel(const RmsNormParams p) {
   __shared__ float red[32];
   const int64_t row = blockIdx.x;
+  griddep_launch_dependents();
+  griddep_wait();
   if (row >= p.rows) {
     const int pads = static_cast<int>(gridDim.x - p.rows);
     pad_scales(p, static_cast<int>(row - p.rows) * blockDim.x + threadIdx.x, pads * blockDim.x);
@@ -437,6 +439,8 @@ template <bool kBf16, bool kWBf16, int kVec, bool kColumns>
 __global__ void __launch_bounds__(512, kColumns && kVec <= 2 ? 2 : 1)
     rmsnorm_backward_direct_kernel(const RmsNormBwdParams p) {
   __shared__ float red[32];
+  griddep_launch_dependents();
+  griddep_wait();
   if constexpr (kColumns) {
     if (blockIdx.x + p.rows < gridDim.x) {
       column_dw<kBf16>(p, static_cast<int64_t>(blockIdx.x) * (128 / kElem<kBf16>));
@@ -685,10 +689,10 @@ cudaError_t launch_norm(const RmsNormParams& p, cudaStream_t stream) {
   if (p.layout != 0 && p.rows % 128 != 0)
     pads = static_cast<int>((p.sf_blocks * 128 + 4 * s.threads - 1) / (4 * s.threads));
   const int grid = static_cast<int>(p.rows) + pads;
-  if (s.vec == 1) rmsnorm_direct_kernel<kBf16, kWBf16, 1><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 2) rmsnorm_direct_kernel<kBf16, kWBf16, 2><<<grid, s.threads, 0, stream>>>(p);
-  else rmsnorm_direct_kernel<kBf16, kWBf16, 4><<<grid, s.threads, 0, stream>>>(p);
-  return cudaGetLastError();
+  auto kernel = s.vec == 1   ? rmsnorm_direct_kernel<kBf16, kWBf16, 1>
+                : s.vec == 2 ? rmsnorm_direct_kernel<kBf16, kWBf16, 2>
+                             : rmsnorm_direct_kernel<kBf16, kWBf16, 4>;
+  return launch_overlapped(kernel, dim3(grid), dim3(s.threads), 0, stream, 1, p);
 }
 
 int backward_direct_grid(int64_t rows) {
@@ -703,15 +707,11 @@ template <bool kBf16, bool kWBf16, bool kColumns>
 cudaError_t launch_bwd_direct(const RmsNormBwdParams& p, int grid, cudaStream_t stream) {
   RowShape s = row_shape(p.k, 512);
   if (kColumns) s.threads = 512;
-  if (s.vec == 1)
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 1, kColumns><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 2)
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 2, kColumns><<<grid, s.threads, 0, stream>>>(p);
-  else if (s.vec == 4)
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4, kColumns><<<grid, s.threads, 0, stream>>>(p);
-  else
-    rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8, kColumns><<<grid, s.threads, 0, stream>>>(p);
-  return cudaGetLastError();
+  auto kernel = s.vec == 1   ? rmsnorm_backward_direct_kernel<kBf16, kWBf16, 1, kColumns>
+                : s.vec == 2 ? rmsnorm_backward_direct_kernel<kBf16, kWBf16, 2, kColumns>
+                : s.vec == 4 ? rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4, kColumns>
+                             : rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8, kColumns>;
+  return launch_overlapped(kernel, dim3(grid), dim3(s.threads), 0, stream, 1, p);
 }
 
 template <bool kBf16, bool kWBf16>
@@ -765,8 +765,8 @@ cudaError_t launch_rmsnorm_backward(const RmsNormBwdParams& p, bool bf16, bool w
 
 cudaError_t launch_column_sum(const float* part, int parts, int64_t k, float* out,
                               cudaStream_t stream) {
-  column_sum_kernel<<<static_cast<int>((k + 31) / 32), dim3(32, 32), 0, stream>>>(part, parts, k,
-                                                                                 out);
+  column_sum_kernel<<<static_cast<unsigned>((k + 31) / 32), dim3(32, 32), 0, stream>>>(part, parts,
+                                                                                     k, out);
   return cudaGetLastError();
 }
 

@@ -96,7 +96,7 @@ __device__ __forceinline__ void lane_store_mx(float v, bool in, uint8_t* q, uint
   if (lane == 0) {
     const int sc = col / 32;
     if (layout == 0) {
-      if (in) sf[row * (n / 32) + sc] = static_cast<uint8_t>(code);
+      if (in) sf[static_cast<int64_t>(row) * (n / 32) + sc] = static_cast<uint8_t>(code);
     } else if (sc < sf_blocks * 4) {  // rows fit one 128-row block: both MMA orders agree
       sf[mma_scale_offset(row, sc, 1, sf_blocks, layout)] = static_cast<uint8_t>(code);
     }

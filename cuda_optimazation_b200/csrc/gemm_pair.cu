@@ -136,7 +136,7 @@ __device__ __forceinline__ void spin_ns(uint64_t ns) {
 // bounds the pipeline.  Compiled out of shipped builds.
 constexpr bool kTracePair = (kDiag & 512u) != 0;
 __device__ __forceinline__ void trace_pair(const GemmParams& p, bool on, int kind, int slot) {
-  if (kTracePair && on && slot < 2048)
+  if (kTracePair && on && p.c && slot < 2048)
     reinterpret_cast<unsigned long long*>(p.c)[kind * 2048 + slot] = globaltimer_ns();
 }
 
@@ -248,7 +248,8 @@ struct PairRoles {
   // The warps (a whole warpgroup, where registers change hands) of the producer
   // and the issuers.
   __device__ static bool feeder(int warp) { return kWide ? warp < 4 : warp == 0 || mma(warp); }
-  __device__ static bool mma(int warp) { return warp == 1 || (!kWide && warp == 10); }
+  // (The second issuer's warp idles unless a build asks for two.)
+  __device__ static bool mma(int warp) { return warp == 1 || warp == (kWide ? 2 : 10); }
   __device__ static bool stager(int warp) {
     return kWide ? warp >= 4 && warp < 8 : warp >= 6 && warp <= 9;
   }
@@ -840,19 +841,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         // (one MX block) at a time.  MXFP8 values and bf16 rows that TMA can
         // store leave through the warp's 4 KB of shared memory: a lane's own
         // stores would touch a line each and hold up the stagers' loads.
-        static_assert(Cfg::kIssuers == 1 || kOut < 4, "one issuer: TMEM column = tile column");
         const int sub = Roles::second(warp);
         const int row0 = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32;
         uint8_t* boxes = epi_smem + (quad * 2 + sub) * 4096;
         float z[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          tmem_ld_32x32b_x32(t_row + ((c / 2) * 2 + sub) * 64 + (c & 1) * 32,
+          tmem_ld_32x32b_x32(t_row + tmem_block((c / 2) * 2 + sub) * 64 + (c & 1) * 32,
                              reinterpret_cast<uint32_t(&)[32]>(z[c]));
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader0);
+        if (lane == 0) {
+          mbar_arrive_cluster_relaxed(acc_empty_leader0);
+          if (Cfg::kIssuers == 2) mbar_arrive_cluster_relaxed(acc_empty_leader1);
+        }
         const EpiParams& e = p.epi;
         // z of 64-column block b of the warp starts at tile column:
         auto zcol = [&](int b) { return n0 + (2 * b + sub) * 64; };
@@ -968,7 +971,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
         // The same, 32 columns at a time in a loop; MXFP8 boxes of 32 columns (the
         // checkpoint's in the first 2 KB of the warp's memory, the output's
         // behind them), odd rows turned in all 4 KB.
-        static_assert(Cfg::kIssuers == 1 || kOut < 4, "one issuer: TMEM column = tile column");
         const int sub = Roles::second(warp);
         const int row0 = mt * 2 * Cfg::kBM + static_cast<int>(rank) * Cfg::kBM + quad * 32;
         uint8_t* boxes = epi_smem + (quad * 2 + sub) * 4096;
@@ -1012,14 +1014,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads<kOut>()
           if (c + 1 < kRuns) epi_fetch_rows(e, next, row0, out_col(c + 1), p.m, cols);
           float z[32], u[Roles::kGated ? 32 : 1];
           __syncwarp();
-          tmem_ld_32x32b_x32(t_row + tcol, reinterpret_cast<uint32_t(&)[32]>(z));
+          tmem_ld_32x32b_x32(t_row + tmem_block(tcol / 64) * 64 + tcol % 64,
+                             reinterpret_cast<uint32_t(&)[32]>(z));
           if constexpr (Roles::kGated)
-            tmem_ld_32x32b_x32(t_row + kGateCols + tcol, reinterpret_cast<uint32_t(&)[32]>(u));
+            tmem_ld_32x32b_x32(t_row + tmem_block(kGateCols / 64 + tcol / 64) * 64 + tcol % 64,
+                               reinterpret_cast<uint32_t(&)[32]>(u));
           tmem_wait_ld();
           if (c == kRuns - 1) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader0);
+            if (lane == 0) {
+              mbar_arrive_cluster_relaxed(acc_empty_leader0);
+              if (Cfg::kIssuers == 2) mbar_arrive_cluster_relaxed(acc_empty_leader1);
+            }
           }
           boxes_free();
           epi_affine(e, z, alpha, c == 0 ? bias[0] : c == 1 ? bias[1] : c == 2 ? bias[2] : bias[3]);

@@ -254,6 +254,20 @@ def test_gemm_long_k_and_residual_in_place(F, qlib):
     close(c, ref, tol)
 
 
+@pytest.mark.parametrize("m,n", [(300, 768), (260, 601)])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_gemm_over_its_residual(F, qlib, m, n, dt):
+    """Several tiles, rows on 16 bytes and odd ones, written over the residual."""
+    a, av = operand(qlib, m, 256, "mxfp8", 45)
+    b, bv = operand(qlib, n, 256, "mxfp8", 46, 0.06)
+    c = rand(m, n, seed=47, dtype=TYPES[dt])
+    ref = av @ bv.t() + c.to(F64)
+    tol = 2.0 ** -16 * (av.abs() @ bv.abs().t()) + 1.01 * STEP[c.dtype] * ref.abs()
+    tol = tol + 2.0 ** -22 * c.to(F64).abs()
+    assert F.gemm_fused(a, b, residual=c, out=c).out is c
+    close(c, ref, tol)
+
+
 def test_gemm_matches_plain_gemm(F, qlib):
     """Without an epilogue the product is the plain GEMM's."""
     for m in (300, 1024):

@@ -42,15 +42,6 @@ constexpr int kTile = 128;  // rows, and columns of a set, of a CTA
 
 // Staging: a thread copies its own pieces of a 32-row group into shared memory
 // (cp.async) two groups ahead of its work, and reads back only what it copied.
-template <int kBytes>
-__device__ __forceinline__ void stage_copy(uint8_t* to, const void* from) {
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from)
-                 : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from)
-                 : "memory");
-}
 __device__ __forceinline__ void stage_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -61,15 +52,15 @@ __device__ __forceinline__ void stage_wait() {
 
 // Eight gradients: 16 bytes of bf16, or two 16-byte pieces `second` apart.
 template <bool kBf16>
-__device__ __forceinline__ void read_grad8(const uint8_t* at, int second, float2 (&v)[4]) {
-  const uint4 a = lds128(at);
+__device__ __forceinline__ void read_grad8(uint32_t at, int second, float2 (&v)[4]) {
+  const uint4 a = lds128_at(at);
   if constexpr (kBf16) {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   } else {
-    const uint4 b = lds128(at + second);
+    const uint4 b = lds128_at(at + second);
     v[0] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
     v[1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
     v[2] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
@@ -78,8 +69,8 @@ __device__ __forceinline__ void read_grad8(const uint8_t* at, int second, float2
 }
 
 // Eight values of an MXFP8 row with scale s.
-__device__ __forceinline__ void read_mx8(const uint8_t* at, float s, float2 (&v)[4]) {
-  const uint2 w = *reinterpret_cast<const uint2*>(at);
+__device__ __forceinline__ void read_mx8(uint32_t at, float s, float2 (&v)[4]) {
+  const uint2 w = lds64_at(at);
   e4m3x4_decode(w.x, v[0], v[1]);
   e4m3x4_decode(w.y, v[2], v[3]);
 #pragma unroll
@@ -142,8 +133,9 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
   // Staged pieces: [row][gradient pieces, sets] of each thread, one slot per row
   // group where all are worked on at once, else two slots by turns.
   constexpr int kSlots = kGroups > 1 ? kGroups : 2;
-  uint8_t* stage_d = staged + (threadIdx.x & 127) * 16;
-  uint8_t* stage_z = staged + kSlots * 4 * kGradBytes * 128 + (threadIdx.x & 127) * 8;
+  const uint32_t stage_d = smem_u32(staged) + (threadIdx.x & 127) * 16;
+  const uint32_t stage_z =
+      smem_u32(staged) + kSlots * 4 * kGradBytes * 128 + (threadIdx.x & 127) * 8;
   const uint8_t* d_next = static_cast<const uint8_t*>(p.dout) +
                           ((m0 + group * 32 + rg * 4) * p.ldd + dc) * (kBf16 ? 2 : 4);
   const uint8_t* z_next = p.z_q + (m0 + group * 32 + rg * 4) * p.n + zc;
@@ -155,14 +147,14 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
       if (rb * 32 + rg * 4 + i < rows) {
         const int at = slot * 4 + i;
         if constexpr (kGrad) {
-          stage_copy<16>(stage_d + at * kGradBytes * 128, d_next + i * d_step);
+          copy_async_at<16>(stage_d + at * kGradBytes * 128, d_next + i * d_step);
           if constexpr (!kBf16)
-            stage_copy<16>(stage_d + (at * 2 + 1) * 2048, d_next + i * d_step + 16);
+            copy_async_at<16>(stage_d + (at * 2 + 1) * 2048, d_next + i * d_step + 16);
         }
         if constexpr (kZ) {
 #pragma unroll
           for (int s = 0; s < kSets; ++s)
-            stage_copy<8>(stage_z + (at * kSets + s) * 1024, z_next + i * p.n + s * kTile);
+            copy_async_at<8>(stage_z + (at * kSets + s) * 1024, z_next + i * p.n + s * kTile);
         }
       }
     }

@@ -112,20 +112,18 @@ template <bool kBf16>
 __device__ __forceinline__ const uint8_t* at_row(const void* base, int64_t row, int64_t ld) {
   return static_cast<const uint8_t*>(base) + row * ld * kElem<kBf16>;
 }
+// `slot`, `at`: 32-bit shared-memory addresses; `second`: bytes from a vector's first
+// chunk to its second.
 template <bool kBf16>
-__device__ __forceinline__ void ring_copy(uint8_t* slot, const uint8_t* row, int v, int nvec) {
+__device__ __forceinline__ void ring_copy(uint32_t at, const uint8_t* from, uint32_t second) {
 #pragma unroll
-  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                     smem_u32(slot + (i * nvec + v) * 16)),
-                 "l"(row + v * 8 * kElem<kBf16> + 16 * i)
-                 : "memory");
+  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) copy_async_at<16>(at + i * second, from + 16 * i);
 }
 template <bool kBf16>
-__device__ __forceinline__ Raw8<kBf16> ring_read(const uint8_t* slot, int v, int nvec) {
+__device__ __forceinline__ Raw8<kBf16> ring_read(uint32_t at, uint32_t second) {
   Raw8<kBf16> r;
 #pragma unroll
-  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) r.c[i] = lds128(slot + (i * nvec + v) * 16);
+  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) r.c[i] = lds128_at(at + i * second);
   return r;
 }
 __device__ __forceinline__ void ring_commit() {
@@ -281,21 +279,27 @@ __global__ void __launch_bounds__(512) rmsnorm_ring_kernel(const RmsNormParams p
   const int nvec = static_cast<int>(p.k / 8);
   const int row_bytes = static_cast<int>(p.k) * kElem<kBf16>;
   const int slot_bytes = p.residual ? 2 * row_bytes : row_bytes;
-  uint8_t* mine = ring + threadIdx.y * kStages * slot_bytes;
+  const bool add = p.residual != nullptr, keep = p.h != nullptr;
+  const uint32_t second = nvec * 16, hop = blockDim.x * 16;  // from vector to vector of a thread
+  const uint32_t mine = smem_u32(ring) + threadIdx.y * kStages * slot_bytes + threadIdx.x * 16;
+  const uint32_t end = mine + kStages * slot_bytes;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-  const uint8_t* x_next = at_row<kBf16>(p.x, first, p.ldx);
-  const uint8_t* r_next = at_row<kBf16>(p.residual, first, p.ldr);
+  const int mine_vecs =  // of this thread
+      (nvec - static_cast<int>(threadIdx.x) + static_cast<int>(blockDim.x) - 1) /
+      static_cast<int>(blockDim.x);
+  const uint32_t reach = blockDim.x * 8 * kElem<kBf16>;
+  const uint8_t* x_next = at_row<kBf16>(p.x, first, p.ldx) + threadIdx.x * 8 * kElem<kBf16>;
+  const uint8_t* r_next = at_row<kBf16>(p.residual, first, p.ldr) + threadIdx.x * 8 * kElem<kBf16>;
   const int64_t x_step = step * p.ldx * kElem<kBf16>, r_step = step * p.ldr * kElem<kBf16>;
   // Starts copying row `row`, and moves on by `step` rows.
-  auto fetch = [&](int64_t row, uint8_t* slot) {
+  auto fetch = [&](int64_t row, uint32_t slot) {
     if (row < p.rows) {
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec) {
-          ring_copy<kBf16>(slot, x_next, v, nvec);
-          if (p.residual) ring_copy<kBf16>(slot + row_bytes, r_next, v, nvec);
+        if (i < mine_vecs) {
+          ring_copy<kBf16>(slot + i * hop, x_next + i * reach, second);
+          if (add) ring_copy<kBf16>(slot + row_bytes + i * hop, r_next + i * reach, second);
         }
       }
     }
@@ -311,7 +315,8 @@ __global__ void __launch_bounds__(512) rmsnorm_ring_kernel(const RmsNormParams p
     const int v = threadIdx.x + i * blockDim.x;
     if (v < nvec) w[i] = load_kept<kWBf16>(p.weight, v * 8);
   }
-  uint8_t* slot = mine;
+  const float inv_k = 1.0f / static_cast<float>(p.k);
+  uint32_t slot = mine;
   uint8_t* q = p.q + first * p.k;
   uint8_t* h_out = static_cast<uint8_t*>(p.h) + first * p.ldh * kElem<kBf16>;
   for (int64_t row = first; row < p.rows; row += step) {
@@ -321,12 +326,11 @@ __global__ void __launch_bounds__(512) rmsnorm_ring_kernel(const RmsNormParams p
     float2 ss = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
       peak[i] = 0.0f;
-      if (v < nvec) {
-        Vec8 h = ring_read<kBf16>(slot, v, nvec).decode();
-        if (p.residual) add_to(h, ring_read<kBf16>(slot + row_bytes, v, nvec).decode());
-        if (p.h) store8<kBf16>(h_out, v * 8, h);
+      if (i < mine_vecs) {
+        Vec8 h = ring_read<kBf16>(slot + i * hop, second).decode();
+        if (add) add_to(h, ring_read<kBf16>(slot + row_bytes + i * hop, second).decode());
+        if (keep) store8<kBf16>(h_out, (threadIdx.x + i * blockDim.x) * 8, h);
         add_squares(ss, h);
         peak[i] = weighted(h, w[i].decode(), t[i]);
       }
@@ -334,15 +338,14 @@ __global__ void __launch_bounds__(512) rmsnorm_ring_kernel(const RmsNormParams p
     }
     fetch(row + kStages * step, slot);
     slot += slot_bytes;
-    if (slot == mine + kStages * slot_bytes) slot = mine;
-    const float rstd = rsqrtf(row_sum(ss.x + ss.y, red) / static_cast<float>(p.k) + p.eps);
+    if (slot == end) slot = mine;
+    const float rstd = rsqrtf(fmaf(row_sum(ss.x + ss.y, red), inv_k, p.eps));
     if (threadIdx.x == 0 && p.rstd) p.rstd[row] = rstd;
     const ScaleRow sr = scale_row(p, row);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      store_y(p, q, sr, v, v < nvec, t[i], peak[i], rstd, threadIdx.x & 31);
-    }
+    for (int i = 0; i < kVec; ++i)
+      store_y(p, q, sr, threadIdx.x + i * blockDim.x, i < mine_vecs, t[i], peak[i], rstd,
+              threadIdx.x & 31);
     q += step * p.k;
     h_out += step * p.ldh * kElem<kBf16>;
   }
@@ -503,23 +506,30 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNor
   const float inv_k = 1.0f / static_cast<float>(p.k);
   const int row_bytes = static_cast<int>(p.k) * kElem<kBf16>;
   const int slot_bytes = p.dres ? 3 * row_bytes : 2 * row_bytes;
-  uint8_t* mine = ring + threadIdx.y * kStages * slot_bytes;
+  const bool add = p.dres != nullptr;
+  const uint32_t second = nvec * 16, hop = blockDim.x * 16;
+  const uint32_t mine = smem_u32(ring) + threadIdx.y * kStages * slot_bytes + threadIdx.x * 16;
+  const uint32_t end = mine + kStages * slot_bytes;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-  const uint8_t* dy_next = at_row<kBf16>(p.dy, first, p.lddy);
-  const uint8_t* h_next = at_row<kBf16>(p.h, first, p.ldh);
-  const uint8_t* r_next = at_row<kBf16>(p.dres, first, p.lddres);
+  const int mine_vecs =
+      (nvec - static_cast<int>(threadIdx.x) + static_cast<int>(blockDim.x) - 1) /
+      static_cast<int>(blockDim.x);
+  const uint32_t reach = blockDim.x * 8 * kElem<kBf16>, lead = threadIdx.x * 8 * kElem<kBf16>;
+  const uint8_t* dy_next = at_row<kBf16>(p.dy, first, p.lddy) + lead;
+  const uint8_t* h_next = at_row<kBf16>(p.h, first, p.ldh) + lead;
+  const uint8_t* r_next = at_row<kBf16>(p.dres, first, p.lddres) + lead;
   const int64_t dy_step = step * p.lddy * kElem<kBf16>, h_step = step * p.ldh * kElem<kBf16>,
                 r_step = step * p.lddres * kElem<kBf16>;
-  auto fetch = [&](int64_t row, uint8_t* slot) {
+  auto fetch = [&](int64_t row, uint32_t slot) {
     if (row < p.rows) {
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec) {
-          ring_copy<kBf16>(slot, dy_next, v, nvec);
-          ring_copy<kBf16>(slot + row_bytes, h_next, v, nvec);
-          if (p.dres) ring_copy<kBf16>(slot + 2 * row_bytes, r_next, v, nvec);
+        if (i < mine_vecs) {
+          const uint32_t at = slot + i * hop;
+          ring_copy<kBf16>(at, dy_next + i * reach, second);
+          ring_copy<kBf16>(at + row_bytes, h_next + i * reach, second);
+          if (add) ring_copy<kBf16>(at + 2 * row_bytes, r_next + i * reach, second);
         }
       }
     }
@@ -539,7 +549,7 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNor
   }
 #pragma unroll
   for (int s = 0; s < kStages; ++s) fetch(first + s * step, mine + s * slot_bytes);
-  uint8_t* slot = mine;
+  uint32_t slot = mine;
   uint8_t* out = static_cast<uint8_t*>(p.dx) + first * p.lddx * kElem<kBf16>;
   for (int64_t row = first; row < p.rows; row += step) {
     const float rstd = __ldg(p.rstd + row);
@@ -547,27 +557,25 @@ __global__ void __launch_bounds__(512) rmsnorm_backward_ring_kernel(const RmsNor
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v < nvec)
-        dot += bwd_dot<kWBf16>(ring_read<kBf16>(slot, v, nvec).decode(),
-                               ring_read<kBf16>(slot + row_bytes, v, nvec).decode(),
+      if (i < mine_vecs)
+        dot += bwd_dot<kWBf16>(ring_read<kBf16>(slot + i * hop, second).decode(),
+                               ring_read<kBf16>(slot + row_bytes + i * hop, second).decode(),
                                w[i].decode(), rstd, dw[i]);
     }
     const float c = row_sum(dot, red) * inv_k;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v < nvec) {
-        Vec8 d = bwd_dx(ring_read<kBf16>(slot, v, nvec).decode(),
-                        ring_read<kBf16>(slot + row_bytes, v, nvec).decode(), w[i].decode(), rstd,
-                        c);
-        if (p.dres) add_to(d, ring_read<kBf16>(slot + 2 * row_bytes, v, nvec).decode());
-        store8<kBf16>(out, v * 8, d);
+      if (i < mine_vecs) {
+        const uint32_t at = slot + i * hop;
+        Vec8 d = bwd_dx(ring_read<kBf16>(at, second).decode(),
+                        ring_read<kBf16>(at + row_bytes, second).decode(), w[i].decode(), rstd, c);
+        if (add) add_to(d, ring_read<kBf16>(at + 2 * row_bytes, second).decode());
+        store8<kBf16>(out, (threadIdx.x + i * blockDim.x) * 8, d);
       }
     }
     fetch(row + kStages * step, slot);
     slot += slot_bytes;
-    if (slot == mine + kStages * slot_bytes) slot = mine;
+    if (slot == end) slot = mine;
     out += step * p.lddx * kElem<kBf16>;
   }
   ring_wait<0>();

@@ -86,6 +86,9 @@ __device__ __forceinline__ Raw8<kBf16> load_kept(const void* base, int64_t elem)
   return r;
 }
 
+// Streaming stores, as for the values below: left to L2's own order the forward pass
+// over 16384 x 8192 took 168 us at full clocks and 157 under the power cap, streamed
+// 152 and 161.
 template <bool kBf16>
 __device__ __forceinline__ void store8(void* base, int64_t elem, const Vec8& x) {
   uint4* p = reinterpret_cast<uint4*>(static_cast<uint8_t*>(base) + elem * kElem<kBf16>);
@@ -96,7 +99,7 @@ __device__ __forceinline__ void store8(void* base, int64_t elem, const Vec8& x) 
       const __nv_bfloat162 b = __floats2bfloat162_rn(x.v[i].x, x.v[i].y);
       w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    *p = make_uint4(w[0], w[1], w[2], w[3]);
+    __stcs(p, make_uint4(w[0], w[1], w[2], w[3]));
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -200,8 +203,9 @@ __device__ __forceinline__ void store_y(const RmsNormParams& p, uint8_t* q, cons
     float2 y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(t.v[i], both(rstd)), both(mul));
-    *reinterpret_cast<uint2*>(q + v * 8) = make_uint2(
-        cvt_e4m3x4(y[0].x, y[0].y, y[1].x, y[1].y), cvt_e4m3x4(y[2].x, y[2].y, y[3].x, y[3].y));
+    __stcs(reinterpret_cast<uint2*>(q + v * 8),
+           make_uint2(cvt_e4m3x4(y[0].x, y[0].y, y[1].x, y[1].y),
+                      cvt_e4m3x4(y[2].x, y[2].y, y[3].x, y[3].y)));
   }
   if (p.layout == 0) {
     if (in && (lane & 3) == 0) sr.at[v / 4] = static_cast<uint8_t>(code);

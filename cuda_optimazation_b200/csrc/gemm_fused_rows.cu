@@ -13,8 +13,8 @@
 // Scales reach TMEM by tcgen05.cp: its fixed cost per 512-byte chunk, which the
 // large-m kernel avoids, hides behind the weight stream here.
 //
-// The epilogue runs across lanes (lane = column): 32 columns of a row, one MX
-// block, are one warp's, so a block's peak is one warp reduction.
+// The epilogue runs across lanes (four columns each): a warp has a row of the
+// tile, eight lanes an MX block of it.
 //
 // Roles (8 warps): warp 0 TMA producer, warp 1 MMA issuer (and TMEM owner),
 // warps 2..5 read the accumulator (one TMEM lane quadrant each); all eight finish
@@ -33,7 +33,6 @@ namespace qg {
 namespace {
 
 constexpr int kPrefetch = 4;  // K blocks of weights prefetched into L2 before the wait
-constexpr int kTogether = 4;  // rows that a thread finishes at a time
 constexpr int kMaxRanks = 8;  // CTAs per cluster (the portable size)
 constexpr int kRowsFmtMxfp8 = 0, kRowsFmtNvfp4 = 1, kRowsFmtMxfp4 = 2;
 
@@ -83,17 +82,20 @@ __device__ __forceinline__ uint32_t cluster_nctas() {
   return r;
 }
 
-// One value per lane: the lane's byte of an MXFP8 row and, from lane 0, the scale
-// of the warp's block.  `in`: the block lies in the matrix.
-__device__ __forceinline__ void lane_store_mx(float v, bool in, uint8_t* q, uint8_t* sf,
+// Four consecutive columns a lane: their bytes of an MXFP8 row and, from every
+// eighth lane, the scale of its 32-column block.  `in`: the block lies in the matrix.
+__device__ __forceinline__ void lane_store_mx(const float (&v)[4], bool in, uint8_t* q, uint8_t* sf,
                                               int layout, int sf_blocks, int row, int col, int n,
                                               int lane) {
-  const uint32_t bits = v == v ? __float_as_uint(fabsf(v)) : 0u;  // NaN has no part in the peak
+  float peak = in ? max3_abs(max3_abs(v[0], v[1], v[2]), v[3], 0.0f) : 0.0f;
+#pragma unroll
+  for (int o = 1; o <= 4; o *= 2) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
   float mul;
-  uint32_t code = mxfp8_scale_code(
-      __uint_as_float(__reduce_max_sync(0xffffffffu, in ? bits : 0u)), mul);
-  if (in) q[static_cast<int64_t>(row) * n + col] = static_cast<uint8_t>(cvt_e4m3x2(v * mul, 0.0f));
-  if (lane == 0) {
+  const uint32_t code = mxfp8_scale_code(peak, mul);
+  if (in)
+    *reinterpret_cast<uint32_t*>(q + static_cast<int64_t>(row) * n + col) =
+        cvt_e4m3x4(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul);
+  if ((lane & 7) == 0) {
     const int sc = col / 32;
     if (layout == 0) {
       if (in) sf[static_cast<int64_t>(row) * (n / 32) + sc] = static_cast<uint8_t>(code);
@@ -281,15 +283,16 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
   if (p.a_ts) alpha *= *p.a_ts;
   if (p.b_ts) alpha *= *p.b_ts;
   const EpiParams& e = p.epi;
-  const int f = threadIdx.x & 127;
+  // In the last step a warp finishes a row at a time, four columns a lane.
+  const int f = lane * 4;
   const int n_out = kGated ? p.n / 2 : p.n;
   const int out_col = (kGated ? tile * 128 : col0) + f;
   const bool in_z = col0 + f < p.n;  // gated: n is a multiple of 256, so both sets are in
-  float bias[Cfg::kSets];
+  float bias[Cfg::kSets][4];
 #pragma unroll
-  for (int s = 0; s < Cfg::kSets; ++s) {
-    bias[s] = epi_bias(e, col0 + s * 128 + f, p.n);
-  }
+  for (int s = 0; s < Cfg::kSets; ++s)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[s][j] = epi_bias(e, col0 + s * 128 + f + j, p.n);
   float* part = reinterpret_cast<float*>(smem);  // [set][row of the pass][128]
   const uint32_t part_addr = smem_u32(part);
   bool ok = true;
@@ -322,71 +325,118 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
     }
     __syncwarp();
     cluster_sync();  // every CTA's partial sums are in place
-    // A CTA half finishes every (2 ranks)-th row of the pass, kTogether rows at
-    // a time: all their remote loads and residuals are in flight at once.
-    for (int i0 = rank * 2 + (threadIdx.x >> 7); i0 < Cfg::kPass && t0 + i0 < p.m;
-         i0 += 2 * ranks * kTogether) {
-      float z[kTogether][Cfg::kSets];
-      uint32_t res[kTogether];  // raw; beyond the matrix its last row or column's
+    // A warp finishes every (8 ranks)-th row of the pass, kTogether rows at a
+    // time: all their remote loads and residuals are in flight at once.
+    constexpr int kTogether = kGated ? 1 : 2;
+    for (int i0 = rank * 8 + warp; i0 < Cfg::kPass && t0 + i0 < p.m;
+         i0 += 8 * ranks * kTogether) {
+      float z[kTogether][Cfg::kSets][4];
+      uint32_t res[kTogether][4];  // raw; beyond the matrix its last row or columns
       if (e.res) {
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
-          const int64_t at = min(t0 + i0 + u * 2 * ranks, p.m - 1) * e.ldr + min(out_col, n_out - 1);
-          if (e.res_bf16) res[u] = static_cast<const uint16_t*>(e.res)[at];
-          else res[u] = static_cast<const uint32_t*>(e.res)[at];
+          const int64_t at = min(t0 + i0 + u * 8 * ranks, p.m - 1) * e.ldr;
+          if (e.res_vec && n_out % 4 == 0) {
+            const int64_t c = at + min(out_col, n_out - 4);
+            if (e.res_bf16) {
+              const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(e.res) + c);
+              res[u][0] = r.x << 16; res[u][1] = r.x & 0xffff0000u;
+              res[u][2] = r.y << 16; res[u][3] = r.y & 0xffff0000u;
+            } else {
+              const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(e.res) + c);
+              res[u][0] = r.x; res[u][1] = r.y; res[u][2] = r.z; res[u][3] = r.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int64_t c = at + min(out_col + j, n_out - 1);
+              if (e.res_bf16) res[u][j] = static_cast<uint32_t>(static_cast<const uint16_t*>(e.res)[c]) << 16;
+              else res[u][j] = static_cast<const uint32_t*>(e.res)[c];
+            }
+          }
         }
       }
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
-        const int i = i0 + u * 2 * ranks;
+        const int i = i0 + u * 8 * ranks;
         const bool on = i < Cfg::kPass && t0 + i < p.m;
 #pragma unroll
         for (int s = 0; s < Cfg::kSets; ++s) {
-          float v[kMaxRanks];
+          float4 v[kMaxRanks];
           const uint32_t at = part_addr + ((s * Cfg::kPass + (on ? i : 0)) * 128 + f) * 4;
 #pragma unroll
           for (int r = 0; r < kMaxRanks; ++r)
-            v[r] = r < ranks ? ld_cluster_f32(mapa_shared(at, static_cast<uint32_t>(r))) : 0.0f;
-          z[u][s] = v[0];
+            v[r] = r < ranks ? ld_cluster_f32x4(mapa_shared(at, static_cast<uint32_t>(r)))
+                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-          for (int r = 1; r < kMaxRanks; ++r) z[u][s] += v[r];
+          for (int r = 1; r < kMaxRanks; ++r) {
+            v[0].x += v[r].x;
+            v[0].y += v[r].y;
+            v[0].z += v[r].z;
+            v[0].w += v[r].w;
+          }
+          z[u][s][0] = v[0].x; z[u][s][1] = v[0].y; z[u][s][2] = v[0].z; z[u][s][3] = v[0].w;
         }
       }
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
-        const int i = i0 + u * 2 * ranks;
+        const int i = i0 + u * 8 * ranks;
         if (i >= Cfg::kPass || t0 + i >= p.m) break;
         const int row = t0 + i;
 #pragma unroll
         for (int s = 0; s < Cfg::kSets; ++s) {
-          z[u][s] = z[u][s] * alpha + bias[s];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[u][s][j] = z[u][s][j] * alpha + bias[s][j];
           if (e.z_q)
             lane_store_mx(z[u][s], in_z, e.z_q, e.z_sf, e.z_layout, e.z_sf_blocks, row,
                           col0 + s * 128 + f, p.n, lane);
         }
-        float y;
-        if constexpr (kGated) {
-          y = act_fwd<kActSilu>(z[u][0]) * z[u][1];
-        } else {
-          y = z[u][0];
-          if (e.act == kActRelu) y = act_fwd<kActRelu>(y);
-          else if (e.act == kActSilu) y = act_fwd<kActSilu>(y);
-          else if (e.act == kActGelu) y = act_fwd<kActGelu>(y);
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kGated) {
+            y[j] = act_fwd<kActSilu>(z[u][0][j]) * z[u][1][j];
+          } else {
+            y[j] = z[u][0][j];
+            if (e.act == kActRelu) y[j] = act_fwd<kActRelu>(y[j]);
+            else if (e.act == kActSilu) y[j] = act_fwd<kActSilu>(y[j]);
+            else if (e.act == kActGelu) y[j] = act_fwd<kActGelu>(y[j]);
+          }
+          if (e.res) y[j] += __uint_as_float(res[u][j]);
         }
-        if (e.res) y += __uint_as_float(e.res_bf16 ? res[u] << 16 : res[u]);
         if (e.out_kind == kEpiMxfp8) {
           lane_store_mx(y, in_z, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout,
                         e.out_sf_blocks, row, out_col, n_out, lane);
-        } else if (in_z) {
+        } else {
           const int64_t at = row * e.ldc + out_col;
-          if (e.out_kind == kEpiBf16)
-            static_cast<__nv_bfloat16*>(e.out)[at] = __float2bfloat16_rn(y);
-          else
-            static_cast<float*>(e.out)[at] = y;
+          const bool whole = e.out_vec && out_col + 4 <= n_out;
+          if (e.out_kind == kEpiBf16) {
+            __nv_bfloat16* c = static_cast<__nv_bfloat16*>(e.out) + at;
+            if (whole) {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]);
+              const __nv_bfloat162 hi = __floats2bfloat162_rn(y[2], y[3]);
+              *reinterpret_cast<uint2*>(c) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo),
+                             *reinterpret_cast<const uint32_t*>(&hi));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (out_col + j < n_out) c[j] = __float2bfloat16_rn(y[j]);
+            }
+          } else {
+            float* c = static_cast<float*>(e.out) + at;
+            if (whole) {
+              *reinterpret_cast<float4*>(c) = make_float4(y[0], y[1], y[2], y[3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (out_col + j < n_out) c[j] = y[j];
+            }
+          }
         }
       }
     }
-    cluster_sync();  // the sums have been read: reuse the buffer, or exit
+    cluster_sync_relaxed();  // the sums have been read: reuse the buffer, or exit
   }
   if (rank == 0) {
     if (e.out_kind == kEpiMxfp8)
@@ -417,6 +467,9 @@ cudaError_t launch_rows(const GemmParams& p, cudaStream_t stream) {
   if (!places[dev][1]) {
     cudaError_t err =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (err != cudaSuccess) return err;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
     if (err != cudaSuccess) return err;
     for (int c = kMaxRanks; c >= 2; --c) {
       cudaLaunchConfig_t cfg{};

@@ -486,14 +486,23 @@ cudaError_t launch_rows(const GemmParams& p, cudaStream_t stream) {
       err = cudaOccupancyMaxActiveClusters(&places[dev][c], kernel, &cfg);
       if (err != cudaSuccess) return err;
     }
-    places[dev][1] = num_sms() * Cfg::kPerSm;
+    places[dev][1] = num_sms();
   }
   // As many CTAs to a cluster as let every tile's find its place at once, with at
-  // least two K blocks each (64 x 4736 x 14336: 37 clusters of 8 do not, and took
-  // 26.8 us in two rounds; one round of smaller ones takes 22.4).
+  // least two K blocks each: one CTA an SM (which is what the runtime counts of
+  // CTAs that use TMEM), or, where that leaves each more than kN / 2 blocks, two.  The
+  // exchange costs every CTA kN x 512 bytes of remote reads: 64 x 4096 x 2048 takes
+  // 6.8 us with 128 CTAs and 9.2 with 192, x 28672 27.1 and 26.5; one token, 2 x 14336
+  // x 4096 gated, 23.8 with 112 and 21.2 with 224.  (A second round costs more than
+  // either: 64 x 4736 x 14336 in 37 clusters of 8 26.8 us, of 6 17.8.)
   const int tiles = p.num_n_tiles;
-  int c = kMaxRanks;
-  while (c > 1 && (tiles > places[dev][c] || p.num_k_blocks < 2 * c)) --c;
+  auto most = [&](int per_sm) {
+    int c = kMaxRanks;
+    while (c > 1 && (tiles > per_sm * places[dev][c] || p.num_k_blocks < 2 * c)) --c;
+    return c;
+  };
+  int c = most(1);
+  if (Cfg::kPerSm == 2 && p.num_k_blocks > c * kN / 2) c = most(2);
   return launch_overlapped(kernel, dim3(static_cast<unsigned>(tiles) * c), dim3(256),
                            Cfg::kSmemBytes, stream, c, p);
 }

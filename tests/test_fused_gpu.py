@@ -413,6 +413,39 @@ def test_transpose(F, qlib, rows, k, layout):
     assert torch.equal(t.block_scales, sf)
 
 
+@pytest.mark.parametrize("low,high", [(127, 127), (120, 125), (100, 112), (100, 113), (60, 200),
+                                      (0, 3), (0, 12), (0, 40), (20, 32), (234, 246)])
+@pytest.mark.parametrize("rows,k", [(70, 96), (128, 4128), (40000, 128)])
+@pytest.mark.parametrize("kind", ["any", "small", "sparse"])
+def test_transpose_scales(F, qlib, low, high, rows, k, kind):
+    """Scales of a block that lie near and far from each other, at both ends of
+    their range; zeros, columns far below the block's peak, NaN (which a peak
+    does not see).  Exact as above."""
+    g = torch.Generator(device=DEV).manual_seed(low * 1000 + high + rows)
+    q = torch.randint(0, 256, (rows, k), generator=g, device=DEV, dtype=torch.uint8)
+    if kind != "any":
+        q[q & 0x7f == 0x7f] = 0
+    if kind == "small":  # of many columns only the lowest subnormals
+        cols = torch.randint(0, 3, (k,), generator=g, device=DEV) > 0
+        q = torch.where(cols, q & 0x83, q)
+    if kind == "sparse":
+        q[torch.rand(rows, k, generator=g, device=DEV) < 0.97] = 0
+        q[::3] = 0
+    e = torch.randint(low, high + 1, (rows, k // 32), generator=g, device=DEV)
+    a = qlib.make_mxfp8(torch.zeros(rows, k, device=DEV), 0)
+    a.quantized.copy_(q.view_as(a.quantized))
+    a.block_scales.copy_(e.to(torch.uint8).view_as(a.block_scales))
+    t = F.transpose_mxfp8(a, 1)
+    rt = (rows + 31) // 32 * 32
+    v = torch.cat([R.value(a).t(), torch.zeros(k, rt - rows, dtype=F64, device=DEV)], 1)
+    bad = v.isnan()
+    want, sf = R.quantise(torch.where(bad, torch.zeros_like(v), v), 1)
+    assert torch.equal(t.block_scales, sf)
+    got = t.quantized.view(k, rt)
+    assert bool((got[bad] & 0x7f == 0x7f).all())
+    assert torch.equal(got[~bad], want[~bad])
+
+
 # ------------------------------------------------------------------ long buffers
 def test_offsets_past_32_bits(F):
     """More than 2^31 elements: the last rows are those of a short call."""

@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
     act_backward_kernel(const ActBackwardParams p) {
   constexpr int kSets = kAct == kActSwiglu ? 2 : 1;
   constexpr bool kGrad = kAct >= 0, kZ = kAct != kActNone;
+  constexpr bool kLines = !kGrad && kGroups == 1;  // a warp's blocks lie side by side
   constexpr int kGradBytes = kGrad ? (kBf16 ? 16 : 32) : 0;
   extern __shared__ __align__(16) uint8_t staged[];
   __shared__ uint4 row_sf[kSets][32], col_sf[kSets][32];  // 512-byte chunks
@@ -125,9 +126,11 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
   const int64_t m0 = static_cast<int64_t>(tm) * kTile;
   const int rows = static_cast<int>(p.m - m0 < kTile ? p.m - m0 : kTile);
   // This lane's first column of z (of the gate set) and of dout.
-  const int64_t zc = static_cast<int64_t>(tc) * kSets * kTile + warp * 32 + cg * 8;
+  const int64_t zc =
+      static_cast<int64_t>(tc) * kSets * kTile + (kLines ? 0 : warp * 32) + cg * 8;
   const int64_t dc = static_cast<int64_t>(tc) * kTile + warp * 32 + cg * 8;
-  const bool active = zc < p.n;  // p.n is a multiple of 32: a warp is in or out as a whole
+  // p.n is a multiple of 32: a warp is in or out as a whole.
+  const bool active = kLines ? warp * 32 < rows : zc < p.n;
   const int64_t row_blocks = (p.m + 127) / 128, n_blocks = (p.n + 127) / 128;
   const int64_t sf_blocks = (p.n / 32 + 3) / 4, t_blocks = (p.mt / 32 + 3) / 4;
   // Staged pieces: [row][gradient pieces, sets] of each thread, one slot per row
@@ -136,6 +139,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
   const uint32_t stage_d = smem_u32(staged) + (threadIdx.x & 127) * 16;
   const uint32_t stage_z =
       smem_u32(staged) + kSlots * 4 * kGradBytes * 128 + (threadIdx.x & 127) * 8;
+  const uint32_t stage_line = smem_u32(staged) + (warp * 32 + rg * 4) * 128 + cg * 8;
   const uint8_t* d_next = static_cast<const uint8_t*>(p.dout) +
                           ((m0 + group * 32 + rg * 4) * p.ldd + dc) * (kBf16 ? 2 : 4);
   const uint8_t* z_next = p.z_q + (m0 + group * 32 + rg * 4) * p.n + zc;
@@ -181,7 +185,23 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
                      << (8 * c);
     }
   }
-  if (active) {
+  if constexpr (kLines) {
+    // All 32 rows of the warp, in whole lines: piece c of row 4 a + b at place
+    // c ^ 2 (a % 4), so that the 4 x 32 bytes that half a warp reads of rows 4 apart
+    // lie in all banks.
+    const int piece = lane & 7, row = warp * 32 + (lane >> 3);
+    const uint8_t* from = p.z_q + (m0 + row) * p.n + tc * kTile + piece * 16;
+    if (static_cast<int64_t>(tc) * kTile + piece * 16 < p.n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (row + i * 4 < rows)
+          copy_async_at<16>(smem_u32(staged) + (row + i * 4) * 128 + (piece ^ 2 * (i & 3)) * 16,
+                            from);
+        from += 4 * p.n;
+      }
+    }
+    stage_commit();
+  } else if (active) {
     fetch(group);
     if constexpr (kGroups == 1) fetch(1);
   }
@@ -205,18 +225,24 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
     for (int j = 0; j < 4; ++j) sum[s][j] = make_float2(0.0f, 0.0f);
   if (active) {
     uint8_t* row_out = p.dz_q + (m0 + group * 32 + rg * 4) * p.n + zc;
-    uint8_t* col_out = p.dzt_q + zc * p.mt + m0 + group * 32 + rg * 4;
+    uint8_t* col_out = p.dzt_q + zc * p.mt + m0 + (kLines ? warp : group) * 32 + rg * 4;
+    if constexpr (kLines) {
+      stage_wait<0>();
+      __syncwarp();
+    }
+    const int64_t end = kLines ? p.n - static_cast<int64_t>(tc) * kTile : rows;
 #pragma unroll 1
-    for (int rb = group; rb * 32 < rows; rb += kGroups) {
+    for (int it = group; it * 32 < end && (!kLines || it < 4); it += kGroups) {
+      const int rb = kLines ? warp : it, cb = kLines ? it : warp;  // block row and column
       const int r0 = rb * 32 + rg * 4;  // this lane's first row of the tile
       const int slot = kGroups > 1 ? rb : rb & 1;
-      stage_wait<(kGroups > 1 ? 0 : 1)>();
+      if constexpr (!kLines) stage_wait<(kGroups > 1 ? 0 : 1)>();
       float2 v[kSets][4][4];
       float zs[kSets][4];
       if constexpr (kZ) {
 #pragma unroll
         for (int s = 0; s < kSets; ++s) {
-          const float4 f = z_scale[s][rb][warp][rg];
+          const float4 f = z_scale[s][rb][cb][rg];
           zs[s][0] = f.x; zs[s][1] = f.y; zs[s][2] = f.z; zs[s][3] = f.w;
         }
       }
@@ -230,7 +256,9 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
           if constexpr (kZ) {
 #pragma unroll
             for (int s = 0; s < kSets; ++s)
-              read_mx8(stage_z + (at * kSets + s) * 1024, zs[s][i], v[s][i]);
+              read_mx8(kLines ? stage_line + i * 128 + (cb * 32 ^ (rg & 3) * 32)
+                              : stage_z + (at * kSets + s) * 1024,
+                       zs[s][i], v[s][i]);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -249,7 +277,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
             for (int j = 0; j < 4; ++j) v[s][i][j] = make_float2(0.0f, 0.0f);
         }
       }
-      if constexpr (kGroups == 1) fetch(rb + 2);  // the slot has been read
+      if constexpr (kGroups == 1 && !kLines) fetch(rb + 2);  // the slot has been read
 #pragma unroll
       for (int s = 0; s < kSets; ++s) {
         float2 (&x)[4][4] = v[s];
@@ -285,7 +313,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
             }
             if (cg == 0) {
               uint8_t* to = reinterpret_cast<uint8_t*>(row_sf[s]) + (rg * 4 + 2 * h) * 16 +
-                            rb * 4 + warp;
+                            rb * 4 + cb;
               to[0] = static_cast<uint8_t>(c >> 7);
               to[16] = static_cast<uint8_t>(c >> 23);
             }
@@ -315,7 +343,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
         const uint32_t c = codes_x128(t[0]), r = reciprocals(c);
         if ((lane & 4) == 0) {
           uint8_t* to = reinterpret_cast<uint8_t*>(col_sf[s]) +
-                        (cg * 8 + (lane >> 3) * 2) * 16 + warp * 4 + rb;
+                        (cg * 8 + (lane >> 3) * 2) * 16 + cb * 4 + rb;
           to[0] = static_cast<uint8_t>(c >> 7);
           to[16] = static_cast<uint8_t>(c >> 23);
         }
@@ -335,7 +363,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
         }
       }
       row_out += 32 * p.n;
-      col_out += 32;
+      col_out += kLines ? 32 * p.mt : 32;
     }
     if constexpr (kGrad) {
       if (p.dbias_part) {
@@ -407,7 +435,8 @@ constexpr int kClusterRows = 8;
 
 template <int kAct, bool kBf16, int kGroups>
 cudaError_t launch_one(const ActBackwardParams& p, int grid, cudaStream_t stream) {
-  constexpr int kSmem = staged_bytes<kAct, kBf16>() * (kGroups > 1 ? kGroups : 2) * 128;
+  constexpr int kSmem = kAct < 0 ? kTile * kTile
+                                 : staged_bytes<kAct, kBf16>() * (kGroups > 1 ? kGroups : 2) * 128;
   auto kernel = act_backward_kernel<kAct, kBf16, kGroups>;
   static bool done[kMaxDevices] = {};
   int dev = 0;

@@ -40,8 +40,8 @@ namespace {
 
 constexpr int kTile = 128;  // rows, and columns of a set, of a CTA
 
-// Staging: a thread copies its own pieces of a 32-row group into shared memory
-// (cp.async) two groups ahead of its work, and reads back only what it copied.
+// Staging (cp.async).  Few tiles: a thread copies its own pieces of a 32-row group
+// and reads back only what it copied.
 __device__ __forceinline__ void stage_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -109,7 +109,10 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
     act_backward_kernel(const ActBackwardParams p) {
   constexpr int kSets = kAct == kActSwiglu ? 2 : 1;
   constexpr bool kGrad = kAct >= 0, kZ = kAct != kActNone;
-  constexpr bool kLines = !kGrad && kGroups == 1;  // a warp's blocks lie side by side
+  // Many tiles: rows are staged in whole lines (32-byte pieces of eight rows cost the
+  // L1 four times as much), of the transposition 32 rows by each warp, whose blocks
+  // then lie side by side, else 32 rows by the CTA at a time.
+  constexpr bool kLines = !kGrad && kGroups == 1, kShared = kGrad && kGroups == 1;
   constexpr int kGradBytes = kGrad ? (kBf16 ? 16 : 32) : 0;
   extern __shared__ __align__(16) uint8_t staged[];
   __shared__ uint4 row_sf[kSets][32], col_sf[kSets][32];  // 512-byte chunks
@@ -140,6 +143,17 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
   const uint32_t stage_z =
       smem_u32(staged) + kSlots * 4 * kGradBytes * 128 + (threadIdx.x & 127) * 8;
   const uint32_t stage_line = smem_u32(staged) + (warp * 32 + rg * 4) * 128 + cg * 8;
+  // Whole lines, of 32 rows: the gradient's, then each set of z.  Row 4 a + b's
+  // 16-byte piece c lies at place c ^ x(a), so that what a part of a warp reads at
+  // once (8 bytes of 4 rows, or 16 of 2, 4 apart) lies in all banks.
+  constexpr int kGradRow = kBf16 ? 256 : 512, kGradPieces = kGradRow / 16;
+  constexpr int kSlotBytes = 32 * ((kGrad ? kGradRow : 0) + (kZ ? kSets * 128 : 0));
+  const uint32_t line_d =
+      smem_u32(staged) + rg * 4 * kGradRow +
+      (kBf16 ? (warp * 4 + cg) ^ 4 * (rg & 1) : (warp * 8 + cg * 2) ^ (rg & 1)) * 16;
+  const uint32_t line_z = smem_u32(staged) + 32 * kGradRow + rg * 4 * 128 +
+                          ((warp * 2 + (cg >> 1)) ^ 2 * (rg & 3)) * 16 + (cg & 1) * 8;
+  const int d_second = kShared ? (rg & 1 ? -16 : 16) : 2048;
   const uint8_t* d_next = static_cast<const uint8_t*>(p.dout) +
                           ((m0 + group * 32 + rg * 4) * p.ldd + dc) * (kBf16 ? 2 : 4);
   const uint8_t* z_next = p.z_q + (m0 + group * 32 + rg * 4) * p.n + zc;
@@ -166,6 +180,44 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
     z_next += 32 * p.n;
     stage_commit();
   };
+  auto fetch_lines = [&](int rb) {
+    const uint32_t to = smem_u32(staged) + (rb & 1) * kSlotBytes;
+    const int t = threadIdx.x;
+    {
+      constexpr int kRows = 128 / kGradPieces;  // of a pass
+      const int piece = t % kGradPieces, row = t / kGradPieces;
+      const int64_t col = static_cast<int64_t>(tc) * kTile + piece * (kBf16 ? 8 : 4);
+      const uint8_t* from = static_cast<const uint8_t*>(p.dout) +
+                            (m0 + rb * 32 + row) * d_step + col * (kBf16 ? 2 : 4);
+      if (col < p.n / kSets) {
+#pragma unroll
+        for (int k = 0; k < 32 / kRows; ++k) {
+          const int place = piece ^ (kBf16 ? row & 4 : k & 1);
+          if (rb * 32 + row + k * kRows < rows)
+            copy_async_at<16>(to + (row + k * kRows) * kGradRow + place * 16, from);
+          from += kRows * d_step;
+        }
+      }
+    }
+    if constexpr (kZ) {
+      const int piece = t & 7, row = t >> 3;
+      const int64_t col = static_cast<int64_t>(tc) * kSets * kTile + piece * 16;
+      const uint8_t* from = p.z_q + (m0 + rb * 32 + row) * p.n + col;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (rb * 32 + row + k * 16 < rows) {
+#pragma unroll
+          for (int s = 0; s < kSets; ++s)
+            if (col + s * kTile < p.n)
+              copy_async_at<16>(to + 32 * kGradRow + s * 4096 + (row + k * 16) * 128 +
+                                    (piece ^ 2 * warp) * 16,
+                                from + s * kTile);
+        }
+        from += 16 * p.n;
+      }
+    }
+    stage_commit();
+  };
   // Scales first: the CTA's barrier waits for them.
   uint32_t zw[4] = {0, 0, 0, 0};
   if (kZ && threadIdx.x < kSets * 32) {
@@ -186,9 +238,6 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
     }
   }
   if constexpr (kLines) {
-    // All 32 rows of the warp, in whole lines: piece c of row 4 a + b at place
-    // c ^ 2 (a % 4), so that the 4 x 32 bytes that half a warp reads of rows 4 apart
-    // lie in all banks.
     const int piece = lane & 7, row = warp * 32 + (lane >> 3);
     const uint8_t* from = p.z_q + (m0 + row) * p.n + tc * kTile + piece * 16;
     if (static_cast<int64_t>(tc) * kTile + piece * 16 < p.n) {
@@ -201,9 +250,10 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
       }
     }
     stage_commit();
+  } else if constexpr (kShared) {
+    fetch_lines(0);
   } else if (active) {
     fetch(group);
-    if constexpr (kGroups == 1) fetch(1);
   }
   if (threadIdx.x < kSets * 32) {
     const int s = threadIdx.x / 32, i = threadIdx.x % 32;
@@ -223,7 +273,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
   for (int s = 0; s < kSets; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[s][j] = make_float2(0.0f, 0.0f);
-  if (active) {
+  if (active || kShared) {
     uint8_t* row_out = p.dz_q + (m0 + group * 32 + rg * 4) * p.n + zc;
     uint8_t* col_out = p.dzt_q + zc * p.mt + m0 + (kLines ? warp : group) * 32 + rg * 4;
     if constexpr (kLines) {
@@ -236,7 +286,12 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
       const int rb = kLines ? warp : it, cb = kLines ? it : warp;  // block row and column
       const int r0 = rb * 32 + rg * 4;  // this lane's first row of the tile
       const int slot = kGroups > 1 ? rb : rb & 1;
-      if constexpr (!kLines) stage_wait<(kGroups > 1 ? 0 : 1)>();
+      if constexpr (!kLines) stage_wait<0>();
+      if constexpr (kShared) {
+        __syncthreads();  // these rows have come, and the rows before them been read
+        if ((it + 1) * 32 < rows) fetch_lines(it + 1);
+        if (!active) continue;
+      }
       float2 v[kSets][4][4];
       float zs[kSets][4];
       if constexpr (kZ) {
@@ -252,12 +307,15 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
           const int at = slot * 4 + i;
           float2 d[4];
           if constexpr (kGrad)
-            read_grad8<kBf16>(stage_d + at * kGradBytes * 128, 2048, d);
+            read_grad8<kBf16>(kShared ? line_d + slot * kSlotBytes + i * kGradRow
+                                      : stage_d + at * kGradBytes * 128,
+                              d_second, d);
           if constexpr (kZ) {
 #pragma unroll
             for (int s = 0; s < kSets; ++s)
-              read_mx8(kLines ? stage_line + i * 128 + (cb * 32 ^ (rg & 3) * 32)
-                              : stage_z + (at * kSets + s) * 1024,
+              read_mx8(kLines    ? stage_line + i * 128 + (cb * 32 ^ (rg & 3) * 32)
+                       : kShared ? line_z + slot * kSlotBytes + s * 4096 + i * 128
+                                 : stage_z + (at * kSets + s) * 1024,
                        zs[s][i], v[s][i]);
           }
 #pragma unroll
@@ -277,7 +335,6 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
             for (int j = 0; j < 4; ++j) v[s][i][j] = make_float2(0.0f, 0.0f);
         }
       }
-      if constexpr (kGroups == 1 && !kLines) fetch(rb + 2);  // the slot has been read
 #pragma unroll
       for (int s = 0; s < kSets; ++s) {
         float2 (&x)[4][4] = v[s];
@@ -366,7 +423,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
       col_out += kLines ? 32 * p.mt : 32;
     }
     if constexpr (kGrad) {
-      if (p.dbias_part) {
+      if (p.dbias_part && active) {
 #pragma unroll
         for (int s = 0; s < kSets; ++s) {
 #pragma unroll

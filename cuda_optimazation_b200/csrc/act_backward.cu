@@ -325,8 +325,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
             else if constexpr (kAct == kActNone)
               v[0][i][j] = d[j];
             else if constexpr (kAct > 0)
-              v[0][i][j] = mul2(d[j], make_float2(act_slope<kAct>(v[0][i][j].x),
-                                                  act_slope<kAct>(v[0][i][j].y)));
+              v[0][i][j] = mul2(d[j], act_slope2<kAct>(v[0][i][j]));
           }
         } else {
 #pragma unroll

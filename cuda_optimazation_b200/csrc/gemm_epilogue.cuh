@@ -3,7 +3,9 @@
 //   z = alpha acc + bias,  y = act(z) (or silu(gate) * factor),  out = y + residual,
 // out in fp32, bf16 or MXFP8, and optionally z itself as an MXFP8 checkpoint.
 // All of it is fp32; each output is rounded once, at its store.  A thread's
-// 32 columns are one MX block, so its amax needs no other lane.
+// 32 columns are one MX block, so its amax needs no other lane.  In the pair kernel
+// it overlaps the next tile's products: 4096 x 28672 x 4096 gated with MXFP8 output and
+// checkpoint takes 374-390 us, the plain GEMM of that shape with bf16 output 366-371.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

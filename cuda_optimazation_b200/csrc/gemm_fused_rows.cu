@@ -4,8 +4,8 @@
 // The product is bound by streaming the weights B [n][k] once, so they are the
 // MMA's M side: D[128 weight rows][kN activation rows] in TMEM, one weight tile
 // (the gated form: the 128 gate rows and their 128 factor rows) per cluster.  The
-// clusters' CTAs split K, as many as keep every SM streaming (two CTAs an SM
-// where their accumulators and rings fit, one otherwise): a CTA's ring holds
+// clusters' CTAs split K, as many as keep every SM streaming (one CTA an SM, or two
+// for long shares where their accumulators and rings fit): a CTA's ring holds
 // ~100 KB, twice what HBM's latency asks of an SM.  The partial sums meet in
 // the cluster's shared memory, where every CTA sums and finishes its share
 // of the rows in a fixed order: no workspace, no atomics, one launch.
@@ -19,6 +19,10 @@
 // Roles (8 warps): warp 0 TMA producer, warp 1 MMA issuer (and TMEM owner),
 // warps 2..5 read the accumulator (one TMEM lane quadrant each); all eight finish
 // rows.  Every wait is bounded (qg_ptx.cuh).
+//
+// Measured (MXFP8): one token, 2 x 14336 x 4096 gated, 21.2 us (5.7 TB/s), x 8192
+// 37.5 (6.45 TB/s, the rate of a copy); 64 x 4096 x 14336 16.6 us, of which about 6
+// are start, exchange and end.  NVFP4 16 x 28672 x 8192 24.6 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

@@ -362,16 +362,19 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
       }
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
+        // Only what this lane goes on to store is read: a store waits for its values, so
+        // every remote read has ended when the warp reaches the closing barrier, after
+        // which the read CTA may be gone.
         const int i = i0 + u * 8 * ranks;
-        const bool on = i < Cfg::kPass && t0 + i < p.m;
+        const bool on = i < Cfg::kPass && t0 + i < p.m && in_z;
 #pragma unroll
         for (int s = 0; s < Cfg::kSets; ++s) {
           float4 v[kMaxRanks];
-          const uint32_t at = part_addr + ((s * Cfg::kPass + (on ? i : 0)) * 128 + f) * 4;
+          const uint32_t at = part_addr + ((s * Cfg::kPass + i) * 128 + f) * 4;
 #pragma unroll
           for (int r = 0; r < kMaxRanks; ++r)
-            v[r] = r < ranks ? ld_cluster_f32x4(mapa_shared(at, static_cast<uint32_t>(r)))
-                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v[r] = on && r < ranks ? ld_cluster_f32x4(mapa_shared(at, static_cast<uint32_t>(r)))
+                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int r = 1; r < kMaxRanks; ++r) {
             v[0].x += v[r].x;

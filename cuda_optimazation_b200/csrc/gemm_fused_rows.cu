@@ -69,10 +69,8 @@ struct RowsCfg {
   static constexpr int kStages = kTwo ? kStagesTwo : kStagesOne;
   static_assert(kStages >= 2, "ring");
   static constexpr int kTmemCols = pow2_at_least(kAccCols + kStages * kSfCols);
-  // Rows whose partial sums are exchanged at a time (in the ring's memory).
-  static constexpr int kPass =
-      kSets * kN * 512 <= kStages * kStageBytes ? kN : kN / 2;
-  static_assert(kSets * kPass * 512 <= kStages * kStageBytes, "exchange buffer");
+  // The partial sums are exchanged through the ring's memory.
+  static_assert(kSets * kN * 512 <= kStages * kStageBytes, "exchange buffer");
   static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
   // Never three CTAs on an SM, whose TMEM would not do.
   static_assert(3 * (kSmemBytes + 1024) > 228 * 1024 && kTmemCols <= (kTwo ? 256 : 512),
@@ -297,7 +295,7 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
   for (int s = 0; s < Cfg::kSets; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) bias[s][j] = epi_bias(e, col0 + s * 128 + f + j, p.n);
-  float* part = reinterpret_cast<float*>(smem);  // [set][row of the pass][128]
+  float* part = reinterpret_cast<float*>(smem);  // [set][row][128]
   const uint32_t part_addr = smem_u32(part);
   bool ok = true;
   if (warp >= 2 && warp <= 5) {
@@ -308,143 +306,139 @@ __global__ void __launch_bounds__(256, RowsCfg<kFmt, kN, kGated>::kPerSm)
     if (ok) mbar_try_wait(acc_full, 0);
     tc_fence_after();
   }
+  if (warp >= 2 && warp <= 5 && ok) {
+    const int quad = warp % 4;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
 #pragma unroll 1
-  for (int t0 = 0; t0 < kN && t0 < p.m; t0 += Cfg::kPass) {
-    if (warp >= 2 && warp <= 5 && ok) {
-      const int quad = warp % 4;
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    for (int s = 0; s < Cfg::kSets; ++s) {
 #pragma unroll 1
-      for (int s = 0; s < Cfg::kSets; ++s) {
-#pragma unroll 1
-        for (int c = 0; c < Cfg::kPass && t0 + c < p.m; c += 16) {
-          uint32_t r[16];
-          __syncwarp();
-          tmem_ld_32x32b_x16(t_row + s * kN + t0 + c, r);
-          tmem_wait_ld();
-          float* to = part + (s * Cfg::kPass + c) * 128 + quad * 32 + lane;
+      for (int c = 0; c < p.m; c += 16) {
+        uint32_t r[16];
+        __syncwarp();
+        tmem_ld_32x32b_x16(t_row + s * kN + c, r);
+        tmem_wait_ld();
+        float* to = part + (s * kN + c) * 128 + quad * 32 + lane;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) to[j * 128] = __uint_as_float(r[j]);
-        }
+        for (int j = 0; j < 16; ++j) to[j * 128] = __uint_as_float(r[j]);
       }
     }
-    __syncwarp();
-    cluster_sync();  // every CTA's partial sums are in place
-    // A warp finishes every (8 ranks)-th row of the pass, kTogether rows at a
-    // time: all their remote loads and residuals are in flight at once.
-    constexpr int kTogether = kGated ? 1 : 2;
-    for (int i0 = rank * 8 + warp; i0 < Cfg::kPass && t0 + i0 < p.m;
-         i0 += 8 * ranks * kTogether) {
-      float z[kTogether][Cfg::kSets][4];
-      uint32_t res[kTogether][4];  // raw; beyond the matrix its last row or columns
-      if (e.res) {
-#pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-          const int64_t at = min(t0 + i0 + u * 8 * ranks, p.m - 1) * e.ldr;
-          if (e.res_vec && n_out % 4 == 0) {
-            const int64_t c = at + min(out_col, n_out - 4);
-            if (e.res_bf16) {
-              const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(e.res) + c);
-              res[u][0] = r.x << 16; res[u][1] = r.x & 0xffff0000u;
-              res[u][2] = r.y << 16; res[u][3] = r.y & 0xffff0000u;
-            } else {
-              const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(e.res) + c);
-              res[u][0] = r.x; res[u][1] = r.y; res[u][2] = r.z; res[u][3] = r.w;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int64_t c = at + min(out_col + j, n_out - 1);
-              if (e.res_bf16) res[u][j] = static_cast<uint32_t>(static_cast<const uint16_t*>(e.res)[c]) << 16;
-              else res[u][j] = static_cast<const uint32_t*>(e.res)[c];
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        // Only what this lane goes on to store is read: a store waits for its values, so
-        // every remote read has ended when the warp reaches the closing barrier, after
-        // which the read CTA may be gone.
-        const int i = i0 + u * 8 * ranks;
-        const bool on = i < Cfg::kPass && t0 + i < p.m && in_z;
-#pragma unroll
-        for (int s = 0; s < Cfg::kSets; ++s) {
-          float4 v[kMaxRanks];
-          const uint32_t at = part_addr + ((s * Cfg::kPass + i) * 128 + f) * 4;
-#pragma unroll
-          for (int r = 0; r < kMaxRanks; ++r)
-            v[r] = on && r < ranks ? ld_cluster_f32x4(mapa_shared(at, static_cast<uint32_t>(r)))
-                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-          for (int r = 1; r < kMaxRanks; ++r) {
-            v[0].x += v[r].x;
-            v[0].y += v[r].y;
-            v[0].z += v[r].z;
-            v[0].w += v[r].w;
-          }
-          z[u][s][0] = v[0].x; z[u][s][1] = v[0].y; z[u][s][2] = v[0].z; z[u][s][3] = v[0].w;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        const int i = i0 + u * 8 * ranks;
-        if (i >= Cfg::kPass || t0 + i >= p.m) break;
-        const int row = t0 + i;
-#pragma unroll
-        for (int s = 0; s < Cfg::kSets; ++s) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) z[u][s][j] = z[u][s][j] * alpha + bias[s][j];
-          if (e.z_q)
-            lane_store_mx(z[u][s], in_z, e.z_q, e.z_sf, e.z_layout, e.z_sf_blocks, row,
-                          col0 + s * 128 + f, p.n, lane);
-        }
-        float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (kGated) {
-            y[j] = act_fwd<kActSilu>(z[u][0][j]) * z[u][1][j];
-          } else {
-            y[j] = z[u][0][j];
-            if (e.act == kActRelu) y[j] = act_fwd<kActRelu>(y[j]);
-            else if (e.act == kActSilu) y[j] = act_fwd<kActSilu>(y[j]);
-            else if (e.act == kActGelu) y[j] = act_fwd<kActGelu>(y[j]);
-          }
-          if (e.res) y[j] += __uint_as_float(res[u][j]);
-        }
-        if (e.out_kind == kEpiMxfp8) {
-          lane_store_mx(y, in_z, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout,
-                        e.out_sf_blocks, row, out_col, n_out, lane);
-        } else {
-          const int64_t at = row * e.ldc + out_col;
-          const bool whole = e.out_vec && out_col + 4 <= n_out;
-          if (e.out_kind == kEpiBf16) {
-            __nv_bfloat16* c = static_cast<__nv_bfloat16*>(e.out) + at;
-            if (whole) {
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]);
-              const __nv_bfloat162 hi = __floats2bfloat162_rn(y[2], y[3]);
-              *reinterpret_cast<uint2*>(c) =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo),
-                             *reinterpret_cast<const uint32_t*>(&hi));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (out_col + j < n_out) c[j] = __float2bfloat16_rn(y[j]);
-            }
-          } else {
-            float* c = static_cast<float*>(e.out) + at;
-            if (whole) {
-              *reinterpret_cast<float4*>(c) = make_float4(y[0], y[1], y[2], y[3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (out_col + j < n_out) c[j] = y[j];
-            }
-          }
-        }
-      }
-    }
-    cluster_sync_relaxed();  // the sums have been read: reuse the buffer, or exit
   }
+  __syncwarp();
+  cluster_sync();  // every CTA's partial sums are in place
+  // A warp finishes every (8 ranks)-th row, kTogether rows at a time: all their remote
+  // loads and residuals are in flight at once.
+  constexpr int kTogether = kGated ? 1 : 2;
+  for (int i0 = rank * 8 + warp; i0 < p.m; i0 += 8 * ranks * kTogether) {
+    float z[kTogether][Cfg::kSets][4];
+    uint32_t res[kTogether][4];  // raw; beyond the matrix its last row or columns
+    if (e.res) {
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const int64_t at = min(i0 + u * 8 * ranks, p.m - 1) * e.ldr;
+        if (e.res_vec && n_out % 4 == 0) {
+          const int64_t c = at + min(out_col, n_out - 4);
+          if (e.res_bf16) {
+            const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(e.res) + c);
+            res[u][0] = r.x << 16; res[u][1] = r.x & 0xffff0000u;
+            res[u][2] = r.y << 16; res[u][3] = r.y & 0xffff0000u;
+          } else {
+            const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(e.res) + c);
+            res[u][0] = r.x; res[u][1] = r.y; res[u][2] = r.z; res[u][3] = r.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int64_t c = at + min(out_col + j, n_out - 1);
+            if (e.res_bf16) res[u][j] = static_cast<uint32_t>(static_cast<const uint16_t*>(e.res)[c]) << 16;
+            else res[u][j] = static_cast<const uint32_t*>(e.res)[c];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      // Only what this lane goes on to store is read: a store waits for its values, so
+      // every remote read has ended when the warp reaches the closing barrier, after
+      // which the read CTA may be gone.
+      const int i = i0 + u * 8 * ranks;
+      const bool on = i < p.m && in_z;
+#pragma unroll
+      for (int s = 0; s < Cfg::kSets; ++s) {
+        float4 v[kMaxRanks];
+        const uint32_t at = part_addr + ((s * kN + i) * 128 + f) * 4;
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; ++r)
+          v[r] = on && r < ranks ? ld_cluster_f32x4(mapa_shared(at, static_cast<uint32_t>(r)))
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int r = 1; r < kMaxRanks; ++r) {
+          v[0].x += v[r].x;
+          v[0].y += v[r].y;
+          v[0].z += v[r].z;
+          v[0].w += v[r].w;
+        }
+        z[u][s][0] = v[0].x; z[u][s][1] = v[0].y; z[u][s][2] = v[0].z; z[u][s][3] = v[0].w;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int i = i0 + u * 8 * ranks;
+      if (i >= p.m) break;
+      const int row = i;
+#pragma unroll
+      for (int s = 0; s < Cfg::kSets; ++s) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[u][s][j] = z[u][s][j] * alpha + bias[s][j];
+        if (e.z_q)
+          lane_store_mx(z[u][s], in_z, e.z_q, e.z_sf, e.z_layout, e.z_sf_blocks, row,
+                        col0 + s * 128 + f, p.n, lane);
+      }
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (kGated) {
+          y[j] = act_fwd<kActSilu>(z[u][0][j]) * z[u][1][j];
+        } else {
+          y[j] = z[u][0][j];
+          if (e.act == kActRelu) y[j] = act_fwd<kActRelu>(y[j]);
+          else if (e.act == kActSilu) y[j] = act_fwd<kActSilu>(y[j]);
+          else if (e.act == kActGelu) y[j] = act_fwd<kActGelu>(y[j]);
+        }
+        if (e.res) y[j] += __uint_as_float(res[u][j]);
+      }
+      if (e.out_kind == kEpiMxfp8) {
+        lane_store_mx(y, in_z, static_cast<uint8_t*>(e.out), e.out_sf, e.out_layout,
+                      e.out_sf_blocks, row, out_col, n_out, lane);
+      } else {
+        const int64_t at = row * e.ldc + out_col;
+        const bool whole = e.out_vec && out_col + 4 <= n_out;
+        if (e.out_kind == kEpiBf16) {
+          __nv_bfloat16* c = static_cast<__nv_bfloat16*>(e.out) + at;
+          if (whole) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]);
+            const __nv_bfloat162 hi = __floats2bfloat162_rn(y[2], y[3]);
+            *reinterpret_cast<uint2*>(c) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&lo),
+                           *reinterpret_cast<const uint32_t*>(&hi));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (out_col + j < n_out) c[j] = __float2bfloat16_rn(y[j]);
+          }
+        } else {
+          float* c = static_cast<float*>(e.out) + at;
+          if (whole) {
+            *reinterpret_cast<float4*>(c) = make_float4(y[0], y[1], y[2], y[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (out_col + j < n_out) c[j] = y[j];
+          }
+        }
+      }
+    }
+  }
+  cluster_sync_relaxed();  // the sums have been read: their CTA may exit
   if (rank == 0) {
     if (e.out_kind == kEpiMxfp8)
       pad_rows(e.out_sf, e.out_layout, e.out_sf_blocks, out_col - f, p.m);

@@ -291,6 +291,8 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
               gated_grad2(d[j], v[0][i][j], v[1][i][j], v[0][i][j], v[1][i][j]);
             else if constexpr (kAct == kActNone)
               v[0][i][j] = d[j];
+            else if constexpr (kAct == kActRelu)
+              v[0][i][j] = relu_grad2(d[j], v[0][i][j]);
             else if constexpr (kAct > 0)
               v[0][i][j] = mul2(d[j], act_slope2<kAct>(v[0][i][j]));
           }

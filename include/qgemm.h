@@ -307,7 +307,8 @@ int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh
 /* Workspace bytes qg_rmsnorm_backward needs for dweight (0: none, NULL will do). */
 size_t qg_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t k);
 
-/* Activations: gelu is the tanh form, relu's slope at 0 is 0.  QG_ACT_SWIGLU gates: of every 256
+/* Activations: gelu is the tanh form; relu's gradient is dout where z > 0 and 0 where
+ * z <= 0, whatever dout is there.  QG_ACT_SWIGLU gates: of every 256
  * columns of z the first 128 are gates g, the next 128 their factors u, and
  * the output's 128 columns are silu(g) * u (n % 256 == 0). */
 typedef enum {

@@ -274,8 +274,9 @@ PyObject* gemm_fused(PyObject*, PyObject* const* a, Py_ssize_t n) {
       e.residual = ptr(res);
       e.residual_dtype = dtype_code(*res, "residual");
     }
-    if (status && (!status->is_cuda() || status->numel() < 1 || status->element_size() != 4))
-      refuse_value("status must be a 32-bit word on the device");
+    if (status &&
+        (status->device() != dev || status->numel() < 1 || status->element_size() != 4))
+      refuse_value("status must be a 32-bit word on " + dev.str());
     Here here(dev);
     at::Tensor out, out_sf, zq, zsf;
     e.out_dtype = out_dtype;

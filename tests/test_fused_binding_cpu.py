@@ -1,0 +1,28 @@
+"""CPU: what the layer operators' binding refuses before it touches a device, shown
+with fake tensors (shapes, types and devices without memory)."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+
+@pytest.fixture(scope="module")
+def F(qlib):
+    from cuda_optimazation_b200 import fused
+    return fused
+
+
+def fake(*shape, dtype=torch.float32, device="cuda:0"):
+    with FakeTensorMode():
+        return torch.empty(*shape, dtype=dtype, device=device)
+
+
+def held(qlib, rows=128, k=128):
+    return qlib.Mxfp8Result(fake(rows * k, dtype=torch.uint8), fake(512, dtype=torch.uint8), rows,
+                            k, 1)
+
+
+def test_status_on_another_device(F, qlib):
+    for where in ("cuda:1", "cpu"):
+        with pytest.raises(ValueError, match="status"):
+            F.gemm_fused(held(qlib), held(qlib),
+                         status=fake(1, dtype=torch.int32, device=where))

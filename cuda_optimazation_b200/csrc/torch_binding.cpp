@@ -309,19 +309,20 @@ PyObject* gemm_fused(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// dout, z (q, sf | None, None), z rows, z columns, z_layout, act, layout, want dbias
+// dout, z (q, sf, or both None), z rows, z columns, z_layout, act, layout, want dbias
 // -> status, dz q, dz sf, dzt q, dzt sf, dbias | None
 PyObject* act_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 9, [&] {
     const at::Tensor& d = tensor(a[0], "dout");
-    const at::Tensor* zq = optional_tensor(a[1], "checkpoint");
-    const at::Tensor* zsf = optional_tensor(a[2], "checkpoint");
+    const bool z = a[1] != Py_None || a[2] != Py_None;
+    const at::Tensor* zq = z ? &tensor(a[1], "checkpoint") : nullptr;
+    const at::Tensor* zsf = z ? &tensor(a[2], "checkpoint") : nullptr;
     const int z_layout = static_cast<int>(integer(a[5]));
     const int act = static_cast<int>(integer(a[6])), layout = static_cast<int>(integer(a[7]));
     const c10::Device dev = cuda_matrix(d, "dout");
     const int64_t m = d.size(0), cols = d.size(1), nn = act == QG_ACT_SWIGLU ? 2 * cols : cols;
     const int code = dtype_code(d, "dout");
-    if (zq && (integer(a[3]) != m || integer(a[4]) != nn ||
+    if (z && (integer(a[3]) != m || integer(a[4]) != nn ||
                held(*zq, *zsf, m, nn, z_layout, QG_FORMAT_MXFP8, "checkpoint") != dev))
       refuse_value("checkpoint must be " + std::to_string(m) + " x " + std::to_string(nn) +
                    " on the device of dout");

@@ -26,3 +26,14 @@ def test_status_on_another_device(F, qlib):
         with pytest.raises(ValueError, match="status"):
             F.gemm_fused(held(qlib), held(qlib),
                          status=fake(1, dtype=torch.int32, device=where))
+
+
+def test_checkpoint_without_scales(F, qlib):
+    z = held(qlib)
+    z.block_scales = None
+    with pytest.raises(TypeError, match="checkpoint"):
+        F.act_backward(fake(128, 128), z, "relu")
+    z = held(qlib)
+    z.quantized = None
+    with pytest.raises(TypeError, match="checkpoint"):
+        F.act_backward(fake(128, 128), z, "relu")

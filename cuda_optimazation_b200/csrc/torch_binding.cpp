@@ -50,7 +50,14 @@ double real(PyObject* o) {
   }
   return v;
 }
-bool flag(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool flag(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    refuse_type("expected a truth value");
+  }
+  return v == 1;
+}
 
 int dtype_code(const at::Tensor& t, const char* what) {
   if (t.scalar_type() == at::kFloat) return QG_DTYPE_F32;

@@ -37,3 +37,13 @@ def test_checkpoint_without_scales(F, qlib):
     z.quantized = None
     with pytest.raises(TypeError, match="checkpoint"):
         F.act_backward(fake(128, 128), z, "relu")
+
+
+class NoTruth:
+    def __bool__(self):
+        raise RuntimeError("no truth value")
+
+
+def test_flag_without_a_truth_value(F, qlib):
+    with pytest.raises(TypeError, match="truth value"):
+        F.gemm_fused(held(qlib), held(qlib), checkpoint=NoTruth())

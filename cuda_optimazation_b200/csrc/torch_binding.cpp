@@ -42,6 +42,12 @@ int64_t integer(PyObject* o) {
   }
   return v;
 }
+// A layout as the C ABI's int (which of them an operator takes is the ABI's to say).
+int layout_code(PyObject* o) {
+  const int64_t v = integer(o);
+  if (v != static_cast<int>(v)) refuse_value("unknown layout " + std::to_string(v));
+  return static_cast<int>(v);
+}
 double real(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) {
@@ -169,7 +175,7 @@ PyObject* rmsnorm_mxfp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor& w = tensor(a[1], "weight");
     const at::Tensor* res = optional_tensor(a[2], "residual");
     const float eps = static_cast<float>(real(a[3]));
-    const int layout = static_cast<int>(integer(a[4]));
+    const int layout = layout_code(a[4]);
     const at::Tensor* h_in = optional_tensor(a[5], "h");
     const c10::Device dev = cuda_matrix(x, "x");
     const int64_t rows = x.size(0), k = x.size(1);
@@ -251,15 +257,15 @@ PyObject* gemm_fused(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor& bsf = tensor(a[6], "b");
     const at::Tensor* bts = optional_tensor(a[7], "b");
     const int64_t nn = integer(a[8]), k = integer(a[9]);
-    const int sf_layout = static_cast<int>(integer(a[10]));
+    const int sf_layout = layout_code(a[10]);
     const at::Tensor* bias = optional_tensor(a[11], "bias");
     const int act = static_cast<int>(integer(a[12]));
     const at::Tensor* res = optional_tensor(a[13], "residual");
     const int out_dtype = static_cast<int>(integer(a[14]));
     const at::Tensor* out_in = optional_tensor(a[15], "out");
-    const int out_layout = static_cast<int>(integer(a[16]));
+    const int out_layout = layout_code(a[16]);
     const bool ckpt = flag(a[17]);
-    const int ckpt_layout = static_cast<int>(integer(a[18]));
+    const int ckpt_layout = layout_code(a[18]);
     const at::Tensor* status = optional_tensor(a[19], "status");
     const c10::Device dev = held(aq, asf, m, k, sf_layout, format, "a");
     if (held(bq, bsf, nn, k, sf_layout, format, "b") != dev)
@@ -324,8 +330,8 @@ PyObject* act_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool z = a[1] != Py_None || a[2] != Py_None;
     const at::Tensor* zq = z ? &tensor(a[1], "checkpoint") : nullptr;
     const at::Tensor* zsf = z ? &tensor(a[2], "checkpoint") : nullptr;
-    const int z_layout = static_cast<int>(integer(a[5]));
-    const int act = static_cast<int>(integer(a[6])), layout = static_cast<int>(integer(a[7]));
+    const int z_layout = layout_code(a[5]);
+    const int act = static_cast<int>(integer(a[6])), layout = layout_code(a[7]);
     const c10::Device dev = cuda_matrix(d, "dout");
     const int64_t m = d.size(0), cols = d.size(1), nn = act == QG_ACT_SWIGLU ? 2 * cols : cols;
     const int code = dtype_code(d, "dout");
@@ -361,7 +367,7 @@ PyObject* transpose_mxfp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor& q = tensor(a[0], "a");
     const at::Tensor& sf = tensor(a[1], "a");
     const int64_t rows = integer(a[2]), k = integer(a[3]);
-    const int layout = static_cast<int>(integer(a[4])), to = static_cast<int>(integer(a[5]));
+    const int layout = layout_code(a[4]), to = layout_code(a[5]);
     const c10::Device dev = held(q, sf, rows, k, layout, QG_FORMAT_MXFP8, "a");
     Here here(dev);
     const int64_t rt = (rows + 31) / 32 * 32;

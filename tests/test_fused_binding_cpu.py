@@ -47,3 +47,16 @@ class NoTruth:
 def test_flag_without_a_truth_value(F, qlib):
     with pytest.raises(TypeError, match="truth value"):
         F.gemm_fused(held(qlib), held(qlib), checkpoint=NoTruth())
+
+
+@pytest.mark.parametrize("layout", [1 + (1 << 32), -(1 << 32), 1 << 40])
+def test_layout_beyond_an_int(F, qlib, layout):
+    """Not cut down to the layout of its low 32 bits."""
+    a = held(qlib)
+    for call in (lambda: F.transpose_mxfp8(a, layout),
+                 lambda: F.gemm_fused(a, a, out="mxfp8", layout=layout),
+                 lambda: F.gemm_fused(a, a, checkpoint=True, checkpoint_layout=layout),
+                 lambda: F.act_backward(fake(128, 128), a, "relu", layout=layout),
+                 lambda: F.rmsnorm_mxfp8(fake(128, 128), fake(128), layout=layout)):
+        with pytest.raises(ValueError, match="layout"):
+            call()

@@ -103,7 +103,11 @@ int64_t scale_bytes(int64_t rows, int64_t k, int sv, int layout) {
 // A quantised operand's buffers against its shape.  format: qg_format.
 c10::Device held(const at::Tensor& q, const at::Tensor& sf, int64_t rows, int64_t k, int layout,
                  int format, const char* what) {
-  const int64_t values = format == QG_FORMAT_MXFP8 ? rows * k : rows * k / 2;
+  int64_t values = 0;
+  // 2^48 values: no device holds them, and nothing below can wrap round.
+  if (__builtin_mul_overflow(rows, k, &values) || values > int64_t{1} << 48)
+    refuse_value(std::string(what) + ": buffers are smaller than the shape needs");
+  if (format != QG_FORMAT_MXFP8) values /= 2;
   const int sv = format == QG_FORMAT_NVFP4 ? 16 : 32;
   if (rows < 0 || k < 0 || q.numel() < values || sf.numel() < scale_bytes(rows, k, sv, layout))
     refuse_value(std::string(what) + ": buffers are smaller than the shape needs");

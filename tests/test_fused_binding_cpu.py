@@ -60,3 +60,16 @@ def test_layout_beyond_an_int(F, qlib, layout):
                  lambda: F.rmsnorm_mxfp8(fake(128, 128), fake(128), layout=layout)):
         with pytest.raises(ValueError, match="layout"):
             call()
+
+
+@pytest.mark.parametrize("rows,k", [(1 << 31, 1 << 33), (1 << 32, 1 << 32), (1 << 62, 32), (1, 1 << 62)])
+def test_shape_whose_size_overflows(F, qlib, rows, k):
+    """The buffers' sizes are compared without wrapping round."""
+    a = held(qlib)
+    a.rows, a.k = rows, k
+    b = held(qlib)
+    b.k = k
+    for call in (lambda: F.transpose_mxfp8(a), lambda: F.gemm_fused(a, a),
+                 lambda: F.gemm_fused(b, a)):
+        with pytest.raises(ValueError, match="smaller than the shape"):
+            call()

@@ -11,6 +11,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <optional>
@@ -162,14 +163,14 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F&& body) {
     PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
     return nullptr;
   }
+  HANDLE_TH_ERRORS  // torch's exceptions as torch's Python errors (OutOfMemoryError)
   try {
     return body();
   } catch (const Refusal& r) {
     PyErr_SetString(r.type, r.what.c_str());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
   }
-  return nullptr;
+  END_HANDLE_TH_ERRORS
 }
 
 // x, weight, residual | None, eps, layout, h | None -> status, q, sf, h | None, rstd

@@ -44,3 +44,13 @@ def test_relu_slope_at_its_edges(F, qlib, m, dt):
     ok[31] = ok[4] = False
     assert torch.equal(o.dbias[ok].double(), want[:, ok].sum(0))
     assert bool(o.dbias[31].isnan()) and float(o.dbias[4]) == INF
+
+
+def test_out_of_memory_error(F, qlib):
+    """An output that does not fit raises torch's own error, as torch.empty does."""
+    d = torch.zeros(1, 1 << 18, device=DEV, dtype=torch.bfloat16).expand(1 << 21, 1 << 18)
+    with pytest.raises(torch.OutOfMemoryError):
+        F.act_backward(d, None, "none")
+    a = torch.zeros(1, 32768, device=DEV).expand(1 << 25, 32768)
+    with pytest.raises(torch.OutOfMemoryError):
+        F.rmsnorm_mxfp8(a, a[0])

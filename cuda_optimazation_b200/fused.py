@@ -58,6 +58,14 @@ def _act_code(act: str) -> int:
     return code
 
 
+def _on(stream: torch.cuda.Stream, held) -> torch.cuda.StreamContext:
+    """`stream` as the current one for a call on `held` (a matrix or an operand)."""
+    device = getattr(getattr(held, "quantized", held), "device", None)
+    if device is not None and device != stream.device:
+        raise ValueError(f"stream is on {stream.device}, the operands on {device}")
+    return torch.cuda.stream(stream)
+
+
 # ------------------------------------------------------------------ RMS norm
 @dataclass
 class RmsNormResult:
@@ -75,7 +83,7 @@ def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torc
     16-byte vectors; residual as x; weight fp32/bf16 [k].  ``h`` may be given
     as the buffer for the sum (x or residual itself, to update in place)."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, x):
             return rmsnorm_mxfp8(x, weight, residual, eps, layout, h)
     rc, q, sf, new_h, rstd = _native().rmsnorm_mxfp8(x, weight, residual, eps, layout, h)
     if rc:
@@ -94,7 +102,7 @@ def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weig
     the gradient that reaches h past the norm.  dx (h's dtype) is the gradient
     of x and of the residual; dweight is fp32 (None if not wanted)."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, dy):
             return rmsnorm_backward(dy, h, rstd, weight, dres, want_dweight)
     rc, dx, dw = _native().rmsnorm_backward(dy, h, rstd, weight, dres, want_dweight)
     if rc:
@@ -132,7 +140,7 @@ def gemm_fused(a: Operand, b: Operand, bias: Optional[torch.Tensor] = None, act:
     (an ``Mxfp8Result`` in ``layout``, the next product's operand) or a tensor to
     write to.  checkpoint=True also returns A . B^T + bias as an ``Mxfp8Result``."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, a):
             return gemm_fused(a, b, bias, act, residual, out, layout, checkpoint,
                               checkpoint_layout, status)
     fmt = _FORMATS.get(type(a))
@@ -179,7 +187,7 @@ def act_backward(dout: torch.Tensor, checkpoint: Optional[Mxfp8Result], act: str
     (qg_act_backward_mxfp8).  dout: fp32/bf16 [m, n] ([m, n / 2] for "swiglu").
     checkpoint may be None for act="none"."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, dout):
             return act_backward(dout, checkpoint, act, layout, want_dbias)
     code = _act_code(act)
     z = checkpoint
@@ -208,7 +216,7 @@ def transpose_mxfp8(a: Mxfp8Result, layout: int = LAYOUT_MMA,
     scales along A's rows (qg_transpose_mxfp8): the kept 8-bit input of a product
     as the operand of its weight gradient."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, a):
             return transpose_mxfp8(a, layout)
     if type(a) is not Mxfp8Result:
         raise TypeError("a must be an Mxfp8Result")

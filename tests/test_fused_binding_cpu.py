@@ -73,3 +73,22 @@ def test_shape_whose_size_overflows(F, qlib, rows, k):
                  lambda: F.gemm_fused(b, a)):
         with pytest.raises(ValueError, match="smaller than the shape"):
             call()
+
+
+class StreamOn:
+    """What the operators look at of a torch.cuda.Stream, on a device of its own."""
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+
+
+def test_stream_of_another_device(F, qlib):
+    """Not run on the current stream of the operands' device instead."""
+    a, x, s = held(qlib), fake(128, 128), StreamOn("cuda:1")
+    for call in (lambda: F.rmsnorm_mxfp8(x, fake(128), stream=s),
+                 lambda: F.rmsnorm_backward(x, x, fake(128), fake(128), stream=s),
+                 lambda: F.gemm_fused(a, a, stream=s),
+                 lambda: F.act_backward(x, a, "relu", stream=s),
+                 lambda: F.transpose_mxfp8(a, stream=s)):
+        with pytest.raises(ValueError, match="stream"):
+            call()

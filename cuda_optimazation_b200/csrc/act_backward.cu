@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
         for (int k = 0; k < 32 / kRows; ++k) {
           const int place = piece ^ (kBf16 ? row & 4 : k & 1);
           if (rb * 32 + row + k * kRows < rows)
-            copy_async_at<16>(to + (row + k * kRows) * kGradRow + place * 16, from);
+            copy_async_at(to + (row + k * kRows) * kGradRow + place * 16, from);
           from += kRows * d_step;
         }
       }
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
 #pragma unroll
           for (int s = 0; s < kSets; ++s)
             if (col + s * kTile < p.n)
-              copy_async_at<16>(to + kZAt + s * 4096 + (row + k * 16) * 128 +
+              copy_async_at(to + kZAt + s * 4096 + (row + k * 16) * 128 +
                                     (piece ^ 2 * warp) * 16,
                                 from + s * kTile);
         }
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (row + i * 4 < rows)
-          copy_async_at<16>(smem_u32(staged) + (row + i * 4) * 128 + (piece ^ 2 * (i & 3)) * 16,
+          copy_async_at(smem_u32(staged) + (row + i * 4) * 128 + (piece ^ 2 * (i & 3)) * 16,
                             from);
         from += 4 * p.n;
       }

@@ -581,12 +581,9 @@ __device__ __forceinline__ uint2 lds64_at(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
-template <int kBytes>
+// 16 bytes of global memory, asynchronously (cp.async; past L1).
 __device__ __forceinline__ void copy_async_at(uint32_t to, const void* from) {
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ uint4 lds128(const void* p) {
   uint4 v;

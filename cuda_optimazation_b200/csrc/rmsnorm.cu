@@ -124,7 +124,7 @@ __device__ __forceinline__ const uint8_t* at_row(const void* base, int64_t row, 
 template <bool kBf16>
 __device__ __forceinline__ void ring_copy(uint32_t at, const uint8_t* from, uint32_t second) {
 #pragma unroll
-  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) copy_async_at<16>(at + i * second, from + 16 * i);
+  for (int i = 0; i < Raw8<kBf16>::kChunks; ++i) copy_async_at(at + i * second, from + 16 * i);
 }
 template <bool kBf16>
 __device__ __forceinline__ Raw8<kBf16> ring_read(uint32_t at, uint32_t second) {

@@ -451,12 +451,20 @@ __global__ void __launch_bounds__(128 * kGroups, kGroups == 1 && kAct == kActSwi
   }
 }
 
-// Few tiles: all four row groups of a tile at once, for latency; enough tiles to
-// fill the SMs with 128-thread CTAs several times: one group after the other.
+// One round of tiles: all four row groups of a tile at once, for latency.  Such a CTA
+// fills an SM (the transposition's half of one), so more tiles than that would take a
+// second round: 128-thread CTAs then, one group after the other.  Measured, us at once /
+// in turn: gelu bf16 of 64 tiles 6.5 / 9.0, 148 9.5 / 10.9, 152 13.8 / 12.0, 512 36.7 /
+// 17.0; transposition of 128 tiles 3.3 / 3.9, 288 5.0 / 5.3, 304 6.8 / 5.4.
 constexpr int kGroupsSmall = 4;
-bool small_grid(int64_t grid) { return grid < 4 * num_sms(); }
+bool small_grid(int64_t grid, int ctas_per_sm) { return grid <= ctas_per_sm * num_sms(); }
 // Row tiles that a cluster may join (the portable size).
 constexpr int kClusterRows = 8;
+// Tiles of which the clusters of `rows` CTAs, one an SM, find a place at once: of 148
+// SMs 148 in clusters of 2, 130 to 135 of 3 to 6, 105 of 7 and 120 of 8.
+int64_t cluster_tiles(int64_t rows) {
+  return num_sms() * (rows <= 2 ? 100 : rows <= 6 ? 87 : 70) / 100;
+}
 
 template <int kAct, bool kBf16, int kGroups>
 cudaError_t launch_one(const ActBackwardParams& p, int grid, cudaStream_t stream) {
@@ -494,8 +502,9 @@ cudaError_t launch_one(const ActBackwardParams& p, int grid, cudaStream_t stream
 
 template <int kAct, bool kBf16>
 cudaError_t launch_act(const ActBackwardParams& p, int grid, cudaStream_t stream) {
-  return small_grid(grid) ? launch_one<kAct, kBf16, kGroupsSmall>(p, grid, stream)
-                          : launch_one<kAct, kBf16, 1>(p, grid, stream);
+  return small_grid(grid, kAct < 0 ? 2 : 1)
+             ? launch_one<kAct, kBf16, kGroupsSmall>(p, grid, stream)
+             : launch_one<kAct, kBf16, 1>(p, grid, stream);
 }
 
 int64_t act_grid(int64_t m, int64_t n, int sets) {
@@ -504,10 +513,13 @@ int64_t act_grid(int64_t m, int64_t n, int sets) {
 
 }  // namespace
 
+// Joining saves the second launch where every cluster finds a place (us with / without:
+// 256 x 4096 gelu 6.5 / 7.3, 1024 x 1024 7.1 / 7.7, 512 x 4096 7.3 / 8.5), and costs a
+// round where one does not (512 x 4608 13.6 / 9.0, 1024 x 2048 13.8 / 8.7).
 bool act_backward_joins(int64_t m, int64_t n, int act) {
   const int64_t parts = (m + kTile - 1) / kTile;
-  return parts == 1 ||
-         (parts <= kClusterRows && small_grid(act_grid(m, n, act == kActSwiglu ? 2 : 1)));
+  return parts == 1 || (parts <= kClusterRows &&
+                        act_grid(m, n, act == kActSwiglu ? 2 : 1) <= cluster_tiles(parts));
 }
 
 cudaError_t launch_act_backward(const ActBackwardParams& in, int act, bool bf16,

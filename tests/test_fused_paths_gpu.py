@@ -143,7 +143,7 @@ def test_gemm_offsets_past_32_bits(F, qlib):
 
 
 # ------------------------------------------------------------------ activation backward
-# Many tiles (from 4 x SMs on): row groups one after the other; every layout of the
+# Many tiles: row groups one after the other; every layout of the
 # checkpoint, ragged last rows and columns, dbias through the partial sums.
 @pytest.mark.parametrize("m", [2500, 2501, 2531])
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
@@ -158,10 +158,13 @@ def test_gated_backward_many_tiles(F, qlib, m, n, dt):
     base.test_act_backward(F, qlib, m, n, "swiglu", dt)
 
 
-# Few tiles: dbias of up to 8 row tiles joined in a cluster, of more through the
-# partial sums; (1000, 9728): gated few tiles where the ungated form has many.
+# One round of tiles (148 SMs) and one more; dbias of up to 8 row tiles joined in a
+# cluster where all clusters find a place, else through the partial sums; (1000, 2048):
+# joined in the gated form, not in the ungated one.
 @pytest.mark.parametrize("m,n", [(500, 512), (769, 256), (1000, 512), (1024, 256), (1025, 256),
-                                 (2000, 256), (9000, 512), (1000, 9728)])
+                                 (2000, 256), (9000, 512), (1000, 9728), (1000, 2048),
+                                 (500, 4736), (500, 4864), (400, 4096), (900, 1792), (250, 18944),
+                                 (250, 19456), (18900, 256)])
 @pytest.mark.parametrize("act", ["gelu", "swiglu"])
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_act_backward_row_tiles(F, qlib, m, n, act, dt):
@@ -170,7 +173,7 @@ def test_act_backward_row_tiles(F, qlib, m, n, act, dt):
 
 # ------------------------------------------------------------------ transposition
 @pytest.mark.parametrize("rows,k", [(2500, 4128), (10001, 1056), (128, 75808), (75777, 128),
-                                    (9473, 1152)])
+                                    (9473, 1152), (4700, 1024), (4740, 1024)])
 @pytest.mark.parametrize("layout", [0, 1, 2])
 def test_transpose_many_tiles(F, qlib, rows, k, layout):
     base.test_transpose(F, qlib, rows, k, layout)

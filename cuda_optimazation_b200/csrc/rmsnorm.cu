@@ -442,7 +442,7 @@ __device__ __forceinline__ void column_dw(const RmsNormBwdParams& p, int64_t col
 
 // kColumns (few rows): the first CTAs take the columns of dw, which need no row's
 // sum, the others one row each: dy and h are read twice, the second time mostly
-// from L2, and nothing is left to join.  dx may not be dy then.
+// from L2 where they fit it, and nothing is left to join.  dx may not be dy then.
 // Otherwise CTA b takes rows b, b + grid, ...; each thread owns the same columns
 // of all of them, so its share of dw stays in registers and is written once, to
 // row b of the partial sums.
@@ -716,8 +716,12 @@ int backward_direct_grid(int64_t rows) {
   return static_cast<int>(rows < most ? rows : most);
 }
 
-// Few rows whose dy and h stay in L2: dw by columns (see the kernel).
-bool backward_by_columns(int64_t rows, int64_t k) { return rows <= 512 && rows * k <= 4 << 20; }
+// Few rows: dw by columns (see the kernel).  Measured against partial sums, us for bf16
+// with dres: 1 x 8192 3.1 / 5.3, 512 x 1024 3.7 / 5.5, 512 x 4096 7.1 / 11.7, 290 x 16384
+// 18.5 / 22.9, 512 x 32768 57.5 / 70.1 (fp32 90.8 / 129): ahead at every k.  Beyond 512
+// rows it depends on k: 2000 x 32 8.8 / 7.3, 2000 x 1024 13.8 / 14.4, 4000 x 1024 25.9 /
+// 24.6, 2048 x 32768 224 / 200.
+bool backward_by_columns(int64_t rows) { return rows <= 512; }
 
 template <bool kBf16, bool kWBf16, bool kColumns>
 cudaError_t launch_bwd_direct(const RmsNormBwdParams& p, int grid, cudaStream_t stream) {
@@ -740,7 +744,7 @@ cudaError_t launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
     e = r.stages == 3
             ? launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream)
             : launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 2>>(p, r, stream);
-  } else if (backward_by_columns(p.rows, p.k)) {
+  } else if (backward_by_columns(p.rows)) {
     const int64_t per = 128 / kElem<kBf16>, columns = p.dw ? (p.k + per - 1) / per : 0;
     return launch_bwd_direct<kBf16, kWBf16, true>(p, static_cast<int>(p.rows + columns), stream);
   } else {
@@ -761,7 +765,7 @@ cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
 }
 
 int rmsnorm_backward_parts(int64_t rows, int64_t k) {
-  int most = backward_by_columns(rows, k) ? 0 : backward_direct_grid(rows);
+  int most = backward_by_columns(rows) ? 0 : backward_direct_grid(rows);
   for (int64_t inputs = 2; inputs <= 3; ++inputs)
     for (int64_t elem = 2; elem <= 4; elem += 2) {
       const RingShape r = ring_shape(rows, k, k * elem * inputs);

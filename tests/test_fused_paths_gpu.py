@@ -199,3 +199,13 @@ def test_transpose_offsets_past_32_bits(F, qlib):
     # K-major chunks: a row block's last tail / 128 chunks.
     whole = t.block_scales.view(k // 128, rows // 128, 512)
     assert torch.equal(whole[:, -tail // 128:], s.block_scales.view(k // 128, tail // 128, 512))
+
+
+# ------------------------------------------------------------------ norm gradient
+# Up to 512 rows by columns, at every width (few rows or too wide for the ring); 513 and
+# 600: partial sums.
+@pytest.mark.parametrize("rows,k", [(512, 64), (513, 64), (290, 16384), (512, 16416), (200, 32768),
+                                    (512, 32768), (513, 32768), (600, 16416)])
+@pytest.mark.parametrize("xt,wt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+def test_norm_backward_rows(F, rows, k, xt, wt):
+    base.test_norm_backward(F, rows, k, xt, wt)

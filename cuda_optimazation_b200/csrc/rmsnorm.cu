@@ -21,8 +21,9 @@
 // own vectors of the next rows into shared memory ahead of time (cp.async, two
 // or three rows deep), so the bytes in flight do not depend on registers or
 // on where a CTA stands between its two barriers.  A thread reads back only
-// what it copied itself, so the ring needs no barrier.  Few rows, or rows too
-// long for the ring: one CTA per row, values straight to registers.
+// what it copied itself, so the ring needs no barrier.  Elsewhere (few rows, rows too
+// long for the ring, most fp32 rows): one CTA per row, values straight to registers;
+// the rules stand at the launches with what was measured on both sides.
 //
 // Measured, of the 6.51 TB/s that a copy reaches here: forward, 16384 x 8192 bf16 with
 // a residual, 152 us (6.2 TB/s); backward with dres 171 us (6.3 TB/s).  One row of
@@ -691,14 +692,30 @@ cudaError_t launch_ring(const P& p, const RingShape& s, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+// Where the ring is ahead of one CTA a row.  Measured, us ring / direct, with a residual:
+// bf16 4800 x 128 6.0 / 5.6, 7200 x 256 7.4 / 8.3, 9600 x 512 12.1 / 10.7, 16384 x 512
+// 15.8 / 17.9, 32768 x 1024 42.1 / 40.4; 16384 x 2048 41.2 / 41.0, 4800 x 4096 27.5 /
+// 25.6, 9600 x 4096 46.4 / 49.3, 1200 x 8192 18.8 / 15.7, 4800 x 8192 46.9 / 53.2, 1200 x
+// 16384 28.3 / 39.8; fp32 9600 x 128 10.1 / 10.7, 9600 x 256 13.0 / 10.8, 16384 x 4096
+// 221 / 129, 2400 x 12288 98 / 73: such rows take twice the ring for the same arithmetic,
+// and too few threads are left to keep up.
+bool forward_ring(int64_t rows, int64_t k, int64_t slot_bytes, bool bf16) {
+  if (k <= 1024) return slot_bytes <= 2048 && rows >= 6144 && rows >= 8 * slot_bytes;
+  return bf16 && (k > 12288 || rows * k * k >= 1ll << 37);
+}
+
 template <bool kBf16, bool kWBf16>
 cudaError_t launch_norm(const RmsNormParams& p, cudaStream_t stream) {
-  const RingShape r =
-      ring_shape(p.rows, p.k, p.k * kElem<kBf16> * (p.residual ? 2 : 1));
-  if (r.stages == 3)
-    return launch_ring<rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream);
-  if (r.stages == 2)
-    return launch_ring<rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 2>>(p, r, stream);
+  const int64_t slot = p.k * kElem<kBf16> * (p.residual ? 2 : 1);
+  if (forward_ring(p.rows, p.k, slot, kBf16)) {
+    const RingShape r = ring_shape(p.rows, p.k, slot);
+    if (r.stages == 3)
+      return launch_ring<rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream);
+    if constexpr (kBf16) {  // (fp32: short rows alone, of which three stages fit)
+      if (r.stages == 2)
+        return launch_ring<rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 2>>(p, r, stream);
+    }
+  }
   const RowShape s = row_shape(p.k, 1024);
   // Padding words of the last chunks, four per thread.
   int pads = 0;

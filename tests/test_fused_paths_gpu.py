@@ -201,6 +201,29 @@ def test_transpose_offsets_past_32_bits(F, qlib):
     assert torch.equal(whole[:, -tail // 128:], s.block_scales.view(k // 128, tail // 128, 512))
 
 
+# ------------------------------------------------------------------ norm
+# Both sides of the rule for the ring: short rows, eight to a CTA, by their bytes and
+# their number, and long ones by both or by k alone.
+@pytest.mark.parametrize("rows,k", [(6143, 64), (6145, 64), (8200, 128), (8200, 256), (16500, 512),
+                                    (16500, 1024), (9000, 32), (8100, 4096), (8200, 4096),
+                                    (2040, 8192), (2050, 8192), (301, 16384), (300, 12320)])
+@pytest.mark.parametrize("xt,wt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+def test_norm_paths(F, rows, k, xt, wt):
+    base.test_norm(F, rows, k, xt, wt)
+
+
+@pytest.mark.parametrize("rows,k", [(8193, 128), (8193, 256), (16500, 512), (16500, 1024),
+                                    (8200, 4096)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_norm_paths_without_a_residual(F, rows, k, dt):
+    x, w = base.rand(rows, k, seed=161, dtype=dt), base.rand(k, seed=162, dtype=dt)
+    o = F.rmsnorm_mxfp8(x, w, eps=1e-5, layout=k // 128 % 3)
+    _, rstd, y = R.norm(x, None, w, 1e-5)
+    assert o.h is x
+    base.close(o.rstd, rstd, 2.0 ** -16 * rstd)
+    R.check_mx(o.y, y, 2.0 ** -15 * y.abs())
+
+
 # ------------------------------------------------------------------ norm gradient
 # Up to 512 rows by columns, at every width (few rows or too wide for the ring); 513 and
 # 600: partial sums.

@@ -638,12 +638,11 @@ constexpr int kRingVec = 4;            // vectors of a row per thread
 // Ring kernels: rows of at most kRingVec x 512 vectors, one warp per row and
 // eight rows per CTA up to 1024 values.  Three slots a row group where two
 // such CTAs fit an SM, else two; none (stages 0) where a CTA does not fit or
-// the rows do not go round: with fewer than two rows per resident CTA nothing
-// would be prefetched.
+// the rows do not go `rounds` times round the resident CTAs.
 struct RingShape {
   int group = 0, rows = 0, stages = 0, smem = 0, grid = 0;
 };
-RingShape ring_shape(int64_t rows, int64_t k, int64_t slot_bytes) {
+RingShape ring_shape(int64_t rows, int64_t k, int64_t slot_bytes, int rounds) {
   RingShape s;
   const int64_t nvec = k / 8;
   if (nvec > 512 * kRingVec) return s;
@@ -656,7 +655,7 @@ RingShape ring_shape(int64_t rows, int64_t k, int64_t slot_bytes) {
   if (ctas < 1) ctas = 1;
   if (ctas > 512 / (s.group * s.rows)) ctas = 512 / (s.group * s.rows);  // 128 registers
   s.grid = static_cast<int>(ctas * num_sms());
-  if (rows < 2ll * s.grid * s.rows) return s;
+  if (rows < static_cast<int64_t>(rounds) * s.grid * s.rows) return s;
   s.stages = stages;
   s.smem = static_cast<int>(stages * slots);
   return s;
@@ -708,7 +707,7 @@ template <bool kBf16, bool kWBf16>
 cudaError_t launch_norm(const RmsNormParams& p, cudaStream_t stream) {
   const int64_t slot = p.k * kElem<kBf16> * (p.residual ? 2 : 1);
   if (forward_ring(p.rows, p.k, slot, kBf16)) {
-    const RingShape r = ring_shape(p.rows, p.k, slot);
+    const RingShape r = ring_shape(p.rows, p.k, slot, 2);  // (one round prefetches nothing)
     if (r.stages == 3)
       return launch_ring<rmsnorm_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream);
     if constexpr (kBf16) {  // (fp32: short rows alone, of which three stages fit)
@@ -733,43 +732,68 @@ int backward_direct_grid(int64_t rows) {
   return static_cast<int>(rows < most ? rows : most);
 }
 
-// Few rows: dw by columns (see the kernel).  Measured against partial sums, us for bf16
-// with dres: 1 x 8192 3.1 / 5.3, 512 x 1024 3.7 / 5.5, 512 x 4096 7.1 / 11.7, 290 x 16384
-// 18.5 / 22.9, 512 x 32768 57.5 / 70.1 (fp32 90.8 / 129): ahead at every k.  Beyond 512
-// rows it depends on k: 2000 x 32 8.8 / 7.3, 2000 x 1024 13.8 / 14.4, 4000 x 1024 25.9 /
-// 24.6, 2048 x 32768 224 / 200.
-bool backward_by_columns(int64_t rows) { return rows <= 512; }
+// Which gradient kernel; measured, us, with dres.
+// By columns (see the direct kernel) up to 512 rows; against partial sums bf16 1 x 8192
+// 3.1 / 5.3, 512 x 1024 3.7 / 5.5, 512 x 4096 7.1 / 11.7, 290 x 16384 18.5 / 22.9, 512 x
+// 32768 57.5 / 70.1, against the ring fp32 384 x 8192 14.9 / 22.5, 384 x 9376 22.8 / 24.9,
+// bf16 512 x 8192 12.2 / 15.2, but 384 x 16384 25.6 / 21.1.  Beyond 512 rows it depends on
+// k: 2000 x 32 8.8 / 7.3, 2000 x 1024 13.8 / 14.4, 4000 x 1024 25.9 / 24.6.
+// The ring against the direct kernel: bf16 2400 x 256 6.6 / 10.0, 1400 x 1280 10.9 / 12.2,
+// 520 x 6144 13.7 / 23.2, 4800 x 8192 58.7 / 107.7, in between from two rounds on (800 x
+// 2048 10.7 / 9.3, 1480 x 2048 12.9 / 13.1); fp32 2400 x 512 12.4 / 17.1, 3600 x 768 19.6 /
+// 24.8, 2400 x 1024 19.9 / 19.0, 4800 x 1024 28.5 / 32.3, 4800 x 1536 40.2 / 35.7, 4800 x
+// 8192 193 / 137, where two CTAs an SM find their rings (4096 is a direct thread's second
+// vector) 2400 x 4096 47 / 42, 4608 53 / 60, 5120 69 / 62, without dres 9600 x 2560 78 /
+// 63, 9600 x 4096 120 / 134, 9600 x 7168 203 / 224, 4800 x 8192 138 / 129, and where a
+// direct thread would hold four vectors 4800 x 9376 184 / 236.
+struct BackwardPlan {
+  RingShape ring;  // stages 0: none
+  bool columns = false;
+  int parts = 0;  // rows of partial sums of dw
+};
+BackwardPlan backward_plan(int64_t rows, int64_t k, int elem, int inputs) {
+  BackwardPlan p;
+  p.columns = rows <= 512;
+  if (p.columns && (elem == 4 || k <= 8192)) return p;
+  const bool f32_too = k <= 768 || (k <= 1280 && rows >= 2560) || k > 8192 ||
+                       (inputs == 2 ? k >= 3104 && k <= 7168 : k > 4096 && k <= 4608);
+  if (elem == 2 || f32_too)
+    p.ring = ring_shape(rows, k, k * elem * inputs,
+                        k <= 1536 || (k >= 3104 && k <= 8192) ? 1 : 2);
+  if (p.ring.stages) p.columns = false;
+  if (!p.columns) p.parts = p.ring.stages ? p.ring.grid : backward_direct_grid(rows);
+  return p;
+}
 
 template <bool kBf16, bool kWBf16, bool kColumns>
 cudaError_t launch_bwd_direct(const RmsNormBwdParams& p, int grid, cudaStream_t stream) {
   RowShape s = row_shape(p.k, 512);
   if (kColumns) s.threads = 512;
-  auto kernel = s.vec == 1   ? rmsnorm_backward_direct_kernel<kBf16, kWBf16, 1, kColumns>
-                : s.vec == 2 ? rmsnorm_backward_direct_kernel<kBf16, kWBf16, 2, kColumns>
-                : s.vec == 4 ? rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4, kColumns>
-                             : rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8, kColumns>;
+  auto kernel = rmsnorm_backward_direct_kernel<kBf16, kWBf16, 8, kColumns>;
+  if (s.vec == 1) kernel = rmsnorm_backward_direct_kernel<kBf16, kWBf16, 1, kColumns>;
+  if constexpr (!kBf16 || kColumns) {  // (bf16 rows of these widths take the ring)
+    if (s.vec == 2) kernel = rmsnorm_backward_direct_kernel<kBf16, kWBf16, 2, kColumns>;
+    if (s.vec == 4) kernel = rmsnorm_backward_direct_kernel<kBf16, kWBf16, 4, kColumns>;
+  }
   return launch_overlapped(kernel, dim3(grid), dim3(s.threads), 0, stream, 1, p);
 }
 
 template <bool kBf16, bool kWBf16>
 cudaError_t launch_norm_bwd(const RmsNormBwdParams& p, cudaStream_t stream) {
-  const RingShape r = ring_shape(p.rows, p.k, p.k * kElem<kBf16> * (p.dres ? 3 : 2));
-  int parts;
-  cudaError_t e;
-  if (r.stages) {
-    parts = r.grid;
-    e = r.stages == 3
-            ? launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream)
-            : launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 2>>(p, r, stream);
-  } else if (backward_by_columns(p.rows)) {
+  const BackwardPlan plan = backward_plan(p.rows, p.k, kElem<kBf16>, p.dres ? 3 : 2);
+  const RingShape& r = plan.ring;
+  if (plan.columns) {
     const int64_t per = 128 / kElem<kBf16>, columns = p.dw ? (p.k + per - 1) / per : 0;
     return launch_bwd_direct<kBf16, kWBf16, true>(p, static_cast<int>(p.rows + columns), stream);
-  } else {
-    parts = backward_direct_grid(p.rows);
-    e = launch_bwd_direct<kBf16, kWBf16, false>(p, parts, stream);
   }
+  const cudaError_t e =
+      r.stages == 3
+          ? launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 3>>(p, r, stream)
+      : r.stages == 2
+          ? launch_ring<rmsnorm_backward_ring_kernel<kBf16, kWBf16, kRingVec, 2>>(p, r, stream)
+          : launch_bwd_direct<kBf16, kWBf16, false>(p, plan.parts, stream);
   if (e != cudaSuccess || !p.dw) return e;
-  return launch_column_sum(p.dw_part, parts, p.k, p.dw, stream);
+  return launch_column_sum(p.dw_part, plan.parts, p.k, p.dw, stream);
 }
 
 }  // namespace
@@ -782,11 +806,11 @@ cudaError_t launch_rmsnorm_mxfp8(const RmsNormParams& p, bool bf16, bool w_bf16,
 }
 
 int rmsnorm_backward_parts(int64_t rows, int64_t k) {
-  int most = backward_by_columns(rows) ? 0 : backward_direct_grid(rows);
-  for (int64_t inputs = 2; inputs <= 3; ++inputs)
-    for (int64_t elem = 2; elem <= 4; elem += 2) {
-      const RingShape r = ring_shape(rows, k, k * elem * inputs);
-      if (r.stages && r.grid > most) most = r.grid;
+  int most = 0;
+  for (int inputs = 2; inputs <= 3; ++inputs)
+    for (int elem = 2; elem <= 4; elem += 2) {
+      const int parts = backward_plan(rows, k, elem, inputs).parts;
+      if (parts > most) most = parts;
     }
   return most;
 }

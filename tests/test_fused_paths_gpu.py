@@ -225,10 +225,14 @@ def test_norm_paths_without_a_residual(F, rows, k, dt):
 
 
 # ------------------------------------------------------------------ norm gradient
-# Up to 512 rows by columns, at every width (few rows or too wide for the ring); 513 and
-# 600: partial sums.
-@pytest.mark.parametrize("rows,k", [(512, 64), (513, 64), (290, 16384), (512, 16416), (200, 32768),
-                                    (512, 32768), (513, 32768), (600, 16416)])
+# Up to 512 rows by columns, or (long bf16 rows) through the ring; beyond by type, width
+# and number of rows through the ring or partial sums.
+@pytest.mark.parametrize("rows,k", [(512, 64), (513, 64), (290, 16384), (300, 16384), (512, 16416),
+                                    (200, 32768), (512, 32768), (513, 32768), (600, 16416),
+                                    (512, 9376), (513, 9376), (520, 6144), (600, 12288),
+                                    (2367, 256), (2368, 256), (2400, 768), (2400, 800),
+                                    (2559, 1024), (2560, 1280), (1300, 1536), (900, 2048),
+                                    (1500, 2048), (640, 3104), (900, 4128), (700, 7200)])
 @pytest.mark.parametrize("xt,wt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")])
 def test_norm_backward_rows(F, rows, k, xt, wt):
     base.test_norm_backward(F, rows, k, xt, wt)

@@ -19,15 +19,15 @@
 // lane's bytes of a row are 8 neighbours and those of a column 4, and no result
 // passes through shared memory.
 //
-// What bounds it is the instruction rate as much as HBM, so the work per element
-// is kept down: fp32 pairs in one instruction (f32x2), and block scales from the
-// upper halves of the peaks' fp32 patterns, two peaks to a register -- a scale
-// needs the exponent of its peak only, and the upper halves order as the
-// peaks do.
+// Issue slots are 66 % busy (gated) and DRAM 50 %: neither is full, and with 16 warps an
+// SM latency counts as well.  So the work per element is kept down: fp32 pairs in one
+// instruction (f32x2), and block scales from the upper halves of the peaks' fp32
+// patterns, two peaks to a register -- a scale needs the exponent of its peak only, and
+// the upper halves order as the peaks do.
 //
-// Measured: 4096 x 28672 gated, bf16, 105 us (4.6 TB/s; 73 M warp instructions, issue
-// slots 66 % busy with 16 warps an SM); 8192 x 14336 gelu 137 us bf16, 143 fp32
-// (5.8 TB/s); transposition of 16384 x 8192 49.7 us (5.6 TB/s; 58 while lanes
+// Measured: 4096 x 28672 gated, bf16, 106 us (4.5 TB/s; 73 M warp instructions); 8192 x
+// 14336 gelu 137 us bf16, relu 106, silu fp32 134 (6.2 TB/s); 1024 x 8192 gelu bf16 17;
+// 333 x 4128 gelu fp32 7.1; transposition of 16384 x 8192 49.7 us (5.6 TB/s; 58 while lanes
 // fetched 8 bytes of 8 rows: the L1's data stage was the limit).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

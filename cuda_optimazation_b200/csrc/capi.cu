@@ -229,9 +229,13 @@ int gemm_prepare(int fmt, const void* a_q, const void* a_sf, const float* a_ts, 
   const int variant = (gather.nranks > 0 || rq || epi || fmt == 2) ? 1 : gemm_variant(fp4, m);
   const bool pair = variant == 1;
   if (epi && m <= 128) {
-    // Few rows: the weights stream past them (gemm_fused_rows.cu).  Against the
-    // pair kernel, whose 256-row tile would be mostly empty: MXFP8 1 x 28672 x
-    // 4096 gated and 64 x 4096 x 14336 (see the kernel's file for the figures).
+    // Few rows: the weights stream past them (gemm_fused_rows.cu), where the pair
+    // kernel's 256-row tile would be mostly empty.  Measured, us against the pair kernel:
+    // MXFP8 1 x 4096 x 4096 7.1 / 19.4, 128 x 4096 x 4096 10.9 / 20.9, 64 x 4096 x 14336
+    // 16.7 / 47.6, 16 x 28672 x 4096 gated 21.7 / 38.0, 128 x 28672 x 4096 gated 34.1 / 36.3.
+    // With 64 to 128 rows of so many columns that the pairs are busy too it is up to 16 %
+    // behind: 128 x 14336 x 4096 26.6 / 24.3, 128 x 28672 x 1024 gated 19.9 / 17.2, NVFP4
+    // 64 x 28672 x 8192 gated 40.6 / 38.2.
     GemmParams& p = out->p;
     std::memset(&p, 0, sizeof(p));
     const int sets = epi->act == QG_ACT_SWIGLU ? 2 : 1;

@@ -18,11 +18,12 @@
 //
 // Roles (8 warps): warp 0 TMA producer, warp 1 MMA issuer (and TMEM owner),
 // warps 2..5 read the accumulator (one TMEM lane quadrant each); all eight finish
-// rows.  Every wait is bounded (qg_ptx.cuh).
+// rows.  Every mbarrier wait is bounded (qg_ptx.cuh), so the cluster's barriers are reached.
 //
 // Measured (MXFP8): one token, 2 x 14336 x 4096 gated, 21.2 us (5.7 TB/s), x 8192
-// 37.5 (6.45 TB/s, the rate of a copy); 64 x 4096 x 14336 16.6 us, of which about 6
-// are start, exchange and end.  NVFP4 16 x 28672 x 8192 24.6 us.
+// 37.5 (6.45 TB/s, the rate of a copy); 64 x 4096 x 14336 16.5 us, of which about 6
+// are start, exchange and end.  NVFP4 16 x 28672 x 8192 24.8 us.  Against the pair kernel:
+// at the rule that chooses between them, in capi.cu.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

@@ -91,9 +91,10 @@ __device__ __forceinline__ Raw8<kBf16> load_kept(const void* base, int64_t elem)
   return r;
 }
 
-// Streaming stores, as for the values below: left to L2's own order the forward pass
-// over 16384 x 8192 took 168 us at full clocks and 157 under the power cap, streamed
-// 152 and 161.
+// bf16 rows by streaming stores, as the values below: left to L2's own order the forward
+// pass over 16384 x 8192 took 168 us at full clocks and 157 under the power cap, streamed
+// 152 and 161.  fp32 by plain ones: dw's shares, some in shared memory, are stored here too
+// and read again at once.
 template <bool kBf16>
 __device__ __forceinline__ void store8(void* base, int64_t elem, const Vec8& x) {
   uint4* p = reinterpret_cast<uint4*>(static_cast<uint8_t*>(base) + elem * kElem<kBf16>);
@@ -113,15 +114,14 @@ __device__ __forceinline__ void store8(void* base, int64_t elem, const Vec8& x) 
   }
 }
 
-// One input's row in a ring slot: 16-byte chunks, the first chunks of all
-// vectors and then (fp32) the second ones, so that a warp's accesses are
-// contiguous.
 template <bool kBf16>
 __device__ __forceinline__ const uint8_t* at_row(const void* base, int64_t row, int64_t ld) {
   return static_cast<const uint8_t*>(base) + row * ld * kElem<kBf16>;
 }
-// `slot`, `at`: 32-bit shared-memory addresses; `second`: bytes from a vector's first
-// chunk to its second.
+// One input's row in a ring slot: 16-byte chunks, the first chunks of all
+// vectors and then (fp32) the second ones, so that a warp's accesses are
+// contiguous.  `at`: 32-bit shared-memory address; `second`: bytes from a vector's
+// first chunk to its second.
 template <bool kBf16>
 __device__ __forceinline__ void ring_copy(uint32_t at, const uint8_t* from, uint32_t second) {
 #pragma unroll

@@ -22,6 +22,11 @@ namespace qg {
 
 namespace {
 
+// An output over an input: elements lie on their own only with one stride (that of a
+// single row is no matter).
+bool shifted(const void* out, int64_t ldo, const void* in, int64_t ldi, int64_t rows) {
+  return in && out == in && rows > 1 && ldo != ldi;
+}
 bool float_dtype(int d) { return d == QG_DTYPE_F32 || d == QG_DTYPE_BF16; }
 int64_t dtype_bytes(int d) { return d == QG_DTYPE_BF16 ? 2 : 4; }
 bool any_layout(int l) { return l >= QG_LAYOUT_REF_LINEAR && l <= QG_LAYOUT_MMA_KMAJOR; }
@@ -616,6 +621,7 @@ int qg_rmsnorm_mxfp8(const void* x, int x_dtype, int64_t ldx, const void* residu
       (h && !vector_rows(h, ldh, x_dtype)) || !aligned16(weight) || !aligned16(q) ||
       !aligned_to(sf, 4) || !aligned_to(rstd, 4))
     return QG_ERR_ALIGN;
+  if (shifted(h, ldh, x, ldx, rows) || shifted(h, ldh, residual, ldr, rows)) return QG_ERR_ARG;
   if (int d = check_device()) return d;
   RmsNormParams p{};
   p.x = x;
@@ -660,6 +666,7 @@ int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh
       !vector_rows(dx, lddx, x_dtype) || (dres && !vector_rows(dres, lddres, x_dtype)) ||
       !aligned16(weight) || !aligned_to(rstd, 4) || !aligned_to(dweight, 4))
     return QG_ERR_ALIGN;
+  if (shifted(dx, lddx, dres, lddres, rows)) return QG_ERR_ARG;
   if (dweight) {
     const size_t need = qg_rmsnorm_backward_workspace_bytes(rows, k);
     if (need && (!workspace || workspace_bytes < need)) return QG_ERR_ARG;
@@ -713,6 +720,9 @@ int qg_gemm_fused(int format, const void* a_q, const void* a_sf, const float* a_
       (u.bias && !aligned_to(u.bias, dtype_bytes(u.bias_dtype))) ||
       (u.residual && !aligned_to(u.residual, dtype_bytes(u.residual_dtype))))
     return QG_ERR_ALIGN;
+  if (u.residual == u.out && (u.residual_dtype != u.out_dtype ||
+                              shifted(u.out, u.ldc, u.residual, u.ldr, m)))
+    return QG_ERR_ARG;
   EpiParams e{};
   e.act = u.act;
   e.bias = u.bias;

@@ -284,7 +284,7 @@ size_t qg_gemm_nvfp4_skinny_workspace_bytes(int64_t m, int64_t n, int64_t k);
  * (layout as there; scale padding of the MMA layouts is written as zero).
  * x, residual and h have x_dtype, weight (k values) w_dtype.  h (the sum,
  * rounded to x_dtype; y is formed from the unrounded sum) and rstd (rows
- * floats) may be NULL.  h may be x or residual itself.
+ * floats) may be NULL.  h may be x or residual itself, with its row stride.
  * k % 32 == 0, 32 <= k <= 32768, eps >= 0. */
 int qg_rmsnorm_mxfp8(const void* x, int x_dtype, int64_t ldx, const void* residual, int64_t ldr,
                      const void* weight, int w_dtype, float eps, int64_t rows, int64_t k,
@@ -296,7 +296,7 @@ int qg_rmsnorm_mxfp8(const void* x, int x_dtype, int64_t ldx, const void* residu
  *   dx = rstd * (g - xh * mean(g * xh)) + dres,   dweight = sum_rows dy * xh.
  * dy, h, dres (NULL: none) and dx have x_dtype; dx is the gradient of x and of
  * the residual alike.  dweight (k floats) may be NULL, and workspace with it.
- * dx may be dres itself, but not dy or h.  Deterministic: sums run in a fixed
+ * dx may be dres itself, with its row stride, but not dy or h.  Deterministic: sums run in a fixed
  * order. */
 int qg_rmsnorm_backward(const void* dy, int64_t lddy, const void* h, int64_t ldh, int x_dtype,
                         const float* rstd, const void* weight, int w_dtype, const void* dres,
@@ -325,7 +325,7 @@ typedef enum {
  * their scales in out_layout (ldc unused).  ckpt_q (NULL: none) and ckpt_sf
  * receive z in MXFP8 (m x n, ckpt_layout, n % 32 == 0), for
  * qg_act_backward_mxfp8.  MXFP8 buffers are 16-byte aligned.  residual may be
- * out itself. */
+ * out itself, of the same type and row stride. */
 typedef struct {
   int act; /* qg_act */
   int bias_dtype;

@@ -4,18 +4,17 @@
     python bench.py [--gpus N] [--steps K] [--warmup W] [--impl ours|reference]
                     [--workload auto|colpar|nvfp4_8192|...] [--no-subrecords]
 
-Headline workload (every N, BASELINE configs[4]): the column-parallel NVFP4
+Headline workload (every N): the column-parallel NVFP4
 GEMM M=16384, N=53248, K=8192.  B is quantised once and sharded along N over
 the ranks (colpar.shard_rows of one K-major operand), A is quantised once and
 broadcast, every rank runs its local GEMM with no communication; at N = 1 the
 one rank owns all of B.  The output gather (NCCL, and fused into the GEMM
 epilogue over peer memory) is timed separately at N > 1.
 
-At N = 1 the line also carries `subrecords` for the other BASELINE configs,
-each with its own steps, ms, roofline and clocks: NVFP4 8192^3,
-the same GEMM with NVFP4 output (the tc6 row), MXFP4 8192^3, MXFP8
-4096x14336x4096 and the decode GEMM at m = 16, 64, 128
-(configs[3]).
+At N = 1 the line also carries `subrecords` for the other workloads, each
+with its own steps, ms, roofline and clocks: NVFP4 8192^3, the same GEMM
+with NVFP4 output (the tc6 row), MXFP4 8192^3, MXFP8 4096x14336x4096 and
+the decode GEMM at m = 16, 64, 128.
 
 A "step" is one GEMM launch over one problem whose quantised operands are
 already resident in HBM.  `value` is whole-job TFLOP/s (all ranks' FLOPs over
@@ -51,7 +50,7 @@ WORKLOADS = {
     "mxfp4_8192": dict(fmt="mxfp4", m=8192, n=8192, k=8192, out="bf16", cfg=1),
     "nvfp4_256": dict(fmt="nvfp4", m=256, n=256, k=256, out="fp32", cfg=0),
     "mxfp8_ffn": dict(fmt="mxfp8", m=4096, n=14336, k=4096, out="bf16", cfg=2),
-    # decode GEMM with fused activation quantisation (configs[3]); HBM bound
+    # decode GEMM with fused activation quantisation; HBM bound
     "skinny_m16": dict(fmt="nvfp4", m=16, n=28672, k=8192, out="bf16", cfg=3, skinny=True),
     "skinny_m64": dict(fmt="nvfp4", m=64, n=28672, k=8192, out="bf16", cfg=3, skinny=True),
     "skinny_m128": dict(fmt="nvfp4", m=128, n=28672, k=8192, out="bf16", cfg=3, skinny=True),
@@ -275,7 +274,7 @@ def timed(torch, stream, fn, steps, dist=None):
 def run_gemm(args, name, w, rank, world, dist, torch, steps, headline=True):
     """One GEMM workload: operands quantised on the device (untimed), the
     timed region, and for the headline the e2e leg, the gather legs (N > 1)
-    and the sample the CPU checker compares against."""
+    and the sample the CPU oracle compares against."""
     from cuda_optimazation_b200 import colpar as cp
     from cuda_optimazation_b200 import qgemm as q
     dev = torch.device("cuda", int(os.environ.get("LOCAL_RANK", 0)))
@@ -309,7 +308,7 @@ def run_gemm(args, name, w, rank, world, dist, torch, steps, headline=True):
         B_full = quant(xb)
         B = cp.shard_rows(B_full, lo, hi) if is_colpar else B_full
         if s == 0 and headline and w["fmt"] == "nvfp4" and not requant and world == 1:
-            # What the CPU checker needs (N = 1 only): the fp32 sample rows
+            # What the CPU oracle needs (N = 1 only): the fp32 sample rows
             # of A and of B (= output columns), the tensors' amax, and the
             # quantised bytes of those rows.
             ri = torch.tensor(rows_s, device=dev)
@@ -415,7 +414,7 @@ def run_gemm(args, name, w, rank, world, dist, torch, steps, headline=True):
                          flops_job, world)
     rec["_check"] = check
     if check is not None:
-        step(0)  # C holds set 0's product for the checker
+        step(0)  # C holds set 0's product for the oracle
         torch.cuda.synchronize()
         ri = torch.tensor(check["rows"], device=dev)
         ci = torch.tensor(check["cols"], device=dev)
@@ -553,7 +552,7 @@ def e2e_leg(args, torch, dist, q, cp, w, dev, stream, m, n, k, b_std, layout, fl
 
 
 def run_skinny(args, name, w, rank, world, dist, torch, steps, headline=True):
-    """Decode GEMM: bf16 activations with 0.1% outliers
+    """Decode GEMM (m x 28672 x 8192): bf16 activations with 0.1% outliers
     x50, pre-quantised NVFP4 weights N(0, 0.02); one step = one
     qg_gemm_nvfp4_skinny call (activation amax pass, quantiser, and the
     stream-K GEMM with its scale/convert epilogue: three launches, the last
@@ -790,7 +789,7 @@ def cpu_baseline(w, budget_s: float = 20.0) -> dict:
 
 
 def cpu_check(chk: dict) -> dict:
-    """The CPU checker on the headline GEMM (rank 0, N = 1): the tensor
+    """The CPU oracle on the headline GEMM (rank 0, N = 1): the tensor
     scales against amax/(448*6) (GEMMsm110/include/requant/nvfp4_reference.cuh:66-74),
     the quantised bytes of the sampled rows of A and B against O1's block
     rule under them (nvfp4_reference.cuh:84-111), and the GPU output on the

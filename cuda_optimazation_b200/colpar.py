@@ -1,8 +1,8 @@
 """Column-parallel (N-sharded) block-scaled GEMM over several GPUs of one box.
 
-The reference is single-GPU; BASELINE config 5 asks for the quant GEMM
-C = A . B^T at M = 16384, N = 53248, K = 8192 sharded along N over 1/2/4/8
-B200s.  The scheme:
+The reference is single-GPU; here the quant GEMM C = A . B^T (benchmarked at
+M = 16384, N = 53248, K = 8192) is sharded along N over 1/2/4/8 B200s.  The
+scheme:
 
 * rank r owns B rows ``shard_range(N, world, r)`` and their scale rows
   (weights are sharded once, at load time);

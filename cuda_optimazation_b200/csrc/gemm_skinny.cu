@@ -5,9 +5,8 @@
 // C^T = W . X^T so the weight rows fill the tensor core's M = 128 side and the
 // activation rows its N side (16 / 32 / 64 / 128).  The reference has no
 // kernel for this shape (its harness only runs square problems,
-// GEMMquant_sm110/src/quant_gemm_bench.cu:3038-3079); BASELINE config 4 names
-// it.  The weights are streamed once from HBM.  Work is (weight-tile,
-// K-block) units: every CTA owns floor(T / G) whole tiles, and the units of
+// GEMMquant_sm110/src/quant_gemm_bench.cu:3038-3079).  The weights are
+// streamed once from HBM.  Work is (weight-tile, K-block) units: every CTA owns floor(T / G) whole tiles, and the units of
 // the remaining T mod G tiles are spread evenly over all CTAs (stream-K), so
 // the 224 x 16 units of N = 28672, K = 8192 split into one whole tile plus
 // ~8 units per CTA on 148 SMs.  A tile that one CTA owns is scaled and

@@ -12,8 +12,7 @@
 // m <= 64.  The decode configuration's weight stream is bound by the bytes a
 // CTA has in flight, so fewer activation bytes per stage are more weight
 // bytes per SM.  The reference has no kernel for this shape (its harness only
-// runs square problems, GEMMquant_sm110/src/quant_gemm_bench.cu:3038-3079);
-// BASELINE config 4 names it.
+// runs square problems, GEMMquant_sm110/src/quant_gemm_bench.cu:3038-3079).
 //
 // Work: pair p owns weight rows [512 p, 512 p + 512): CTA rank r holds rows
 // 512 p + 256 h + 128 r + [0, 128) of half h.  Every pair streams its tile's

@@ -29,7 +29,7 @@
 // quantised on the device by the library.  The check recomputes sampled
 // output rows on the host from the quantised operands the device produced
 // (double accumulation, as guide::block_scaled_reference_mnk does) and
-// applies the north-star tolerance: relative Frobenius error <= 1e-5 and
+// applies this tolerance: relative Frobenius error <= 1e-5 and
 // |err| <= 1e-3 * ||row||_2 for fp32 output, plus the bf16 rounding bound
 // for bf16 output.
 #include <cublasLt.h>
@@ -402,7 +402,7 @@ Row run_skinny(const Options& o) {
 }
 
 // Column-parallel NVFP4 GEMM over the first P GPUs of this process
-// (nvfp4_colpar_q0; BASELINE config 5, M=16384 N=53248 K=8192 at P = 1..8).
+// (nvfp4_colpar_q0; M=16384 N=53248 K=8192 at P = 1..8).
 // A and B are quantised once on GPU 0 (one tensor scale each, K-major scale
 // chunks so a run of whole 128-row blocks is contiguous); GPU r receives A
 // and the B rows [lo_r, hi_r) (256-row aligned, the split of

@@ -380,11 +380,10 @@ int qg_transpose_mxfp8(const void* q, const void* sf, int layout, int64_t rows, 
                        void* tq, void* tsf, int out_layout, qg_stream_t stream);
 
 /* ---- Column-parallel GEMM with the output all-gather fused in ----------
- * BASELINE config 5 shards B along N over the GPUs of one box
- * (GEMMquant_sm110 itself is single-GPU; the north star asks for the N-sharded
- * split with an optional output all-gather).  Instead of a GEMM followed by
- * a collective, the CTA-pair GEMM's epilogue TMA-stores every output box
- * into the C buffer of EVERY rank, so the NVLink transfer overlaps the math
+ * B sharded along N over the GPUs of one box (GEMMquant_sm110 itself is
+ * single-GPU), with an optional all-gather of the output.  Instead of a GEMM
+ * followed by a collective, the CTA-pair GEMM's epilogue TMA-stores every
+ * output box into the C buffer of EVERY rank, so the NVLink transfer overlaps the math
  * tile by tile.
  *
  * c_ranks[r] (r < nranks <= QG_MAX_RANKS) is rank r's full bf16 C (m rows,

@@ -1,4 +1,4 @@
-"""ctypes view of the CPU parity checker (TEST INFRASTRUCTURE ONLY).
+"""ctypes view of the CPU oracle (TEST INFRASTRUCTURE ONLY).
 
 Loads oracle/_build/libqg_oracle.so (this repo's restatement, qg_oracle.cpp)
 and, when present, oracle/_ref/libqg_ref.so (the reference's own host headers

@@ -1,6 +1,6 @@
 // qg_oracle.cpp -- CPU restatement of the reference's block-scaled GEMM path.
 //
-// TEST INFRASTRUCTURE ONLY.  This file is the parity checker for the CUDA
+// TEST INFRASTRUCTURE ONLY.  This file is the oracle for the CUDA
 // library in cuda_optimazation_b200/.  Only tests/, __graft_entry__.smoke() and
 // bench.py's cpu_baseline / --impl reference legs may load it.  The product
 // never links, imports or calls anything built from here.
